@@ -30,6 +30,7 @@ SHARD_WAIT_PREV = 1
 SHARD_NO_SIGNAL = 2
 SHARD_PAD_WORDS = 16
 IPC_HANDLE_BYTES = 64
+MAX_TOP_K = 32
 HOST_IO = X_HOST | Y_HOST
 
 _P = ctypes.c_void_p
@@ -79,6 +80,14 @@ SIGNATURES = {
     "cllm_cuda_rope_table": (_I, [ctypes.c_float, _I, _I, _P]),
     "cllm_cuda_rope_kv": (_I, [_P, _P, _P, _I, _I, _I, _I, _P, _I, _P, _P, _P]),
     "cllm_cuda_attention": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P]),
+    "cllm_cuda_kv4_page_bytes": (_I64, [_I, _I, _I]),
+    "cllm_cuda_kv4_append": (_I, [_P, _I64, _P, _P, _P, _I64, _I, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _I, _I,
+                                  _P, _P, _P]),
+    "cllm_cuda_kv4_attention": (_I, [_P, _I64, _P, _I, _I, _P, _I, _I, _I, _I, _P, _P, _I, _I, ctypes.c_float, _P, _P,
+                                     _P]),
+    "cllm_cuda_kv4_fork": (_I, [_P, _I, _I, _I64, _I, _P, _P, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "cllm_cuda_kv4_compact": (_I, [_P, _I, _I, _I64, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "cllm_cuda_token_scores": (_I, [_P, _I64, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P]),
     "cllm_cuda_check_device_status": (_I, []),
     "cllm_cuda_last_error": (_I, [ctypes.c_char_p, _SZ]),
 }

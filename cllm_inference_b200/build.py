@@ -73,15 +73,31 @@ def _run(cmd, verbose):
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> None:
     os.makedirs(LIB, exist_ok=True)
-    deps = _sources(CSRC) + [os.path.join(INCLUDE, "cllm_cuda.h")]
-    if force or ptxas_info or _stale(CUDA_SO, deps):
-        digest = _digest(deps)  # of the sources as compiled
-        cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
-               "-o", CUDA_SO, os.path.join(CSRC, "cllm_cuda.cu")]
-        if ptxas_info:
-            cmd[1:1] = ["-Xptxas", "-v"]
-        _run(cmd, verbose)
-        _mark(CUDA_SO, deps, digest)
+    header = os.path.join(INCLUDE, "cllm_cuda.h")
+    common = [os.path.join(CSRC, f) for f in ("common.cuh", "host.h")] + [header]
+    units = {  # object -> (source, what it is built from)
+        "cllm_cuda": (os.path.join(CSRC, "cllm_cuda.cu"), _sources(CSRC) + [header]),
+        "serve": (os.path.join(CSRC, "serve", "serve.cu"), _sources(os.path.join(CSRC, "serve")) + common),
+    }
+    jobs = []
+    for name, (src, deps) in units.items():
+        obj = os.path.join(LIB, name + ".o")
+        if force or ptxas_info or _stale(obj, deps):
+            cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-c", "-o", obj, src]
+            if ptxas_info:
+                cmd[1:1] = ["-Xptxas", "-v"]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            jobs.append((subprocess.Popen(cmd), cmd, obj, deps, _digest(deps)))  # of the sources as compiled
+    for proc, cmd, obj, deps, digest in jobs:  # the units compile side by side
+        if proc.wait():
+            raise subprocess.CalledProcessError(proc.returncode, cmd)
+        _mark(obj, deps, digest)
+    objs = [os.path.join(LIB, name + ".o") for name in units]
+    if force or ptxas_info or _stale(CUDA_SO, objs):
+        digest = _digest(objs)
+        _run([NVCC, *ARCH, "-Xcompiler", "-fPIC", "-shared", "-o", CUDA_SO, *objs], verbose)
+        _mark(CUDA_SO, objs, digest)
     shim_dir = os.path.join(CSRC, "shim")
     shim_deps = _sources(shim_dir, os.path.join(shim_dir, "cllm", "core")) + [CUDA_SO]
     if os.path.exists(os.path.join(shim_dir, "quant_shim.cpp")):

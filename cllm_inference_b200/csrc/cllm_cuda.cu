@@ -26,6 +26,7 @@
 #include "common.cuh"
 #include "dequant.cuh"
 #include "fallback.cuh"
+#include "host.h"
 #include "gemm_tc.cuh"
 #include "gemm_tc_q6k.cuh"
 #include "gemv.cuh"
@@ -1526,15 +1527,43 @@ int cllm_cuda_shard_barrier(uint32_t* const* signal_pads, uint32_t* epoch, int w
 
 int cllm_cuda_check_device_status(void) {
     CLLM_CUDA_TRY(cudaDeviceSynchronize());
-    int status = 0, zero = 0;
+    int status = 0, serve = 0, zero = 0;
     CLLM_CUDA_TRY(cudaMemcpyFromSymbol(&status, g_device_status, sizeof(int)));
     CLLM_CUDA_TRY(cudaMemcpyToSymbol(g_device_status, &zero, sizeof(int)));
-    if (status == kStatusTimeout)
+    if (int rc = serve_take_status(&serve)) return rc;
+    if (status == kStatusTimeout || (serve & kServeTimeout))
         return fail(CLLM_ERR_KERNEL_TIMEOUT, "a kernel's bounded wait expired (pipeline copy never landed)");
+    if (serve & kServeBadPage)
+        return fail(CLLM_ERR_INVALID_ARG, "a page table names a page or a position outside the cache");
     return CLLM_OK;
 }
 
 }  // extern "C"
+
+// ---- what the library's other translation units share (host.h) -------------
+namespace cllm {
+
+int host_fail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    g_last_error = buf;
+    return code;
+}
+
+int host_device(int* dev, int* sms) {
+    if (int rc = ensure_device(dev)) return rc;
+    *sms = g_dev[*dev].sms;
+    return CLLM_OK;
+}
+
+int host_workspace(int dev, size_t bytes, uint8_t** out, std::unique_lock<std::mutex>& lk) {
+    return workspace(dev, bytes, out, lk);
+}
+
+}  // namespace cllm
 
 // The device-resident engine step (its own C ABI section of include/cllm_cuda.h).
 #include "engine.cuh"

@@ -1,0 +1,218 @@
+// C ABI of the serving operators (include/cllm_cuda.h, "Serving many
+// sequences"): argument checks, workspace layout and launches.  A translation
+// unit of its own beside cllm_cuda.cu, whose host services it uses (host.h).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "kv4_append.cuh"
+#include "kv4_attention.cuh"
+#include "kv4_format.cuh"
+#include "kv4_pages.cuh"
+#include "scores.cuh"
+
+namespace cllm {
+
+int serve_take_status(int* bits) {
+    int zero = 0;
+    CLLM_HOST_TRY(cudaMemcpyFromSymbol(bits, serve::g_serve_status, sizeof(int)));
+    CLLM_HOST_TRY(cudaMemcpyToSymbol(serve::g_serve_status, &zero, sizeof(int)));
+    return CLLM_OK;
+}
+
+namespace serve {
+namespace {
+
+size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check_geometry(const char* who, int n_pages, int page_len, int n_head_kv, int head_dim) {
+    if (head_dim != 64 && head_dim != 128)
+        return host_fail(CLLM_ERR_INVALID_ARG, "%s: head_dim %d (64 or 128)", who, head_dim);
+    if (page_len <= 0 || page_len % kTile || page_len > 4096)
+        return host_fail(CLLM_ERR_INVALID_ARG, "%s: page_len %d (a multiple of 16, at most 4096)", who, page_len);
+    if (n_head_kv <= 0 || n_head_kv > 65535 || n_pages <= 0)
+        return host_fail(CLLM_ERR_INVALID_ARG, "%s: bad arguments (%d KV heads, %d pages)", who, n_head_kv, n_pages);
+    return CLLM_OK;
+}
+
+}  // namespace
+}  // namespace serve
+}  // namespace cllm
+
+using namespace cllm;
+using namespace cllm::serve;
+
+extern "C" {
+
+int64_t cllm_cuda_kv4_page_bytes(int page_len, int n_head_kv, int head_dim) {
+    if ((head_dim != 64 && head_dim != 128) || page_len <= 0 || page_len % kTile || page_len > 4096 || n_head_kv <= 0)
+        return 0;
+    return (int64_t)page_len / kTile * n_head_kv * (20 * head_dim);
+}
+
+int cllm_cuda_kv4_append(const float* q, int64_t ldq, float* q_out, const float* k, const float* v, int64_t ldkv,
+                         int n_tok, int n_head, const float* rope_table, int n_pos, const int* token_seq,
+                         const int* token_pos, void* pages, int n_pages, int page_len, int n_head_kv, int head_dim,
+                         const int* page_table, int n_seqs, int max_pages, float* k_out, float* v_out, void* stream) {
+    if (int rc = check_geometry("kv4_append", n_pages, page_len, n_head_kv, head_dim)) return rc;
+    if (n_tok < 0 || n_head < 0 || n_seqs <= 0 || max_pages <= 0 || (rope_table && n_pos <= 0))
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_append: bad sizes");
+    if (n_tok == 0) return CLLM_OK;
+    if (!k || !v || !token_seq || !token_pos || !pages || !page_table || (n_head > 0 && (!q || !q_out)))
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_append: null argument");
+    if (!aligned16(pages)) return host_fail(CLLM_ERR_INVALID_ARG, "kv4_append: pages must be 16-byte aligned");
+    if (ldkv < (int64_t)n_head_kv * head_dim || (n_head > 0 && ldq < (int64_t)n_head * head_dim))
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_append: a row is shorter than its heads");
+    if (n_head > 0 && q_out == q && ldq != (int64_t)n_head * head_dim)
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_append: q in place needs dense rows");
+    int dev, sms;
+    if (int rc = host_device(&dev, &sms)) return rc;
+    AppendArgs a{};
+    a.q = q; a.k = k; a.v = v; a.rope = rope_table;
+    a.q_out = q_out; a.k_out = k_out; a.v_out = v_out;
+    a.ldq = ldq; a.ldkv = ldkv;
+    a.token_seq = token_seq; a.token_pos = token_pos;
+    a.n_tok = n_tok; a.n_head = n_head; a.n_pos = n_pos;
+    a.vec = aligned16(q) && aligned16(q_out) && aligned16(k) && aligned16(v) && aligned16(k_out) && aligned16(v_out) &&
+            ldkv % 4 == 0 && (n_head == 0 || ldq % 4 == 0);
+    a.c = Cache{static_cast<uint8_t*>(pages), page_table, nullptr, n_pages, page_len, n_head_kv, n_seqs, max_pages};
+    const int64_t units = (int64_t)n_tok * (n_head + 2 * n_head_kv), per_cta = kAppendThreads / (head_dim / 4);
+    const int64_t ctas = (units + per_cta - 1) / per_cta;
+    if (ctas > INT_MAX) return host_fail(CLLM_ERR_TOO_LARGE, "kv4_append: too many tokens in one call");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (head_dim == 128) kv4_append_kernel<128><<<(unsigned)ctas, kAppendThreads, 0, st>>>(a);
+    else kv4_append_kernel<64><<<(unsigned)ctas, kAppendThreads, 0, st>>>(a);
+    CLLM_HOST_TRY(cudaGetLastError());
+    return CLLM_OK;
+}
+
+int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int n_tok, int n_head, const void* pages,
+                            int n_pages, int page_len, int n_head_kv, int head_dim, const int* page_table,
+                            const int* seq_len, int n_seqs, int max_pages, float scale, float* out, float* lse,
+                            void* stream) {
+    if (int rc = check_geometry("kv4_attention", n_pages, page_len, n_head_kv, head_dim)) return rc;
+    if (n_tok < 0 || n_head <= 0 || n_head % n_head_kv || n_seqs <= 0 || max_pages <= 0 ||
+        (int64_t)max_pages * page_len > INT_MAX || !(std::fabs(scale) <= 3e38f))
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: bad sizes (%d heads over %d KV heads)", n_head, n_head_kv);
+    if (!q_begin && n_tok != n_seqs)
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: %d rows for %d sequences need q_begin", n_tok, n_seqs);
+    if (n_tok == 0) return CLLM_OK;
+    if (!q || !pages || !page_table || !seq_len || !out)
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: null argument");
+    if (!aligned16(pages)) return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: pages must be 16-byte aligned");
+    if (ldq < (int64_t)n_head * head_dim)
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: a row is shorter than its heads");
+    int dev, sms;
+    if (int rc = host_device(&dev, &sms)) return rc;
+    AttnArgs a{};
+    a.q = q; a.ldq = ldq; a.q_begin = q_begin; a.n_tok = n_tok; a.n_head = n_head;
+    a.scale = scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale;
+    a.out = out; a.lse = lse;
+    a.c = Cache{const_cast<uint8_t*>(static_cast<const uint8_t*>(pages)), page_table, seq_len, n_pages, page_len,
+                n_head_kv, n_seqs, max_pages};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const dim3 grid(n_tok, (n_head + 3) / 4);
+    if (head_dim == 128) kv4_attention_kernel<128><<<grid, 128, 0, st>>>(a);
+    else kv4_attention_kernel<64><<<grid, 128, 0, st>>>(a);
+    CLLM_HOST_TRY(cudaGetLastError());
+    return CLLM_OK;
+}
+
+static int pages_call(const char* who, PagesArgs a, void* pages, int64_t page_bytes, bool fork, void* stream) {
+    if (a.n_layers <= 0 || a.n_pages <= 0 || a.page_len <= 0 || a.page_len % kTile || a.max_pages <= 0 ||
+        page_bytes <= 0 || page_bytes % 16 || (int64_t)a.max_pages * a.page_len > INT_MAX)
+        return host_fail(CLLM_ERR_INVALID_ARG, "%s: bad sizes", who);
+    if (!aligned16(pages)) return host_fail(CLLM_ERR_INVALID_ARG, "%s: pages must be 16-byte aligned", who);
+    int dev, sms;
+    if (int rc = host_device(&dev, &sms)) return rc;
+    a.pages = static_cast<uint8_t*>(pages);
+    a.page_bytes = page_bytes;
+    const size_t words = ((size_t)a.n_pages + 31) / 32, n = (size_t)a.n_pages;
+    const size_t bits = align256(4 * words), list = align256(4 * n), pairs = align256(8 * n);
+    const size_t seqs = align256(4 * (size_t)a.n_new);
+    uint8_t* ws;
+    std::unique_lock<std::mutex> lk;
+    if (int rc = host_workspace(dev, 2 * bits + 3 * list + pairs + 2 * seqs + 256, &ws, lk)) return rc;
+    auto take = [&](size_t bytes) {
+        uint8_t* p = ws;
+        ws += bytes;
+        return p;
+    };
+    uint8_t* ones = ws;
+    a.free_bits = reinterpret_cast<uint32_t*>(take(bits));
+    a.part_bits = reinterpret_cast<uint32_t*>(take(bits));
+    a.owner = reinterpret_cast<uint32_t*>(take(list));
+    a.ids = reinterpret_cast<int*>(take(list));
+    a.moved = reinterpret_cast<int*>(take(list));
+    a.copies = reinterpret_cast<int2*>(take(pairs));
+    a.first = reinterpret_cast<int*>(take(seqs));
+    a.held = reinterpret_cast<int*>(take(seqs));
+    a.count = reinterpret_cast<int*>(take(256));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    CLLM_HOST_TRY(cudaMemsetAsync(ones, 0xFF, 2 * bits + list, st));
+    const dim3 mark(a.n_new, (a.max_pages + 1023) / 1024);
+    if (mark.y > 65535) return host_fail(CLLM_ERR_TOO_LARGE, "%s: %d pages per sequence", who, a.max_pages);
+    const unsigned apply = (unsigned)a.n_new + 8u * (unsigned)sms;
+    if (fork) {
+        fork_mark_kernel<<<mark, 256, 0, st>>>(a);
+        fork_plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
+        fork_apply_kernel<<<apply, kCopyThreads, 0, st>>>(a);
+    } else {
+        compact_mark_kernel<<<mark, 256, 0, st>>>(a);
+        compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
+        compact_apply_kernel<<<apply, kCopyThreads, 0, st>>>(a);
+    }
+    CLLM_HOST_TRY(cudaGetLastError());
+    return CLLM_OK;
+}
+
+int cllm_cuda_kv4_fork(void* pages, int n_layers, int n_pages, int64_t page_bytes, int page_len,
+                       const int* page_table, const int* seq_len, int n_old, const int* source, const int* new_len,
+                       int n_new, int max_pages, int* table_out, int* len_out, void* stream) {
+    if (n_old <= 0 || n_new < 0) return host_fail(CLLM_ERR_INVALID_ARG, "kv4_fork: bad sizes");
+    if (n_new == 0) return CLLM_OK;
+    if (!pages || !page_table || !seq_len || !source || !new_len || !table_out || !len_out)
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_fork: null argument");
+    if (table_out == page_table || len_out == seq_len)
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_fork: the new table and lengths need buffers of their own");
+    PagesArgs a{};
+    a.n_layers = n_layers; a.n_pages = n_pages; a.page_len = page_len; a.max_pages = max_pages;
+    a.table = page_table; a.seq_len = seq_len; a.source = source; a.new_len = new_len;
+    a.n_old = n_old; a.n_new = n_new; a.table_out = table_out; a.len_out = len_out;
+    return pages_call("kv4_fork", a, pages, page_bytes, true, stream);
+}
+
+int cllm_cuda_kv4_compact(void* pages, int n_layers, int n_pages, int64_t page_bytes, int page_len,
+                          const int* page_table, const int* seq_len, int n_seqs, int max_pages, int* table_out,
+                          int* n_live, void* stream) {
+    if (n_seqs <= 0) return host_fail(CLLM_ERR_INVALID_ARG, "kv4_compact: bad sizes");
+    if (!pages || !page_table || !seq_len || !table_out || !n_live)
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_compact: null argument");
+    PagesArgs a{};
+    a.n_layers = n_layers; a.n_pages = n_pages; a.page_len = page_len; a.max_pages = max_pages;
+    a.table = page_table; a.seq_len = seq_len; a.n_old = a.n_new = n_seqs; a.table_out = table_out; a.n_live = n_live;
+    return pages_call("kv4_compact", a, pages, page_bytes, false, stream);
+}
+
+int cllm_cuda_token_scores(const float* logits, int64_t ld, int rows, int vocab, const int* tokens, int top_k,
+                           float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprobs,
+                           void* stream) {
+    if (rows < 0 || vocab <= 0 || ld < vocab) return host_fail(CLLM_ERR_INVALID_ARG, "token_scores: bad sizes");
+    if (top_k < 0 || top_k > CLLM_MAX_TOP_K || top_k > vocab)
+        return host_fail(CLLM_ERR_INVALID_ARG, "token_scores: top_k %d (0 to %d, at most the vocabulary)", top_k,
+                         CLLM_MAX_TOP_K);
+    if (rows == 0) return CLLM_OK;
+    if (!logits || (top_k > 0 && (!top_ids || !top_logprobs)) || ((logprob || rank) && !tokens))
+        return host_fail(CLLM_ERR_INVALID_ARG, "token_scores: null argument");
+    int dev, sms;
+    if (int rc = host_device(&dev, &sms)) return rc;
+    ScoreArgs a{logits, ld, rows, vocab, top_k, tokens, logprob, entropy, rank, top_ids, top_logprobs};
+    token_scores_kernel<<<rows, kScoreThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    CLLM_HOST_TRY(cudaGetLastError());
+    return CLLM_OK;
+}
+
+}  // extern "C"

@@ -363,8 +363,110 @@ int cllm_cuda_rope_kv(float* q, const float* k, const float* v, int n_tok, int n
 int cllm_cuda_attention(const float* q, const float* k_cache, const float* v_cache, int n_tok, int pos0, int n_head,
                         int n_head_kv, int head_dim, float* out, void* stream);
 
+/* ---- Serving many sequences: a paged cache held in 4 bits ------------------
+ * No counterpart in the reference, whose engine serves one sequence from a
+ * contiguous fp32 cache (engine.cpp:119-146).  Device pointers, fp32 in and
+ * out, asynchronous on `stream`, no host read of anything on the device: every
+ * call can be captured into a CUDA graph (make a first call of the largest
+ * size before, as for cllm_cuda_matmul_quant: attention, fork and compact use
+ * the library's workspace, so calls that can overlap must be ordered).
+ *
+ * Pool.  `pages` (16-byte aligned) holds n_layers x n_pages pages of
+ * cllm_cuda_kv4_page_bytes bytes; the calls that work on one layer get that
+ * layer's first page.  A page holds page_len positions (a multiple of 16) of
+ * every KV head, keys and values: [kv head][tile of 16 positions][tile].  A
+ * head's vector (head_dim 64 or 128) is split into groups of 32 values, each
+ * with an fp16 scale d and minimum m; a value is d * n + m, n = 0..15.
+ * A tile is, in this order (two numbers a byte, the first in the low half):
+ *   keys    [position 16][t 4][group][8]: value 32 group + 8 t + (0..7)
+ *   values  [a 2][r 8][t 4][b 2][group][c 4]: position 4 t + 2 a + b,
+ *           value 32 group + 8 c + r
+ *   scales  (d, m) of the keys [position 16][group], then of the values.
+ *
+ * Sequences.  Sequence s has seq_len[s] positions (int32; negative counts as
+ * 0) in the pages page_table[s * max_pages + i], i < ceil(seq_len / page_len).
+ * Entries past those are not read.  A page may belong to several sequences.
+ * A page id outside the pool, or a position past max_pages * page_len, is
+ * never followed; it sets the device status, which
+ * cllm_cuda_check_device_status reports as CLLM_ERR_INVALID_ARG. */
+
+/* Bytes of one page of one layer; 0 for a geometry that is not supported. */
+int64_t cllm_cuda_kv4_page_bytes(int page_len, int n_head_kv, int head_dim);
+
+/* RoPE on q and k (as cllm_cuda_rope_kv) and the append of the rotated k and
+ * of v to the pages of one layer, quantised.  Token t belongs to sequence
+ * token_seq[t] (-1: padding, nothing is stored and its output rows are 0) at
+ * position token_pos[t]; tokens of one call have different (sequence,
+ * position) pairs.  q: rows of ldq floats (n_head * head_dim used), q_out:
+ * dense rows, may be q itself where ldq is n_head * head_dim; n_head 0: no
+ * queries.  k, v: rows of ldkv floats.  rope_table: as cllm_cuda_rope_table,
+ * n_pos positions; NULL: no rotation.  Per group of 32 values: m = fp16(min),
+ * d = fp16((max - min) * fp32(1/15)), n = (x - m) / d rounded to nearest even
+ * and clamped to 0..15 (0 where d is 0); a group that holds a NaN or an
+ * infinity, or leaves the fp16 range, reads back as NaN.  k_out, v_out (NULL:
+ * none): dense [n_tok][n_head_kv * head_dim], the values the cache now holds. */
+int cllm_cuda_kv4_append(const float* q, int64_t ldq, float* q_out, const float* k, const float* v, int64_t ldkv,
+                         int n_tok, int n_head, const float* rope_table, int n_pos, const int* token_seq,
+                         const int* token_pos, void* pages, int n_pages, int page_len, int n_head_kv, int head_dim,
+                         const int* page_table, int n_seqs, int max_pages, float* k_out, float* v_out, void* stream);
+
+/* GQA attention of each sequence's newest rows over its pages of one layer.
+ * Sequence s brings the rows q_begin[s] .. q_begin[s+1] of q (q_begin NULL:
+ * one row each, n_tok == n_seqs); of its n rows, row i sees the positions
+ * before seq_len[s] - (n - 1 - i).  out: dense [n_tok][n_head * head_dim];
+ * lse (NULL: none): [n_tok][n_head], log(sum(exp(scale * q.k))).  A row that
+ * sees nothing, or belongs to no sequence, gets out = 0 and lse = -inf.
+ * scale 0: 1 / sqrt(head_dim).  n_head: any multiple of n_head_kv.  Products
+ * are taken on tensor cores with fp32 accuracy. */
+int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int n_tok, int n_head, const void* pages,
+                            int n_pages, int page_len, int n_head_kv, int head_dim, const int* page_table,
+                            const int* seq_len, int n_seqs, int max_pages, float scale, float* out, float* lse,
+                            void* stream);
+
+/* Fork, reorder, grow, truncate and free sequences.  New sequence s (of n_new)
+ * holds the first min(seq_len[source[s]], new_len[s]) positions of old
+ * sequence source[s] (of n_old; -1: none) and has pages for new_len[s]; its
+ * row of table_out and len_out[s] = new_len[s] are written (entries past its
+ * pages are -1).  Old sequences that no new one continues are freed.  Pages
+ * that end whole inside the continued part are shared.  The page in which it
+ * ends is kept by the lowest s that ends in it, unless a new sequence has it
+ * whole; every other one gets a copy, made in all n_layers layers.  Free pages
+ * are those no new sequence holds, given out lowest id first in order of s.  A
+ * sequence that finds no room (or whose new_len needs more than max_pages
+ * pages, or whose source is out of range) gets len_out -1 and no pages; what
+ * the first kind continued counts as held in this call.
+ * table_out and len_out may not be page_table and seq_len; page_bytes: of one
+ * page of one layer, a multiple of 16. */
+int cllm_cuda_kv4_fork(void* pages, int n_layers, int n_pages, int64_t page_bytes, int page_len,
+                       const int* page_table, const int* seq_len, int n_old, const int* source, const int* new_len,
+                       int n_new, int max_pages, int* table_out, int* len_out, void* stream);
+
+/* Move the pages in use to the lowest ids: with n pages in use, those with an
+ * id of n or more go, in order, to the free ids below n, in order, in all
+ * layers.  Writes table_out (may be page_table; entries past a sequence's
+ * pages are -1) and n_live[0] = n. */
+int cllm_cuda_kv4_compact(void* pages, int n_layers, int n_pages, int64_t page_bytes, int page_len,
+                          const int* page_table, const int* seq_len, int n_seqs, int max_pages, int* table_out,
+                          int* n_live, void* stream);
+
+/* What a sampler reports of `rows` rows of logits (row stride ld): with p =
+ * softmax(row), logprob[r] = log p[tokens[r]]; rank[r] = how many entries come
+ * before the token in the order of (logit descending, index ascending);
+ * entropy[r] = -sum p log p; top_ids, top_logprobs [rows][top_k]: the first
+ * top_k entries of that order (top_k 0: none, at most 32 and at most vocab).
+ * logprob, rank (both need tokens), entropy may be NULL.  -inf entries are
+ * allowed (p = 0); a row with a NaN, a +inf or nothing but -inf has no
+ * distribution: its floats are NaN, and in the order NaN counts as -inf.  A
+ * token outside 0..vocab-1 gets logprob NaN and rank -1. */
+#define CLLM_MAX_TOP_K 32
+int cllm_cuda_token_scores(const float* logits, int64_t ld, int rows, int vocab, const int* tokens, int top_k,
+                           float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprobs,
+                           void* stream);
+
 /* Read and clear the device-side status word that kernels set when a bounded
- * wait expires (CLLM_ERR_KERNEL_TIMEOUT); synchronizes the device. */
+ * wait expires (CLLM_ERR_KERNEL_TIMEOUT) or a page table names a page or a
+ * position that does not exist (CLLM_ERR_INVALID_ARG); synchronizes the
+ * device. */
 int cllm_cuda_check_device_status(void);
 
 /* Copy the calling thread's last error message into buf (NUL-terminated,

@@ -1,23 +1,14 @@
-// Attention over the 4-bit cache (cllm_cuda_kv4_attention): one warp per query
+// Attention of many rows per sequence: one warp per query
 // row and head, lane = head_dim/32 values, positions one after the other with
 // the running maximum and sum of the softmax.
 #pragma once
-#include "kv4_format.cuh"
+#include "kv4_decode.cuh"
 
 namespace cllm {
 namespace serve {
 
-struct AttnArgs {
-    const float* q;
-    int64_t ldq;
-    const int* q_begin;  // nullptr: row s belongs to sequence s
-    int n_tok, n_head;
-    float scale;
-    float *out, *lse;
-    Cache c;
-};
-
-// Sequence of row t and the positions it sees (0 for a row of no sequence).
+// Sequence of row t and the positions it sees (0 for a row of no sequence, -1
+// for one that kv4_rows_kernel has).
 __device__ __forceinline__ int row_sees(const AttnArgs& a, int t, int* seq) {
     int s = t, i = 0, n = 1;
     if (a.q_begin) {
@@ -28,11 +19,12 @@ __device__ __forceinline__ int row_sees(const AttnArgs& a, int t, int* seq) {
             else hi = mid;
         }
         s = lo;
-        if (s >= a.c.n_seqs || t < a.q_begin[s]) return 0;
+        if (s >= a.c.n_seqs || t < a.q_begin[s]) return -1;
         i = t - a.q_begin[s];
         n = a.q_begin[s + 1] - a.q_begin[s];
     }
     *seq = s;
+    if ((int64_t)n * a.rep <= a.rows_max) return -1;
     return max(0, a.c.length(s) - (n - 1 - i));
 }
 
@@ -44,6 +36,7 @@ __global__ void __launch_bounds__(128) kv4_attention_kernel(const AttnArgs a) {
     const int kvh = h / (a.n_head / a.c.n_kv);
     int seq = 0;
     const int sees = row_sees(a, t, &seq);
+    if (sees < 0) return;
     float q[D], acc[D];
 #pragma unroll
     for (int e = 0; e < D; ++e) {

@@ -1,0 +1,651 @@
+// Attention of a few rows per sequence over the 4-bit cache
+// (cllm_cuda_kv4_attention; generated tokens).
+//
+// What bounds it: every stored byte is read once and serves rep query heads
+// with 4 * rep * head_dim operations a position, so the HBM stream.  At 6.4
+// TB/s an SM gets a tile of 16 positions every 110 cycles (head_dim 128), in
+// which its four schedulers issue 440 instructions: the numbers must reach the
+// tensor cores with very few of them.
+//
+// * Numbers become fp16 two at a time: (w & 0x000F000F) | 0x64006400 is the pair
+//   (1024 + n, 1024 + n'), and one fused operation takes the 1024 off (and the 16
+//   of a number that sits in the next four bits): two instructions a pair.
+//   Subnormals (the bare four bits) would save one of them, but the tensor cores
+//   align products by the exponents of the operands' encodings and cut off what
+//   lies 24 bits below: 37 positions were off by 7e-6, 131071 by 4e-4.
+// * Scales outside.  q.k = sum over groups of d_g (q . n)_g + m_g sum(q)_g: one
+//   accumulator per group, multiplied by d_g in fp32, and one more product whose
+//   operand is the scale words themselves (k index 2g is d_g, met by a zero, 2g + 1
+//   is m_g, met by sum(q)_g).  sum p v = (p d) . (n - 8) + p . (m + 8 d): around the
+//   middle of the numbers, because p d n alone adds up to many times the result
+//   and every instruction cuts off towards zero; m + 8 d is an exact fp16 pair.
+// * fp32 accuracy.  The query rows (and p, p d) enter as fp16 hi + lo in the two
+//   halves of the instruction's 16 rows, 22 bits together: with at most 8 rows of
+//   one KV head the second half would be empty anyway.  hi and lo of p d come from
+//   three fp16 operations: hi = p_hi d, lo = fma(p_lo, d, fma(p_hi, d, -hi)).
+// * An instruction adds up 16 positions only; its sums are added to the result in
+//   fp32, rounded to nearest.
+// * No number changes lanes.  The tile's order gives each lane its operands of a
+//   16 x head_dim tile in two 16-byte loads, for keys and for values, and the
+//   score a lane computes is the p that the same lane needs as an operand.
+// * The running reference (in place of the maximum) of a row moves only when a
+//   score exceeds it by 2^14, so the accumulators are hardly ever rescaled; a p
+//   of at most 2^14 keeps p d inside fp16 (values' scales of 2 and more lower it).
+// * Work: steps of 64 positions of (sequence, KV head, 8 rows), numbered through
+//   and cut into equal runs, one per CTA, whatever the lengths are.  A CTA's four
+//   warps take a tile each, from a ring of their own that one lane fills with
+//   bulk copies across the runs' borders.  A run that ends inside an item leaves a
+//   partial result, which kv4_join_kernel puts together in order.
+#pragma once
+#include "kv4_format.cuh"
+
+namespace cllm {
+namespace serve {
+
+constexpr int kRowWarps = 4;
+constexpr int kRowThreads = 32 * kRowWarps;
+constexpr int kRowStages = 4;               // tiles of a warp's ring
+constexpr int kRowTile = 8;                 // query rows of an item
+constexpr int kStepLen = kTile * kRowWarps; // positions of a step
+constexpr int kRowCtasPerSm = 3;
+constexpr int kMaxRowCtas = 1024;
+
+struct AttnArgs {
+    const float* q;
+    int64_t ldq;
+    const int* q_begin;  // nullptr: row s belongs to sequence s
+    int n_tok, n_head, rep;
+    int rows_max;        // sequences with more rows * rep are the prompt kernel's
+    float scale;
+    float *out, *lse;
+    Cache c;
+};
+
+// An item that begins in a CTA's run and ends in another's.
+struct Part {
+    int seq, item;  // item: KV head * row groups + row group
+    int parts;      // CTAs that have a part of it, this one first; 0: nothing to join here
+    int slot;       // of this CTA's part (the others': their first slot)
+};
+
+struct RowsArgs {
+    AttnArgs a;
+    Part* last;      // [ctas]
+    float* part_ml;  // [2 * ctas][kRowTile][2] reference (log2) and sum; slot 2c: first item of CTA c, 2c + 1: last
+    float* part_o;   // [2 * ctas][kRowTile][HD]
+};
+
+// ---- rows of a sequence -------------------------------------------------------
+
+__device__ __forceinline__ void seq_rows(const AttnArgs& a, int s, int* begin, int* n) {
+    if (!a.q_begin) {
+        *begin = s;
+        *n = 1;
+        return;
+    }
+    const int b = min(max(a.q_begin[s], 0), a.n_tok), e = min(max(a.q_begin[s + 1], 0), a.n_tok);
+    *begin = b;
+    *n = max(0, e - b);
+}
+
+// What a sequence asks of this kernel: items (0: nothing) of `steps` steps each.
+struct SeqWork {
+    int begin, n, len, items, steps;
+};
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int s) {
+    SeqWork w;
+    seq_rows(a, s, &w.begin, &w.n);
+    w.items = 0;
+    w.steps = 1;
+    w.len = 0;
+    const int64_t rows = (int64_t)w.n * a.rep;
+    if (rows == 0 || rows > a.rows_max) return w;
+    w.len = a.c.length(s);
+    w.items = a.c.n_kv * (int)((rows + kRowTile - 1) / kRowTile);
+    w.steps = max(1, (w.len + kStepLen - 1) / kStepLen);  // one even for no positions: its rows are zeros
+    return w;
+}
+
+// A place in the numbered steps.
+struct Cursor {
+    int s, item, step, left;  // left: steps up to the end of this CTA's run
+    SeqWork w;
+    __device__ __forceinline__ void next(const AttnArgs& a, int steps) {  // over `steps` steps inside the item
+        left -= steps;
+        step += steps;
+        if (step < w.steps) return;
+        step = 0;
+        if (++item < w.items) return;
+        item = 0;
+        while (left > 0 && s + 1 < a.c.n_seqs) {
+            w = seq_work(a, ++s);
+            if (w.items) return;
+        }
+    }
+};
+
+__device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t* s_warp, int64_t* total) {  // exclusive, kRowThreads threads
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    int64_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+        before += w < warp ? s_warp[w] : 0;
+        all += s_warp[w];
+    }
+    __syncthreads();
+    *total = all;
+    return before + x - v;
+}
+
+// ---- instructions ---------------------------------------------------------------
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The product alone (accumulator 0).
+__device__ __forceinline__ void mma16816_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t h2bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t b) { return *reinterpret_cast<__half2*>(&b); }
+// (x, y) = hi + lo, each an fp16 pair, to 22 bits
+__device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    *hi = h2bits(h);
+    *lo = h2bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+// The numbers in bits 0-3 (UP: 4-7) of both halves of w, plus `off`, as an fp16 pair.
+template <bool UP>
+__device__ __forceinline__ uint32_t numbers(uint32_t w, float off) {
+    uint32_t x;
+    if constexpr (UP) {
+        asm("lop3.b32 %0, %1, 0x00F000F0, 0x64006400, 0xEA;" : "=r"(x) : "r"(w));
+        return h2bits(__hfma2(bits_h2(x), __float2half2_rn(0.0625f), __float2half2_rn(off - 64.f)));
+    }
+    asm("lop3.b32 %0, %1, 0x000F000F, 0x64006400, 0xEA;" : "=r"(x) : "r"(w));
+    return h2bits(__hadd2(bits_h2(x), __float2half2_rn(off - 1024.f)));
+}
+// The exact sum of two fp16 pairs as a pair of fp16 pairs.
+__device__ __forceinline__ void sum2(__half2 a, __half2 b, uint32_t* hi, uint32_t* lo) {
+    const __half2 s = __hadd2(a, b), x = __hsub2(s, a);
+    *hi = h2bits(s);
+    *lo = h2bits(__hadd2(__hsub2(a, __hsub2(s, x)), __hsub2(b, x)));
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+template <int W>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[W]) {
+    if constexpr (W == 4) {
+        const uint4 v = lds128(a);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+        const uint2 v = lds64(a);
+        w[0] = v.x; w[1] = v.y;
+    }
+}
+__device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 255u) == 0 && global_timer_ns() - t0 > kWaitLimitNs) {
+            atomicOr(&g_serve_status, kServeTimeout);
+            return false;
+        }
+    }
+}
+
+template <int HD>
+struct RowsSmem {
+    static constexpr int kLd = HD + 8;  // row stride of the merge buffer: no two rows of a half warp in one bank
+    uint8_t ring[kRowWarps][kRowStages][Tile<HD>::kBytes];
+    float o[kRowWarps][kRowTile][kLd];
+    float ml[kRowWarps][kRowTile][2];
+    uint64_t full[kRowWarps][kRowStages];
+    int64_t scan[kRowWarps];
+    int start[4];
+};
+
+// Column r of a score tile i (and row of a values' operand) is this position of the tile: lane t of
+// a row group then holds the positions 4t .. 4t+3, whose scale rows lie in different banks for all t.
+__device__ __forceinline__ int tile_pos(int i, int r) { return 4 * (r >> 1) + 2 * i + ((r & 1) ^ (r >> 2)); }
+
+// ---- the kernel --------------------------------------------------------------------
+
+template <int HD>
+__global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(const RowsArgs ra) {
+    constexpr int G = Tile<HD>::G, KS = HD / 16;  // k steps of 16 for keys
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    RowsSmem<HD>& sm = *reinterpret_cast<RowsSmem<HD>*>(smem_raw);
+    const AttnArgs& a = ra.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
+
+    if (lane == 0) {
+        for (int i = 0; i < kRowStages; ++i) mbar_init(smem_addr(&sm.full[warp][i]), 1);
+        fence_mbar_init();
+    }
+    // rows of no sequence
+    if (a.q_begin) {
+        const int b = min(max(a.q_begin[0], 0), a.n_tok), e = max(b, min(a.q_begin[a.c.n_seqs], a.n_tok));
+        for (int i = blockIdx.x; i < b + a.n_tok - e; i += gridDim.x) {
+            const int64_t row = i < b ? i : e + i - b;
+            for (int j = threadIdx.x; j < a.n_head * HD; j += kRowThreads) a.out[row * a.n_head * HD + j] = 0.f;
+            if (a.lse)
+                for (int j = threadIdx.x; j < a.n_head; j += kRowThreads) a.lse[row * a.n_head + j] = -INFINITY;
+        }
+    }
+    // all steps, and this CTA's run of them
+    const int per = (a.c.n_seqs + kRowThreads - 1) / kRowThreads;
+    const int s0 = min(a.c.n_seqs, (int)threadIdx.x * per), s1 = min(a.c.n_seqs, s0 + per);
+    int64_t mine = 0;
+    for (int s = s0; s < s1; ++s) {
+        const SeqWork w = seq_work(a, s);
+        mine += (int64_t)w.items * w.steps;
+    }
+    int64_t all;
+    const int64_t before = cta_scan(mine, sm.scan, &all);
+    const int ctas = (int)min((int64_t)gridDim.x, all);
+    if (threadIdx.x == 0) ra.last[blockIdx.x].parts = 0;
+    if ((int)blockIdx.x >= ctas) return;
+    const int64_t run0 = blockIdx.x * all / ctas, run1 = (blockIdx.x + 1) * all / ctas;
+    if (mine && before <= run0 && run0 < before + mine) {
+        int64_t at = before;
+        for (int s = s0; s < s1; ++s) {
+            const SeqWork w = seq_work(a, s);
+            const int64_t next = at + (int64_t)w.items * w.steps;
+            if (run0 < next) {
+                sm.start[0] = s;
+                sm.start[1] = (int)((run0 - at) / w.steps);
+                sm.start[2] = (int)((run0 - at) % w.steps);
+                break;
+            }
+            at = next;
+        }
+    }
+    __syncthreads();
+    Cursor cur;
+    cur.s = sm.start[0];
+    cur.item = sm.start[1];
+    cur.step = sm.start[2];
+    cur.left = (int)(run1 - run0);
+    cur.w = seq_work(a, cur.s);
+
+    // The producer runs ahead of the warp's own tiles; the page of its next
+    // tile is looked up one call before it is needed.
+    Cursor pro = cur;
+    int pro_id = 0, pro_head = 0, pro_at = -1;  // pro_at < 0: nothing left
+    int issued = 0;
+    auto seek = [&]() {
+        pro_at = -1;
+        while (pro.left > 0) {
+            const int p = (pro.step * kRowWarps + warp) * kTile;
+            const bool there = p < pro.w.len;
+            if (there) {
+                pro_head = pro.item / (pro.w.items / a.c.n_kv);
+                pro_at = p;
+                pro_id = a.c.table[(int64_t)pro.s * a.c.max_pages + p / a.c.page_len];
+            }
+            pro.next(a, 1);
+            if (there) return;
+        }
+    };
+    auto produce = [&]() {
+        if (pro_at < 0) return;
+        if (lane == 0) {
+            int id = pro_id;
+            if ((unsigned)id >= (unsigned)a.c.n_pages) {
+                atomicOr(&g_serve_status, kServeBadPage);
+                id = 0;
+            }
+            const int st = issued % kRowStages;
+            const uint32_t bar = smem_addr(&sm.full[warp][st]);
+            mbar_arrive_expect_tx(bar, Tile<HD>::kBytes);
+            bulk_g2s(smem_addr(sm.ring[warp][st]), a.c.tile<HD>(id, pro_head, pro_at % a.c.page_len), Tile<HD>::kBytes, bar);
+        }
+        ++issued;
+        seek();
+    };
+    seek();
+#pragma unroll 1
+    for (int i = 0; i < kRowStages; ++i) produce();
+
+    bool alive = true;
+    int used = 0;
+    for (bool first = true; cur.left > 0; first = false) {
+        // ---- one item (or the part of it inside the run)
+        const int steps = min(cur.left, cur.w.steps - cur.step), groups = cur.w.items / a.c.n_kv;
+        const int kvh = cur.item / groups, row0 = (cur.item - kvh * groups) * kRowTile;
+        const int rows = min(kRowTile, cur.w.n * a.rep - row0);
+        const int tok = (row0 + r) / a.rep;  // row r of the tile: token and head
+        const int sees = r < rows ? cur.w.len - (cur.w.n - 1 - tok) : 0;
+        const int sees_all = cur.w.len - (cur.w.n - 1 - row0 / a.rep);  // positions that every row sees
+        // the query row as operands: q * 2^k, its largest value in [2^9, 2^10)
+        uint32_t qa[KS][4], qs_hi = 0, qs_lo = 0;
+        float f_log2;  // score (log2) over what the products give
+        {
+            float q[G][8];
+            float top = 0.f;
+            const float* src = a.q + (int64_t)(cur.w.begin + tok) * a.ldq + (kvh * a.rep + (row0 + r) % a.rep) * HD + 8 * t;
+            const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (a.ldq * 4)) & 15) == 0;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                if (r < rows && vec) {
+                    const float4 x = *reinterpret_cast<const float4*>(src + 32 * g);
+                    const float4 y = *reinterpret_cast<const float4*>(src + 32 * g + 4);
+                    q[g][0] = x.x; q[g][1] = x.y; q[g][2] = x.z; q[g][3] = x.w;
+                    q[g][4] = y.x; q[g][5] = y.y; q[g][6] = y.z; q[g][7] = y.w;
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) q[g][n] = r < rows ? src[32 * g + n] : 0.f;
+                }
+#pragma unroll
+                for (int n = 0; n < 8; ++n) top = fmaxf(top, fabsf(q[g][n]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            const int e = min(max((int)(__float_as_uint(top) >> 23), 30), 230);
+            const float up = __uint_as_float((uint32_t)(127 + 136 - e) << 23), down = __uint_as_float((uint32_t)(e - 9) << 23);
+            f_log2 = a.scale * 1.44269504088896340736f * down;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                float sum = 0.f;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    q[g][n] *= up;
+                    sum += q[g][n];
+                }
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+                if (t == g) split2(0.f, sum, &qs_hi, &qs_lo);
+                split2(q[g][0], q[g][4], &qa[2 * g][0], &qa[2 * g][1]);
+                split2(q[g][1], q[g][5], &qa[2 * g][2], &qa[2 * g][3]);
+                split2(q[g][2], q[g][6], &qa[2 * g + 1][0], &qa[2 * g + 1][1]);
+                split2(q[g][3], q[g][7], &qa[2 * g + 1][2], &qa[2 * g + 1][3]);
+            }
+        }
+        float2 o[G][4], om = make_float2(0.f, 0.f);  // values' numbers: [group][c], and the minima's part
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[g][c] = make_float2(0.f, 0.f);
+        float ref = -3.0e38f, l = 0.f;
+
+#pragma unroll 1
+        for (int i = 0; i < steps; ++i) {
+            const int p0 = ((cur.step + i) * kRowWarps + warp) * kTile;
+            if (p0 >= cur.w.len) break;  // and so are the warp's further tiles
+            const int st = used % kRowStages;
+            if (alive) alive = wait_full(smem_addr(&sm.full[warp][st]), (uint32_t)(used / kRowStages) & 1u);
+            const uint32_t tile = smem_addr(sm.ring[warp][st]);
+            ++used;
+            // ---- scores of positions 4t .. 4t+3 for row r
+            float s[4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int pr = tile_pos(h, r);
+                uint32_t kw[G], d0[G], d1[G];
+                lds_words<G>(tile + pr * (HD / 2) + t * (HD / 8), kw);
+                lds_words<G>(tile + Tile<HD>::kScaleK + (4 * t + 2 * h + (t >> 1)) * (HD / 8), d0);
+                lds_words<G>(tile + Tile<HD>::kScaleK + (4 * t + 2 * h + 1 - (t >> 1)) * (HD / 8), d1);
+                uint32_t mw = 0;
+                if (G == 4 || t < G) mw = lds32(tile + Tile<HD>::kScaleK + pr * (HD / 8) + t * 4);
+                float cm[4];
+                mma16816_zero(cm, qs_hi, qs_lo, 0u, 0u, mw, 0u);
+                float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    float c[4];
+                    const uint32_t w = kw[g], w8 = w >> 8;
+                    mma16816_zero(c, qa[2 * g][0], qa[2 * g][1], qa[2 * g][2], qa[2 * g][3], numbers<false>(w, 0.f),
+                                  numbers<true>(w, 0.f));
+                    mma16816(c, qa[2 * g + 1][0], qa[2 * g + 1][1], qa[2 * g + 1][2], qa[2 * g + 1][3],
+                             numbers<false>(w8, 0.f), numbers<true>(w8, 0.f));
+                    acc = __ffma2_rn(add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])),
+                                     make_float2(h2f(d0[g]), h2f(d1[g])), acc);
+                }
+                acc = add2(acc, add2(make_float2(cm[0], cm[1]), make_float2(cm[2], cm[3])));
+                s[2 * h] = acc.x * f_log2;
+                s[2 * h + 1] = acc.y * f_log2;
+            }
+            // ---- weights
+            uint32_t vd[4][G];  // (d, m) of the values of the lane's positions
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                lds_words<G>(tile + Tile<HD>::kScaleV + (4 * t + (j ^ (t >> 1))) * (HD / 8), vd[j]);
+            const uint2 sv = lds64(tile + Tile<HD>::kScaleV + (lane & (HD / 4 - 1)) * 8);
+            uint32_t big = max(sv.x & 0x7FFFu, sv.y & 0x7FFFu);  // largest scale (bits) of two groups, of all in the warp
+            const bool edge = p0 + kTile > sees_all;
+            if (edge) {  // positions that the row does not see: whatever is stored there must not touch it
+                big = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        if (p0 + 4 * t + (j ^ (t >> 1)) >= sees) {
+                            s[j] = -INFINITY;
+                            vd[j][g] = 0u;
+                        }
+                        big = max(big, vd[j][g] & 0x7FFFu);
+                    }
+            }
+            float room = 14.f;
+            if (__any_sync(0xFFFFFFFFu, big >= 0x4000u))  // a scale of 2 or more: p d stays below 2^15
+                room = 14.f - (float)((int)(__reduce_max_sync(0xFFFFFFFFu, big) >> 10) - 15);
+            const float smax = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            if (__any_sync(0xFFFFFFFFu, smax > ref + room)) {
+                float m = fmaxf(smax, __shfl_xor_sync(0xFFFFFFFFu, smax, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+                const float to = m > ref + room ? m - (room - 4.f) : ref;
+                const float keep = exp2_fast(ref - to);
+                ref = to;
+                l *= keep;
+                const float2 k2 = make_float2(keep, keep);
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[g][c] = __fmul2_rn(o[g][c], k2);
+                om = __fmul2_rn(om, k2);
+            }
+            float p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = exp2_fast(s[j] - ref);
+            l += (p[0] + p[1]) + (p[2] + p[3]);
+            uint32_t ph[2], pl[2];
+            split2(p[0], p[1], &ph[0], &pl[0]);
+            split2(p[2], p[3], &ph[1], &pl[1]);
+            // ---- p . (m / 2 + 4 d): column 2g of the product, lanes of an even r
+            if (!edge) {
+                uint32_t w[4];  // (d, m) of group r / 2 at the positions of the lane's operand
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    w[j] = G == 4 || r < 4 ? lds32(tile + Tile<HD>::kScaleV + (4 * t + (j ^ (t >> 1))) * (HD / 8) + (r >> 1) * 4) : 0u;
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    sum2(__hmul2(bits_h2(__byte_perm(w[2 * k], w[2 * k + 1], 0x5410)), __float2half2_rn(4.f)),
+                         __hmul2(bits_h2(__byte_perm(w[2 * k], w[2 * k + 1], 0x7632)), __float2half2_rn(0.5f)), &hi[k], &lo[k]);
+                float c[4];
+                mma16816_zero(c, ph[0], pl[0], ph[1], pl[1], lo[0], lo[1]);
+                om = add2(om, add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
+                mma16816_zero(c, ph[0], pl[0], ph[1], pl[1], hi[0], hi[1]);
+                om = add2(om, add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
+            } else {  // row by row, so that a NaN stays with the rows that see it
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x = fmaf(p[j], fmaf(4.f, h2f(vd[j][g]), 0.5f * h2f(vd[j][g] >> 16)), x);
+                    x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
+                    x += __shfl_xor_sync(0xFFFFFFFFu, x, 2);
+                    if (t == g) om.x += x;
+                }
+            }
+            // ---- (p d) . n
+            uint32_t va[G], vb[G];
+            lds_words<G>(tile + Tile<HD>::kV + lane * (HD / 8), va);
+            lds_words<G>(tile + Tile<HD>::kV + (32 + lane) * (HD / 8), vb);
+            const uint32_t low = t < 2 ? 0x5410u : 0x1054u, high = t < 2 ? 0x7632u : 0x3276u;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                uint32_t hi[2], lo[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const __half2 d = bits_h2(__byte_perm(vd[2 * k][g], vd[2 * k + 1][g], 0x5410));
+                    const __half2 h = __hmul2(bits_h2(ph[k]), d);
+                    hi[k] = h2bits(h);
+                    lo[k] = h2bits(__hfma2(bits_h2(pl[k]), d, __hfma2(bits_h2(ph[k]), d, __hneg2(h))));
+                }
+                const uint32_t sel = g & 1 ? high : low;
+                const uint32_t x0 = __byte_perm(va[g / 2], va[G / 2 + g / 2], sel), x1 = __byte_perm(vb[g / 2], vb[G / 2 + g / 2], sel);
+                const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+                const uint32_t b[4][2] = {{numbers<false>(x0, -8.f), numbers<false>(x1, -8.f)},
+                                          {numbers<true>(x0, -8.f), numbers<true>(x1, -8.f)},
+                                          {numbers<false>(y0, -8.f), numbers<false>(y1, -8.f)},
+                                          {numbers<true>(y0, -8.f), numbers<true>(y1, -8.f)}};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float c[4];
+                    mma16816_zero(c, hi[0], lo[0], hi[1], lo[1], b[j][0], b[j][1]);
+                    o[g][j] = add2(o[g][j], add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
+                }
+            }
+            __syncwarp();
+            produce();
+        }
+
+        // ---- the four warps' results together
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+        {
+            // sums of p (m / 2 + 4 d): column 2g, i.e. lane t = g, element 0
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const float mid = __shfl_sync(0xFFFFFFFFu, om.x, (lane & ~3) + g);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    *reinterpret_cast<float2*>(&sm.o[warp][r][32 * g + 8 * c + 2 * t]) =
+                        make_float2(fmaf(2.f, mid, o[g][c].x), fmaf(2.f, mid, o[g][c].y));
+            }
+            if (t == 0) {
+                sm.ml[warp][r][0] = ref;
+                sm.ml[warp][r][1] = l;
+            }
+        }
+        __syncthreads();
+        const bool whole = steps == cur.w.steps;
+        const int slot = 2 * blockIdx.x + (first ? 0 : 1);
+        for (int i = threadIdx.x; i < kRowTile * HD / 4; i += kRowThreads) {
+            const int rr = i / (HD / 4), d = 4 * (i % (HD / 4));
+            float m = sm.ml[0][rr][0];
+#pragma unroll
+            for (int w = 1; w < kRowWarps; ++w) m = fmaxf(m, sm.ml[w][rr][0]);
+            float sum = 0.f;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kRowWarps; ++w) {
+                const float k = exp2_fast(sm.ml[w][rr][0] - m);
+                const float4 y = *reinterpret_cast<const float4*>(&sm.o[w][rr][d]);
+                sum = fmaf(k, sm.ml[w][rr][1], sum);
+                x.x = fmaf(k, y.x, x.x); x.y = fmaf(k, y.y, x.y); x.z = fmaf(k, y.z, x.z); x.w = fmaf(k, y.w, x.w);
+            }
+            if (whole) {
+                if (rr < rows) {
+                    const int64_t at = (int64_t)(cur.w.begin + (row0 + rr) / a.rep) * a.n_head + kvh * a.rep + (row0 + rr) % a.rep;
+                    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+                    if (sum == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    *reinterpret_cast<float4*>(a.out + at * HD + d) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+                    if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (m + log2f(sum));
+                }
+            } else {
+                *reinterpret_cast<float4*>(ra.part_o + ((int64_t)slot * kRowTile + rr) * HD + d) = x;
+                if (d == 0) *reinterpret_cast<float2*>(ra.part_ml + (slot * kRowTile + rr) * 2) = make_float2(m, sum);
+            }
+        }
+        if (!whole && cur.step == 0 && threadIdx.x == 0) {  // the item begins here and ends in another CTA
+            const int64_t end = run1 - cur.left + cur.w.steps;  // number of the step after the item
+            ra.last[blockIdx.x] = Part{cur.s, cur.item, (int)((end * ctas - 1) / all) - (int)blockIdx.x + 1, slot};
+        }
+        __syncthreads();
+        cur.next(a, steps);
+    }
+    if (!alive)  // let the copies in flight land before the CTA ends
+        for (; used < issued; ++used) wait_full(smem_addr(&sm.full[warp][used % kRowStages]), (uint32_t)(used / kRowStages) & 1u);
+}
+
+// The parts of the item that begins in CTA blockIdx.x's run and ends in
+// another's: its row blockIdx.y, the parts added in their order.
+constexpr int kJoinThreads = 512;
+template <int HD>
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const RowsArgs ra) {
+    constexpr int kGroups = kJoinThreads / HD;
+    __shared__ float s_w[kMaxRowCtas], s_max[kJoinThreads / 32], s_sum[kJoinThreads / 32], s_o[kJoinThreads];
+    const AttnArgs& a = ra.a;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const Part part = ra.last[blockIdx.x];
+    if (!part.parts) return;
+    const SeqWork w = seq_work(a, part.seq);
+    const int groups = w.items / a.c.n_kv, kvh = part.item / groups, row = (part.item - kvh * groups) * kRowTile + blockIdx.y;
+    if (row >= w.n * a.rep) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto slot = [&](int i) -> int64_t { return (int64_t)(i ? 2 * ((int)blockIdx.x + i) : part.slot) * kRowTile + blockIdx.y; };
+    float m = -3.0e38f;
+    for (int i = threadIdx.x; i < part.parts; i += kJoinThreads) m = fmaxf(m, ra.part_ml[2 * slot(i)]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    if (lane == 0) s_max[warp] = m;
+    __syncthreads();
+    for (int i = 0; i < kJoinThreads / 32; ++i) m = fmaxf(m, s_max[i]);
+    float sum = 0.f;
+    for (int i = threadIdx.x; i < part.parts; i += kJoinThreads) {
+        const float2 x = *reinterpret_cast<const float2*>(ra.part_ml + 2 * slot(i));
+        s_w[i] = exp2_fast(x.x - m);
+        sum = fmaf(s_w[i], x.y, sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
+    for (int i = 0; i < kJoinThreads / 32; ++i) sum += s_sum[i];
+    const int d = threadIdx.x % HD, g = threadIdx.x / HD;
+    float x = 0.f;
+#pragma unroll 4
+    for (int i = g; i < part.parts; i += kGroups) x = fmaf(s_w[i], ra.part_o[slot(i) * HD + d], x);
+    s_o[threadIdx.x] = x;
+    __syncthreads();
+    if (g) return;
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) x += s_o[i * HD + d];
+    const int64_t at = (int64_t)(w.begin + row / a.rep) * a.n_head + kvh * a.rep + row % a.rep;
+    a.out[at * HD + d] = sum == 0.f ? 0.f : __fdiv_rn(x, sum);
+    if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (m + log2f(sum));
+}
+
+}  // namespace serve
+}  // namespace cllm

@@ -9,6 +9,7 @@
 
 #include "kv4_append.cuh"
 #include "kv4_attention.cuh"
+#include "kv4_decode.cuh"
 #include "kv4_format.cuh"
 #include "kv4_pages.cuh"
 #include "scores.cuh"
@@ -35,6 +36,44 @@ int check_geometry(const char* who, int n_pages, int page_len, int n_head_kv, in
         return host_fail(CLLM_ERR_INVALID_ARG, "%s: page_len %d (a multiple of 16, at most 4096)", who, page_len);
     if (n_head_kv <= 0 || n_head_kv > 65535 || n_pages <= 0)
         return host_fail(CLLM_ERR_INVALID_ARG, "%s: bad arguments (%d KV heads, %d pages)", who, n_head_kv, n_pages);
+    return CLLM_OK;
+}
+
+// Rows * heads of a KV head up to which a sequence is kv4_rows_kernel's.
+constexpr int kRowsMax = 64;
+
+template <int HD>
+int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
+    static std::once_flag once[64];
+    cudaError_t attr = cudaSuccess;
+    std::call_once(once[dev], [&] {
+        attr = cudaFuncSetAttribute(kv4_rows_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(RowsSmem<HD>));
+    });
+    CLLM_HOST_TRY(attr);
+    const int ctas = std::min(kMaxRowCtas, kRowCtasPerSm * sms);
+    const size_t last = align256(sizeof(Part) * ctas), ml = align256((size_t)2 * ctas * kRowTile * 2 * 4);
+    uint8_t* ws;
+    std::unique_lock<std::mutex> lk;
+    if (int rc = host_workspace(dev, last + ml + (size_t)2 * ctas * kRowTile * HD * 4, &ws, lk)) return rc;
+    RowsArgs ra{a, reinterpret_cast<Part*>(ws), reinterpret_cast<float*>(ws + last), reinterpret_cast<float*>(ws + last + ml)};
+    kv4_rows_kernel<HD><<<ctas, kRowThreads, sizeof(RowsSmem<HD>), st>>>(ra);
+    CLLM_HOST_TRY(cudaGetLastError());
+    if ((int64_t)a.c.max_pages * a.c.page_len > kStepLen) {  // an item can have more than one step
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(ctas, kRowTile);
+        cfg.blockDim = dim3(kJoinThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute pdl[1];
+        pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        pdl[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = pdl;
+        cfg.numAttrs = 1;
+        CLLM_HOST_TRY(cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD>, ra));
+    }
+    if (a.q_begin && (int64_t)a.n_tok * a.rep > a.rows_max) {
+        kv4_attention_kernel<HD><<<dim3(a.n_tok, (a.n_head + 3) / 4), 128, 0, st>>>(a);
+        CLLM_HOST_TRY(cudaGetLastError());
+    }
     return CLLM_OK;
 }
 
@@ -102,23 +141,21 @@ int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int
     if (n_tok == 0) return CLLM_OK;
     if (!q || !pages || !page_table || !seq_len || !out)
         return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: null argument");
-    if (!aligned16(pages)) return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: pages must be 16-byte aligned");
+    if (!aligned16(pages) || !aligned16(out))
+        return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: pages and out must be 16-byte aligned");
     if (ldq < (int64_t)n_head * head_dim)
         return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: a row is shorter than its heads");
     int dev, sms;
     if (int rc = host_device(&dev, &sms)) return rc;
     AttnArgs a{};
-    a.q = q; a.ldq = ldq; a.q_begin = q_begin; a.n_tok = n_tok; a.n_head = n_head;
+    a.q = q; a.ldq = ldq; a.q_begin = q_begin; a.n_tok = n_tok; a.n_head = n_head; a.rep = n_head / n_head_kv;
+    a.rows_max = std::max(kRowsMax, a.rep);
     a.scale = scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale;
     a.out = out; a.lse = lse;
     a.c = Cache{const_cast<uint8_t*>(static_cast<const uint8_t*>(pages)), page_table, seq_len, n_pages, page_len,
                 n_head_kv, n_seqs, max_pages};
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const dim3 grid(n_tok, (n_head + 3) / 4);
-    if (head_dim == 128) kv4_attention_kernel<128><<<grid, 128, 0, st>>>(a);
-    else kv4_attention_kernel<64><<<grid, 128, 0, st>>>(a);
-    CLLM_HOST_TRY(cudaGetLastError());
-    return CLLM_OK;
+    return head_dim == 128 ? launch_attention<128>(a, dev, sms, static_cast<cudaStream_t>(stream))
+                           : launch_attention<64>(a, dev, sms, static_cast<cudaStream_t>(stream));
 }
 
 static int pages_call(const char* who, PagesArgs a, void* pages, int64_t page_bytes, bool fork, void* stream) {

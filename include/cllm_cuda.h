@@ -416,7 +416,8 @@ int cllm_cuda_kv4_append(const float* q, int64_t ldq, float* q_out, const float*
  * before seq_len[s] - (n - 1 - i).  out: dense [n_tok][n_head * head_dim];
  * lse (NULL: none): [n_tok][n_head], log(sum(exp(scale * q.k))).  A row that
  * sees nothing, or belongs to no sequence, gets out = 0 and lse = -inf.
- * scale 0: 1 / sqrt(head_dim).  n_head: any multiple of n_head_kv.  Products
+ * out is 16-byte aligned.  scale 0: 1 / sqrt(head_dim).  n_head: any multiple
+ * of n_head_kv.  Products
  * are taken on tensor cores with fp32 accuracy. */
 int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int n_tok, int n_head, const void* pages,
                             int n_pages, int page_len, int n_head_kv, int head_dim, const int* page_table,

@@ -23,17 +23,18 @@
 //   halves of the instruction's 16 rows, 22 bits together: with at most 8 rows of
 //   one KV head the second half would be empty anyway.  hi and lo of p d come from
 //   three fp16 operations: hi = p_hi d, lo = fma(p_lo, d, fma(p_hi, d, -hi)).
-// * An instruction adds up 16 positions only; its sums are added to the result in
-//   fp32, rounded to nearest.
+// * The tensor cores add up the 32 positions of a step only; their sums are added
+//   to the result in fp32, rounded to nearest.
 // * No number changes lanes.  The tile's order gives each lane its operands of a
 //   16 x head_dim tile in two 16-byte loads, for keys and for values, and the
 //   score a lane computes is the p that the same lane needs as an operand.
 // * The running reference (in place of the maximum) of a row moves only when a
 //   score exceeds it by 2^14, so the accumulators are hardly ever rescaled; a p
 //   of at most 2^14 keeps p d inside fp16 (values' scales of 2 and more lower it).
-// * Work: steps of 64 positions of (sequence, KV head, 8 rows), numbered through
-//   and cut into equal runs, one per CTA, whatever the lengths are.  A CTA's four
-//   warps take a tile each, from a ring of their own that one lane fills with
+// * Work: steps of 128 positions of (sequence, KV head, 8 rows), numbered through
+//   (and some for the item itself) and cut into equal runs, one per CTA,
+//   whatever the lengths are.  A CTA's four
+//   warps take two tiles each, from a ring of their own that one lane fills with
 //   bulk copies across the runs' borders.  A run that ends inside an item leaves a
 //   partial result, which kv4_join_kernel puts together in order.
 #pragma once
@@ -44,11 +45,13 @@ namespace serve {
 
 constexpr int kRowWarps = 4;
 constexpr int kRowThreads = 32 * kRowWarps;
-constexpr int kRowStages = 4;               // tiles of a warp's ring
+constexpr int kRowStages = 2;               // pairs of tiles in a warp's ring
 constexpr int kRowTile = 8;                 // query rows of an item
-constexpr int kStepLen = kTile * kRowWarps; // positions of a step
+constexpr int kPairLen = 2 * kTile;         // positions of a warp's step
+constexpr int kStepLen = kPairLen * kRowWarps;
 constexpr int kRowCtasPerSm = 3;
-constexpr int kMaxRowCtas = 1024;
+constexpr int kMaxRowCtas = 640;
+constexpr uint32_t kNoTile = 0xFFFFFFFFu;
 
 struct AttnArgs {
     const float* q;
@@ -59,6 +62,14 @@ struct AttnArgs {
     float scale;
     float *out, *lse;
     Cache c;
+    int page_tiles;        // tiles of a page and head
+    uint32_t page_magic;   // ceil(2^32 / page_tiles), 0 where that is 2^32
+    // Slot of the page that holds a tile (< 2^27): the product is at most one too large.
+    __device__ __forceinline__ int page_of(int tile) const {
+        if (page_magic == 0) return tile;
+        const int s = (int)__umulhi((uint32_t)tile, page_magic);
+        return s * page_tiles > tile ? s - 1 : s;
+    }
 };
 
 // An item that begins in a CTA's run and ends in another's.
@@ -88,9 +99,14 @@ __device__ __forceinline__ void seq_rows(const AttnArgs& a, int s, int* begin, i
     *n = max(0, e - b);
 }
 
-// What a sequence asks of this kernel: items (0: nothing) of `steps` steps each.
+// What a sequence asks of this kernel: items (0: nothing) of `steps` steps
+// each.  An item costs as much again as kItemUnits steps (its queries, the
+// warps' results put together), so it counts steps + kItemUnits units.
+constexpr int kItemUnits = 2;
 struct SeqWork {
     int begin, n, len, items, steps;
+    __device__ __forceinline__ int units() const { return steps + kItemUnits; }
+    __device__ __forceinline__ int step(int unit) const { return max(0, unit - kItemUnits); }
 };
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int s) {
     SeqWork w;
@@ -106,15 +122,15 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int s) {
     return w;
 }
 
-// A place in the numbered steps.
+// A place in the numbered units.
 struct Cursor {
-    int s, item, step, left;  // left: steps up to the end of this CTA's run
+    int s, item, unit, left;  // left: units up to the end of this CTA's run
     SeqWork w;
-    __device__ __forceinline__ void next(const AttnArgs& a, int steps) {  // over `steps` steps inside the item
-        left -= steps;
-        step += steps;
-        if (step < w.steps) return;
-        step = 0;
+    __device__ __forceinline__ void next(const AttnArgs& a, int units) {  // over `units` units inside the item
+        left -= units;
+        unit += units;
+        if (unit < w.units()) return;
+        unit = 0;
         if (++item < w.items) return;
         item = 0;
         while (left > 0 && s + 1 < a.c.n_seqs) {
@@ -149,7 +165,7 @@ __device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t* s_warp, int64_t*
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -157,7 +173,7 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 // The product alone (accumulator 0).
 __device__ __forceinline__ void mma16816_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                               uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
@@ -224,13 +240,31 @@ __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity) {
 template <int HD>
 struct RowsSmem {
     static constexpr int kLd = HD + 8;  // row stride of the merge buffer: no two rows of a half warp in one bank
-    uint8_t ring[kRowWarps][kRowStages][Tile<HD>::kBytes];
+    uint8_t ring[kRowWarps][kRowStages][2 * Tile<HD>::kBytes];
+    uint4 qa[HD / 16][32];  // the query rows as operands: a k step of 16, a lane
+    uint32_t qs[2][32];     // and their groups' sums
     float o[kRowWarps][kRowTile][kLd];
     float ml[kRowWarps][kRowTile][2];
     uint64_t full[kRowWarps][kRowStages];
     int64_t scan[kRowWarps];
     int start[4];
 };
+
+// A place in a warp's ring.
+struct Stage {
+    uint32_t i = 0, parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++i == kRowStages) {
+            i = 0;
+            parity ^= 1u;
+        }
+    }
+};
+// A lane's offset into a tile, computed once: without this it is computed again for every tile.
+__device__ __forceinline__ uint32_t keep(uint32_t x) {
+    asm volatile("" : "+r"(x));
+    return x;
+}
 
 // Column r of a score tile i (and row of a values' operand) is this position of the tile: lane t of
 // a row group then holds the positions 4t .. 4t+3, whose scale rows lie in different banks for all t.
@@ -240,14 +274,15 @@ __device__ __forceinline__ int tile_pos(int i, int r) { return 4 * (r >> 1) + 2 
 
 template <int HD>
 __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(const RowsArgs ra) {
-    constexpr int G = Tile<HD>::G, KS = HD / 16;  // k steps of 16 for keys
+    constexpr int G = Tile<HD>::G;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     RowsSmem<HD>& sm = *reinterpret_cast<RowsSmem<HD>*>(smem_raw);
     const AttnArgs& a = ra.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
 
+    const uint32_t full = smem_addr(sm.full[warp]), ring = smem_addr(sm.ring[warp]);
     if (lane == 0) {
-        for (int i = 0; i < kRowStages; ++i) mbar_init(smem_addr(&sm.full[warp][i]), 1);
+        for (int i = 0; i < kRowStages; ++i) mbar_init(full + 8 * i, 1);
         fence_mbar_init();
     }
     // rows of no sequence
@@ -260,13 +295,13 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                 for (int j = threadIdx.x; j < a.n_head; j += kRowThreads) a.lse[row * a.n_head + j] = -INFINITY;
         }
     }
-    // all steps, and this CTA's run of them
+    // all units, and this CTA's run of them
     const int per = (a.c.n_seqs + kRowThreads - 1) / kRowThreads;
     const int s0 = min(a.c.n_seqs, (int)threadIdx.x * per), s1 = min(a.c.n_seqs, s0 + per);
     int64_t mine = 0;
     for (int s = s0; s < s1; ++s) {
         const SeqWork w = seq_work(a, s);
-        mine += (int64_t)w.items * w.steps;
+        mine += (int64_t)w.items * w.units();
     }
     int64_t all;
     const int64_t before = cta_scan(mine, sm.scan, &all);
@@ -278,11 +313,11 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
         int64_t at = before;
         for (int s = s0; s < s1; ++s) {
             const SeqWork w = seq_work(a, s);
-            const int64_t next = at + (int64_t)w.items * w.steps;
+            const int64_t next = at + (int64_t)w.items * w.units();
             if (run0 < next) {
                 sm.start[0] = s;
-                sm.start[1] = (int)((run0 - at) / w.steps);
-                sm.start[2] = (int)((run0 - at) % w.steps);
+                sm.start[1] = (int)((run0 - at) / w.units());
+                sm.start[2] = (int)((run0 - at) % w.units());
                 break;
             }
             at = next;
@@ -292,61 +327,81 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     Cursor cur;
     cur.s = sm.start[0];
     cur.item = sm.start[1];
-    cur.step = sm.start[2];
+    cur.unit = sm.start[2];
     cur.left = (int)(run1 - run0);
     cur.w = seq_work(a, cur.s);
 
-    // The producer runs ahead of the warp's own tiles; the page of its next
-    // tile is looked up one call before it is needed.
+    // The producer runs ahead of the warp's own tiles.  Lane i holds the places
+    // of the i-th of up to 32 pairs of one item and copies them itself.
     Cursor pro = cur;
-    int pro_id = 0, pro_head = 0, pro_at = -1;  // pro_at < 0: nothing left
-    int issued = 0;
-    auto seek = [&]() {
-        pro_at = -1;
-        while (pro.left > 0) {
-            const int p = (pro.step * kRowWarps + warp) * kTile;
-            const bool there = p < pro.w.len;
+    uint32_t pro_a = 0, pro_b = kNoTile;  // tiles of the pool, counted from the layer's first
+    int pro_i = 0, pro_n = 0;
+    Stage put, get;
+    auto place = [&](int tile) -> uint32_t {
+        const int slot = a.page_of(tile);
+        int id = a.c.page(pro.s, slot);
+        if (id < 0) id = 0;  // flagged; the copy has to stay inside the pool
+        return ((uint32_t)id * a.c.n_kv + pro.item / (pro.w.items / a.c.n_kv)) * a.page_tiles + (tile - slot * a.page_tiles);
+    };
+    auto refill = [&]() {
+        pro_i = pro_n = 0;
+        while (pro.left > 0 && pro_n == 0) {
+            const int units = min(32, min(pro.left, pro.w.units() - pro.unit));
+            const int step = pro.unit + lane - kItemUnits, tile = 2 * (step * kRowWarps + warp);
+            const bool there = lane < units && step >= 0 && tile * kTile < pro.w.len;
             if (there) {
-                pro_head = pro.item / (pro.w.items / a.c.n_kv);
-                pro_at = p;
-                pro_id = a.c.table[(int64_t)pro.s * a.c.max_pages + p / a.c.page_len];
+                pro_a = place(tile);
+                pro_b = (tile + 1) * kTile < pro.w.len ? place(tile + 1) : kNoTile;
             }
-            pro.next(a, 1);
-            if (there) return;
+            const uint32_t lanes = __ballot_sync(0xFFFFFFFFu, there);  // consecutive
+            if (lanes) {
+                pro_i = __ffs(lanes) - 1;
+                pro_n = pro_i + __popc(lanes);
+            }
+            pro.next(a, units);
         }
     };
     auto produce = [&]() {
-        if (pro_at < 0) return;
-        if (lane == 0) {
-            int id = pro_id;
-            if ((unsigned)id >= (unsigned)a.c.n_pages) {
-                atomicOr(&g_serve_status, kServeBadPage);
-                id = 0;
-            }
-            const int st = issued % kRowStages;
-            const uint32_t bar = smem_addr(&sm.full[warp][st]);
-            mbar_arrive_expect_tx(bar, Tile<HD>::kBytes);
-            bulk_g2s(smem_addr(sm.ring[warp][st]), a.c.tile<HD>(id, pro_head, pro_at % a.c.page_len), Tile<HD>::kBytes, bar);
+        if (pro_i == pro_n) {
+            refill();
+            if (pro_n == 0) return;
         }
-        ++issued;
-        seek();
+        if (lane == pro_i) {
+            const uint32_t bar = full + 8 * put.i, to = ring + put.i * (2 * Tile<HD>::kBytes);
+            const bool two = pro_b != kNoTile;
+            mbar_arrive_expect_tx(bar, two ? 2 * Tile<HD>::kBytes : Tile<HD>::kBytes);
+            bulk_g2s(to, a.c.pages + (uint64_t)pro_a * Tile<HD>::kBytes, Tile<HD>::kBytes, bar);
+            if (two) bulk_g2s(to + Tile<HD>::kBytes, a.c.pages + (uint64_t)pro_b * Tile<HD>::kBytes, Tile<HD>::kBytes, bar);
+        }
+        ++pro_i;
+        put.next();
     };
-    seek();
 #pragma unroll 1
     for (int i = 0; i < kRowStages; ++i) produce();
 
     bool alive = true;
-    int used = 0;
-    for (bool first = true; cur.left > 0; first = false) {
+    const uint32_t at_k = keep(tile_pos(0, r) * (HD / 2) + t * (HD / 8));                             // keys' numbers
+    const uint32_t at_m = keep(Tile<HD>::kScaleK + tile_pos(0, r) * (HD / 8) + t * 4);                // word (d, m) t
+    const uint32_t at_d0 = keep(Tile<HD>::kScaleK + (4 * t + (t >> 1)) * (HD / 8));                   // scale rows of
+    const uint32_t at_d1 = keep(Tile<HD>::kScaleK + (4 * t + 1 - (t >> 1)) * (HD / 8));               // two columns
+    const uint32_t at_v = keep(Tile<HD>::kV + lane * (HD / 8));                                       // values' numbers
+    const uint32_t low = keep(t < 2 ? 0x5410u : 0x1054u), high = keep(t < 2 ? 0x7632u : 0x3276u);
+    constexpr uint32_t kToV = Tile<HD>::kScaleV - Tile<HD>::kScaleK, kTwo = 2 * (HD / 8);             // two rows on
+    bool first = true;  // the run's first item
+    while (cur.left > 0) {
         // ---- one item (or the part of it inside the run)
-        const int steps = min(cur.left, cur.w.steps - cur.step), groups = cur.w.items / a.c.n_kv;
+        const int units = min(cur.left, cur.w.units() - cur.unit), groups = cur.w.items / a.c.n_kv;
+        const int step0 = cur.w.step(cur.unit), step1 = cur.w.step(cur.unit + units);
+        if (step0 == step1) {  // the run ends before the item's first step
+            cur.next(a, units);
+            continue;
+        }
         const int kvh = cur.item / groups, row0 = (cur.item - kvh * groups) * kRowTile;
         const int rows = min(kRowTile, cur.w.n * a.rep - row0);
         const int tok = (row0 + r) / a.rep;  // row r of the tile: token and head
         const int sees = r < rows ? cur.w.len - (cur.w.n - 1 - tok) : 0;
         const int sees_all = cur.w.len - (cur.w.n - 1 - row0 / a.rep);  // positions that every row sees
-        // the query row as operands: q * 2^k, its largest value in [2^9, 2^10)
-        uint32_t qa[KS][4], qs_hi = 0, qs_lo = 0;
+        // the query rows as operands: q * 2^k, the row's largest value in [2^9, 2^10); a group per warp
         float f_log2;  // score (log2) over what the products give
         {
             float q[G][8];
@@ -364,9 +419,11 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
 #pragma unroll
                     for (int n = 0; n < 8; ++n) q[g][n] = r < rows ? src[32 * g + n] : 0.f;
                 }
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int n = 0; n < 8; ++n) top = fmaxf(top, fabsf(q[g][n]));
-            }
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
             const int e = min(max((int)(__float_as_uint(top) >> 23), 30), 230);
@@ -374,6 +431,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
             f_log2 = a.scale * 1.44269504088896340736f * down;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
+                if (g != warp) continue;
                 float sum = 0.f;
 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
@@ -382,14 +440,21 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                 }
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-                if (t == g) split2(0.f, sum, &qs_hi, &qs_lo);
-                split2(q[g][0], q[g][4], &qa[2 * g][0], &qa[2 * g][1]);
-                split2(q[g][1], q[g][5], &qa[2 * g][2], &qa[2 * g][3]);
-                split2(q[g][2], q[g][6], &qa[2 * g + 1][0], &qa[2 * g + 1][1]);
-                split2(q[g][3], q[g][7], &qa[2 * g + 1][2], &qa[2 * g + 1][3]);
+                if (t == g) split2(0.f, sum, &sm.qs[0][lane], &sm.qs[1][lane]);
+                if (G == 2 && t == g + 2) sm.qs[0][lane] = sm.qs[1][lane] = 0u;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    uint4 x;
+                    split2(q[g][2 * k], q[g][2 * k + 4], &x.x, &x.y);
+                    split2(q[g][2 * k + 1], q[g][2 * k + 5], &x.z, &x.w);
+                    sm.qa[2 * g + k][lane] = x;
+                }
             }
         }
-        float2 o[G][4], om = make_float2(0.f, 0.f);  // values' numbers: [group][c], and the minima's part
+        __syncthreads();
+        const uint32_t qa = smem_addr(sm.qa) + 16 * lane, qs_hi = sm.qs[0][lane], qs_lo = sm.qs[1][lane];
+        float2 o[G][4];  // values' numbers less 8: [group][c]
+        float om = 0.f;  // and their middles, of group t
 #pragma unroll
         for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -397,67 +462,97 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
         float ref = -3.0e38f, l = 0.f;
 
 #pragma unroll 1
-        for (int i = 0; i < steps; ++i) {
-            const int p0 = ((cur.step + i) * kRowWarps + warp) * kTile;
+        for (int i = step0; i < step1; ++i) {
+            const int p0 = (i * kRowWarps + warp) * kPairLen;
             if (p0 >= cur.w.len) break;  // and so are the warp's further tiles
-            const int st = used % kRowStages;
-            if (alive) alive = wait_full(smem_addr(&sm.full[warp][st]), (uint32_t)(used / kRowStages) & 1u);
-            const uint32_t tile = smem_addr(sm.ring[warp][st]);
-            ++used;
-            // ---- scores of positions 4t .. 4t+3 for row r
-            float s[4];
+            if (alive) alive = wait_full(full + 8 * get.i, get.parity);
+            const uint32_t pair = ring + get.i * (2 * Tile<HD>::kBytes);
+            get.next();
+            // ---- scores of positions 4t .. 4t+3 of both tiles for row r
+            float s[2][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int pr = tile_pos(h, r);
-                uint32_t kw[G], d0[G], d1[G];
-                lds_words<G>(tile + pr * (HD / 2) + t * (HD / 8), kw);
-                lds_words<G>(tile + Tile<HD>::kScaleK + (4 * t + 2 * h + (t >> 1)) * (HD / 8), d0);
-                lds_words<G>(tile + Tile<HD>::kScaleK + (4 * t + 2 * h + 1 - (t >> 1)) * (HD / 8), d1);
-                uint32_t mw = 0;
-                if (G == 4 || t < G) mw = lds32(tile + Tile<HD>::kScaleK + pr * (HD / 8) + t * 4);
-                float cm[4];
-                mma16816_zero(cm, qs_hi, qs_lo, 0u, 0u, mw, 0u);
-                float2 acc = make_float2(0.f, 0.f);
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t tile = pair + u * Tile<HD>::kBytes;
+                uint32_t kw[2][G], kd[4][G];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    lds_words<G>(tile + at_k + h * HD, kw[h]);
+                    lds_words<G>(tile + at_d0 + h * kTwo, kd[2 * h]);
+                    lds_words<G>(tile + at_d1 + h * kTwo, kd[2 * h + 1]);
+                }
+                float2 acc[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float cm[4];
+                    mma16816_zero(cm, qs_hi, qs_lo, 0u, 0u, G == 4 || t < G ? lds32(tile + at_m + h * kTwo) : 0u, 0u);
+                    acc[h] = add2(make_float2(cm[0], cm[1]), make_float2(cm[2], cm[3]));
+                }
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    float c[4];
-                    const uint32_t w = kw[g], w8 = w >> 8;
-                    mma16816_zero(c, qa[2 * g][0], qa[2 * g][1], qa[2 * g][2], qa[2 * g][3], numbers<false>(w, 0.f),
-                                  numbers<true>(w, 0.f));
-                    mma16816(c, qa[2 * g + 1][0], qa[2 * g + 1][1], qa[2 * g + 1][2], qa[2 * g + 1][3],
-                             numbers<false>(w8, 0.f), numbers<true>(w8, 0.f));
-                    acc = __ffma2_rn(add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])),
-                                     make_float2(h2f(d0[g]), h2f(d1[g])), acc);
-                }
-                acc = add2(acc, add2(make_float2(cm[0], cm[1]), make_float2(cm[2], cm[3])));
-                s[2 * h] = acc.x * f_log2;
-                s[2 * h + 1] = acc.y * f_log2;
-            }
-            // ---- weights
-            uint32_t vd[4][G];  // (d, m) of the values of the lane's positions
+                    const uint4 q0 = lds128(qa + 1024 * g), q1 = lds128(qa + 1024 * g + 512);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                lds_words<G>(tile + Tile<HD>::kScaleV + (4 * t + (j ^ (t >> 1))) * (HD / 8), vd[j]);
-            const uint2 sv = lds64(tile + Tile<HD>::kScaleV + (lane & (HD / 4 - 1)) * 8);
-            uint32_t big = max(sv.x & 0x7FFFu, sv.y & 0x7FFFu);  // largest scale (bits) of two groups, of all in the warp
-            const bool edge = p0 + kTile > sees_all;
+                    for (int h = 0; h < 2; ++h) {
+                        float c[4];
+                        const uint32_t w = kw[h][g], w8 = w >> 8;
+                        mma16816_zero(c, q0.x, q0.y, q0.z, q0.w, numbers<false>(w, 0.f), numbers<true>(w, 0.f));
+                        mma16816(c, q1.x, q1.y, q1.z, q1.w, numbers<false>(w8, 0.f), numbers<true>(w8, 0.f));
+                        acc[h] = __ffma2_rn(add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])),
+                                            make_float2(h2f(kd[2 * h][g]), h2f(kd[2 * h + 1][g])), acc[h]);
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    s[u][2 * h] = acc[h].x * f_log2;
+                    s[u][2 * h + 1] = acc[h].y * f_log2;
+                }
+            }
+            // ---- the values' scales of the lane's positions as pairs, and whether one is large
+            __half2 d[2][2][G];
+            uint32_t big = 0;
+            const bool edge = p0 + kPairLen > sees_all;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t w0[G], w1[G];
+                    lds_words<G>(pair + u * Tile<HD>::kBytes + at_d0 + kToV + k * kTwo, w0);
+                    lds_words<G>(pair + u * Tile<HD>::kBytes + at_d1 + kToV + k * kTwo, w1);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) d[u][k][g] = bits_h2(__byte_perm(w0[g], w1[g], 0x5410));
+                }
             if (edge) {  // positions that the row does not see: whatever is stored there must not touch it
+                __syncwarp();
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (p0 + u * kTile + 4 * t + (j ^ (t >> 1)) >= sees) {
+                            s[u][j] = -INFINITY;
+#pragma unroll
+                            for (int g = 0; g < G; ++g)
+                                d[u][j >> 1][g] = bits_h2(h2bits(d[u][j >> 1][g]) & (j & 1 ? 0x0000FFFFu : 0xFFFF0000u));
+                        }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) big |= h2bits(d[u][k][g]);
+            float room = 14.f;
+            if (__any_sync(0xFFFFFFFFu, (big & 0x40004000u) != 0)) {  // a scale of 2 or more: p d stays below 2^15
                 big = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        if (p0 + 4 * t + (j ^ (t >> 1)) >= sees) {
-                            s[j] = -INFINITY;
-                            vd[j][g] = 0u;
-                        }
-                        big = max(big, vd[j][g] & 0x7FFFu);
-                    }
-            }
-            float room = 14.f;
-            if (__any_sync(0xFFFFFFFFu, big >= 0x4000u))  // a scale of 2 or more: p d stays below 2^15
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int g = 0; g < G; ++g) big = max(big, max(h2bits(d[u][k][g]) & 0x7FFFu, h2bits(d[u][k][g]) >> 16 & 0x7FFFu));
                 room = 14.f - (float)((int)(__reduce_max_sync(0xFFFFFFFFu, big) >> 10) - 15);
-            const float smax = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            }
+            // ---- weights
+            const float smax = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
             if (__any_sync(0xFFFFFFFFu, smax > ref + room)) {
                 float m = fmaxf(smax, __shfl_xor_sync(0xFFFFFFFFu, smax, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
@@ -470,70 +565,88 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                 for (int g = 0; g < G; ++g)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) o[g][c] = __fmul2_rn(o[g][c], k2);
-                om = __fmul2_rn(om, k2);
+                om *= keep;
             }
-            float p[4];
+            uint32_t ph[2][2], pl[2][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = exp2_fast(s[j] - ref);
-            l += (p[0] + p[1]) + (p[2] + p[3]);
-            uint32_t ph[2], pl[2];
-            split2(p[0], p[1], &ph[0], &pl[0]);
-            split2(p[2], p[3], &ph[1], &pl[1]);
+            for (int u = 0; u < 2; ++u) {
+                float p[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[j] = exp2_fast(s[u][j] - ref);
+                l += (p[0] + p[1]) + (p[2] + p[3]);
+                split2(p[0], p[1], &ph[u][0], &pl[u][0]);
+                split2(p[2], p[3], &ph[u][1], &pl[u][1]);
+                if (edge) {  // p . (m / 2 + 4 d) row by row, so that a NaN stays with the rows that see it
+                    __syncwarp();
+#pragma unroll 1
+                    for (int g = 0; g < G; ++g) {
+                        float x = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t w = lds32(pair + u * Tile<HD>::kBytes + (j & 1 ? at_d1 : at_d0) + kToV + (j >> 1) * kTwo + 4 * g);
+                            if (p0 + u * kTile + 4 * t + (j ^ (t >> 1)) < sees) x = fmaf(p[j], fmaf(4.f, h2f(w), 0.5f * h2f(w >> 16)), x);
+                        }
+                        x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
+                        x += __shfl_xor_sync(0xFFFFFFFFu, x, 2);
+                        if (t == g) om += x;
+                    }
+                }
+            }
             // ---- p . (m / 2 + 4 d): column 2g of the product, lanes of an even r
             if (!edge) {
-                uint32_t w[4];  // (d, m) of group r / 2 at the positions of the lane's operand
+                float chi[4], clo[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    w[j] = G == 4 || r < 4 ? lds32(tile + Tile<HD>::kScaleV + (4 * t + (j ^ (t >> 1))) * (HD / 8) + (r >> 1) * 4) : 0u;
-                uint32_t hi[2], lo[2];
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {  // (d, m) of group r / 2 at the positions of the lane's operand
+                        const uint32_t row = pair + u * Tile<HD>::kBytes + kToV + k * kTwo + (r >> 1) * 4;
+                        const uint32_t w0 = G == 4 || r < 4 ? lds32(row + at_d0) : 0u, w1 = G == 4 || r < 4 ? lds32(row + at_d1) : 0u;
+                        sum2(__hmul2(bits_h2(__byte_perm(w0, w1, 0x5410)), __float2half2_rn(4.f)),
+                             __hmul2(bits_h2(__byte_perm(w0, w1, 0x7632)), __float2half2_rn(0.5f)), &hi[k], &lo[k]);
+                    }
+                    if (u == 0) {
+                        mma16816_zero(chi, ph[u][0], pl[u][0], ph[u][1], pl[u][1], hi[0], hi[1]);
+                        mma16816_zero(clo, ph[u][0], pl[u][0], ph[u][1], pl[u][1], lo[0], lo[1]);
+                    } else {
+                        mma16816(chi, ph[u][0], pl[u][0], ph[u][1], pl[u][1], hi[0], hi[1]);
+                        mma16816(clo, ph[u][0], pl[u][0], ph[u][1], pl[u][1], lo[0], lo[1]);
+                    }
+                }
+                om += (chi[0] + chi[2]) + (clo[0] + clo[2]);
+            }
+            // ---- (p d) . (n - 8)
+            uint32_t v[2][2][G];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
-                    sum2(__hmul2(bits_h2(__byte_perm(w[2 * k], w[2 * k + 1], 0x5410)), __float2half2_rn(4.f)),
-                         __hmul2(bits_h2(__byte_perm(w[2 * k], w[2 * k + 1], 0x7632)), __float2half2_rn(0.5f)), &hi[k], &lo[k]);
-                float c[4];
-                mma16816_zero(c, ph[0], pl[0], ph[1], pl[1], lo[0], lo[1]);
-                om = add2(om, add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
-                mma16816_zero(c, ph[0], pl[0], ph[1], pl[1], hi[0], hi[1]);
-                om = add2(om, add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
-            } else {  // row by row, so that a NaN stays with the rows that see it
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    float x = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) x = fmaf(p[j], fmaf(4.f, h2f(vd[j][g]), 0.5f * h2f(vd[j][g] >> 16)), x);
-                    x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
-                    x += __shfl_xor_sync(0xFFFFFFFFu, x, 2);
-                    if (t == g) om.x += x;
-                }
-            }
-            // ---- (p d) . n
-            uint32_t va[G], vb[G];
-            lds_words<G>(tile + Tile<HD>::kV + lane * (HD / 8), va);
-            lds_words<G>(tile + Tile<HD>::kV + (32 + lane) * (HD / 8), vb);
-            const uint32_t low = t < 2 ? 0x5410u : 0x1054u, high = t < 2 ? 0x7632u : 0x3276u;
+                    lds_words<G>(pair + u * Tile<HD>::kBytes + at_v + k * (4 * HD), v[u][k]);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                uint32_t hi[2], lo[2];
+                float c[4][4];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const __half2 d = bits_h2(__byte_perm(vd[2 * k][g], vd[2 * k + 1][g], 0x5410));
-                    const __half2 h = __hmul2(bits_h2(ph[k]), d);
-                    hi[k] = h2bits(h);
-                    lo[k] = h2bits(__hfma2(bits_h2(pl[k]), d, __hfma2(bits_h2(ph[k]), d, __hneg2(h))));
-                }
-                const uint32_t sel = g & 1 ? high : low;
-                const uint32_t x0 = __byte_perm(va[g / 2], va[G / 2 + g / 2], sel), x1 = __byte_perm(vb[g / 2], vb[G / 2 + g / 2], sel);
-                const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
-                const uint32_t b[4][2] = {{numbers<false>(x0, -8.f), numbers<false>(x1, -8.f)},
-                                          {numbers<true>(x0, -8.f), numbers<true>(x1, -8.f)},
-                                          {numbers<false>(y0, -8.f), numbers<false>(y1, -8.f)},
-                                          {numbers<true>(y0, -8.f), numbers<true>(y1, -8.f)}};
+                for (int u = 0; u < 2; ++u) {
+                    uint32_t hi[2], lo[2], x[2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float c[4];
-                    mma16816_zero(c, hi[0], lo[0], hi[1], lo[1], b[j][0], b[j][1]);
-                    o[g][j] = add2(o[g][j], add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
+                    for (int k = 0; k < 2; ++k) {
+                        const __half2 h = __hmul2(bits_h2(ph[u][k]), d[u][k][g]);
+                        hi[k] = h2bits(h);
+                        lo[k] = h2bits(__hfma2(bits_h2(pl[u][k]), d[u][k][g], __hfma2(bits_h2(ph[u][k]), d[u][k][g], __hneg2(h))));
+                        x[k] = __byte_perm(v[u][k][g / 2], v[u][k][G / 2 + g / 2], g & 1 ? high : low);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t x0 = j < 2 ? x[0] : x[0] >> 8, x1 = j < 2 ? x[1] : x[1] >> 8;
+                        const uint32_t b0 = j & 1 ? numbers<true>(x0, -8.f) : numbers<false>(x0, -8.f);
+                        const uint32_t b1 = j & 1 ? numbers<true>(x1, -8.f) : numbers<false>(x1, -8.f);
+                        if (u == 0) mma16816_zero(c[j], hi[0], lo[0], hi[1], lo[1], b0, b1);
+                        else mma16816(c[j], hi[0], lo[0], hi[1], lo[1], b0, b1);
+                    }
                 }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    o[g][j] = add2(o[g][j], add2(make_float2(c[j][0], c[j][1]), make_float2(c[j][2], c[j][3])));
             }
             __syncwarp();
             produce();
@@ -546,7 +659,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
             // sums of p (m / 2 + 4 d): column 2g, i.e. lane t = g, element 0
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const float mid = __shfl_sync(0xFFFFFFFFu, om.x, (lane & ~3) + g);
+                const float mid = __shfl_sync(0xFFFFFFFFu, om, (lane & ~3) + g);
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     *reinterpret_cast<float2*>(&sm.o[warp][r][32 * g + 8 * c + 2 * t]) =
@@ -558,8 +671,9 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
             }
         }
         __syncthreads();
-        const bool whole = steps == cur.w.steps;
+        const bool whole = step1 - step0 == cur.w.steps;
         const int slot = 2 * blockIdx.x + (first ? 0 : 1);
+        first = false;
         for (int i = threadIdx.x; i < kRowTile * HD / 4; i += kRowThreads) {
             const int rr = i / (HD / 4), d = 4 * (i % (HD / 4));
             float m = sm.ml[0][rr][0];
@@ -587,63 +701,71 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                 if (d == 0) *reinterpret_cast<float2*>(ra.part_ml + (slot * kRowTile + rr) * 2) = make_float2(m, sum);
             }
         }
-        if (!whole && cur.step == 0 && threadIdx.x == 0) {  // the item begins here and ends in another CTA
-            const int64_t end = run1 - cur.left + cur.w.steps;  // number of the step after the item
+        if (!whole && step0 == 0 && threadIdx.x == 0) {  // the item begins here and ends in another CTA
+            const int64_t end = run1 - cur.left + cur.w.units() - cur.unit;  // number of the unit after the item
             ra.last[blockIdx.x] = Part{cur.s, cur.item, (int)((end * ctas - 1) / all) - (int)blockIdx.x + 1, slot};
         }
         __syncthreads();
-        cur.next(a, steps);
+        cur.next(a, units);
     }
     if (!alive)  // let the copies in flight land before the CTA ends
-        for (; used < issued; ++used) wait_full(smem_addr(&sm.full[warp][used % kRowStages]), (uint32_t)(used / kRowStages) & 1u);
+        for (; get.i != put.i || get.parity != put.parity; get.next()) wait_full(full + 8 * get.i, get.parity);
 }
 
 // The parts of the item that begins in CTA blockIdx.x's run and ends in
-// another's: its row blockIdx.y, the parts added in their order.
-constexpr int kJoinThreads = 512;
+// another's, added in their order: 128 threads per row, four values each.
+constexpr int kJoinThreads = 128 * kRowTile;
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const RowsArgs ra) {
-    constexpr int kGroups = kJoinThreads / HD;
-    __shared__ float s_w[kMaxRowCtas], s_max[kJoinThreads / 32], s_sum[kJoinThreads / 32], s_o[kJoinThreads];
+    constexpr int kLanes = HD / 4, kGroups = 128 / kLanes;
+    __shared__ float s_w[kRowTile][kMaxRowCtas], s_max[kRowTile][4], s_sum[kRowTile][4];
+    __shared__ __align__(16) float4 s_o[kRowTile][128];
     const AttnArgs& a = ra.a;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Part part = ra.last[blockIdx.x];
     if (!part.parts) return;
     const SeqWork w = seq_work(a, part.seq);
-    const int groups = w.items / a.c.n_kv, kvh = part.item / groups, row = (part.item - kvh * groups) * kRowTile + blockIdx.y;
-    if (row >= w.n * a.rep) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto slot = [&](int i) -> int64_t { return (int64_t)(i ? 2 * ((int)blockIdx.x + i) : part.slot) * kRowTile + blockIdx.y; };
+    const int groups = w.items / a.c.n_kv, kvh = part.item / groups;
+    const int rr = threadIdx.x >> 7, tid = threadIdx.x & 127, row = (part.item - kvh * groups) * kRowTile + rr;
+    auto slot = [&](int i) -> int64_t { return (int64_t)(i ? 2 * ((int)blockIdx.x + i) : part.slot) * kRowTile + rr; };
     float m = -3.0e38f;
-    for (int i = threadIdx.x; i < part.parts; i += kJoinThreads) m = fmaxf(m, ra.part_ml[2 * slot(i)]);
+    for (int i = tid; i < part.parts; i += 128) m = fmaxf(m, ra.part_ml[2 * slot(i)]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if (lane == 0) s_max[warp] = m;
+    if ((tid & 31) == 0) s_max[rr][tid >> 5] = m;
     __syncthreads();
-    for (int i = 0; i < kJoinThreads / 32; ++i) m = fmaxf(m, s_max[i]);
+    m = fmaxf(fmaxf(s_max[rr][0], s_max[rr][1]), fmaxf(s_max[rr][2], s_max[rr][3]));
     float sum = 0.f;
-    for (int i = threadIdx.x; i < part.parts; i += kJoinThreads) {
+    for (int i = tid; i < part.parts; i += 128) {
         const float2 x = *reinterpret_cast<const float2*>(ra.part_ml + 2 * slot(i));
-        s_w[i] = exp2_fast(x.x - m);
-        sum = fmaf(s_w[i], x.y, sum);
+        s_w[rr][i] = exp2_fast(x.x - m);
+        sum = fmaf(s_w[rr][i], x.y, sum);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if (lane == 0) s_sum[warp] = sum;
+    if ((tid & 31) == 0) s_sum[rr][tid >> 5] = sum;
     __syncthreads();
-    sum = 0.f;
-    for (int i = 0; i < kJoinThreads / 32; ++i) sum += s_sum[i];
-    const int d = threadIdx.x % HD, g = threadIdx.x / HD;
-    float x = 0.f;
+    sum = (s_sum[rr][0] + s_sum[rr][1]) + (s_sum[rr][2] + s_sum[rr][3]);
+    const int d = tid % kLanes, g = tid / kLanes;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = g; i < part.parts; i += kGroups) x = fmaf(s_w[i], ra.part_o[slot(i) * HD + d], x);
-    s_o[threadIdx.x] = x;
+    for (int i = g; i < part.parts; i += kGroups) {
+        const float k = s_w[rr][i];
+        const float4 y = *reinterpret_cast<const float4*>(ra.part_o + slot(i) * HD + 4 * d);
+        x.x = fmaf(k, y.x, x.x); x.y = fmaf(k, y.y, x.y); x.z = fmaf(k, y.z, x.z); x.w = fmaf(k, y.w, x.w);
+    }
+    s_o[rr][tid] = x;
     __syncthreads();
-    if (g) return;
+    if (g || row >= w.n * a.rep) return;
 #pragma unroll
-    for (int i = 1; i < kGroups; ++i) x += s_o[i * HD + d];
+    for (int i = 1; i < kGroups; ++i) {
+        const float4 y = s_o[rr][i * kLanes + d];
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
     const int64_t at = (int64_t)(w.begin + row / a.rep) * a.n_head + kvh * a.rep + row % a.rep;
-    a.out[at * HD + d] = sum == 0.f ? 0.f : __fdiv_rn(x, sum);
+    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+    *reinterpret_cast<float4*>(a.out + at * HD + 4 * d) =
+        sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
     if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (m + log2f(sum));
 }
 

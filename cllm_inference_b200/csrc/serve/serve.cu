@@ -60,7 +60,7 @@ int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
     CLLM_HOST_TRY(cudaGetLastError());
     if ((int64_t)a.c.max_pages * a.c.page_len > kStepLen) {  // an item can have more than one step
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(ctas, kRowTile);
+        cfg.gridDim = dim3(ctas);
         cfg.blockDim = dim3(kJoinThreads);
         cfg.stream = st;
         cudaLaunchAttribute pdl[1];
@@ -145,6 +145,8 @@ int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int
         return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: pages and out must be 16-byte aligned");
     if (ldq < (int64_t)n_head * head_dim)
         return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: a row is shorter than its heads");
+    if ((int64_t)n_pages * n_head_kv > (int64_t)0xFFFFFFFE / (page_len / kTile))
+        return host_fail(CLLM_ERR_TOO_LARGE, "kv4_attention: a layer of more than 2^32 tiles");
     int dev, sms;
     if (int rc = host_device(&dev, &sms)) return rc;
     AttnArgs a{};
@@ -154,6 +156,8 @@ int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int
     a.out = out; a.lse = lse;
     a.c = Cache{const_cast<uint8_t*>(static_cast<const uint8_t*>(pages)), page_table, seq_len, n_pages, page_len,
                 n_head_kv, n_seqs, max_pages};
+    a.page_tiles = page_len / kTile;
+    a.page_magic = (uint32_t)(((uint64_t(1) << 32) + a.page_tiles - 1) / a.page_tiles);
     return head_dim == 128 ? launch_attention<128>(a, dev, sms, static_cast<cudaStream_t>(stream))
                            : launch_attention<64>(a, dev, sms, static_cast<cudaStream_t>(stream));
 }

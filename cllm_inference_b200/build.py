@@ -74,7 +74,7 @@ def _run(cmd, verbose):
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> None:
     os.makedirs(LIB, exist_ok=True)
     header = os.path.join(INCLUDE, "cllm_cuda.h")
-    common = [os.path.join(CSRC, f) for f in ("common.cuh", "host.h")] + [header]
+    common = [os.path.join(CSRC, f) for f in ("common.cuh", "host.h", "tc_ptx.cuh")] + [header]
     units = {  # object -> (source, what it is built from)
         "cllm_cuda": (os.path.join(CSRC, "cllm_cuda.cu"), _sources(CSRC) + [header]),
         "serve": (os.path.join(CSRC, "serve", "serve.cu"), _sources(os.path.join(CSRC, "serve")) + common),

@@ -8,10 +8,10 @@
 #include <cmath>
 
 #include "kv4_append.cuh"
-#include "kv4_attention.cuh"
 #include "kv4_decode.cuh"
 #include "kv4_format.cuh"
 #include "kv4_pages.cuh"
+#include "kv4_prompt.cuh"
 #include "scores.cuh"
 
 namespace cllm {
@@ -48,6 +48,9 @@ int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
     cudaError_t attr = cudaSuccess;
     std::call_once(once[dev], [&] {
         attr = cudaFuncSetAttribute(kv4_rows_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(RowsSmem<HD>));
+        if (attr == cudaSuccess)
+            attr = cudaFuncSetAttribute(kv4_prompt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        sizeof(PromptSmem<HD>) + 1024);
     });
     CLLM_HOST_TRY(attr);
     const int ctas = std::min(kMaxRowCtas, kRowCtasPerSm * sms);
@@ -71,7 +74,11 @@ int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
         CLLM_HOST_TRY(cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD>, ra));
     }
     if (a.q_begin && (int64_t)a.n_tok * a.rep > a.rows_max) {
-        kv4_attention_kernel<HD><<<dim3(a.n_tok, (a.n_head + 3) / 4), 128, 0, st>>>(a);
+        // as many CTAs as there can be tiles of sequences with more rows than that
+        const int64_t rows = (int64_t)a.n_tok * a.rep, seqs = std::min<int64_t>(a.c.n_seqs, rows / (a.rows_max + 1));
+        const int64_t items = (rows / kPromptRows + seqs) * a.c.n_kv;
+        if (items > INT_MAX) return host_fail(CLLM_ERR_TOO_LARGE, "kv4_attention: too many rows in one call");
+        kv4_prompt_kernel<HD><<<(unsigned)items, kPromptThreads, sizeof(PromptSmem<HD>) + 1024, st>>>(a);
         CLLM_HOST_TRY(cudaGetLastError());
     }
     return CLLM_OK;

@@ -188,10 +188,12 @@ __device__ __forceinline__ uint32_t h2bits(__half2 h) { return *reinterpret_cast
 __device__ __forceinline__ __half2 bits_h2(uint32_t b) { return *reinterpret_cast<__half2*>(&b); }
 // (x, y) = hi + lo, each an fp16 pair, to 22 bits
 __device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t* lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    *hi = h2bits(h);
-    *lo = h2bits(__floats2half2_rn(x - f.x, y - f.y));
+    const uint32_t h = h2bits(__floats2half2_rn(x, y));
+    float ex, ey;  // hi - x, exact
+    asm("sub.rn.f32.f16 %0, %1, %2;" : "=f"(ex) : "h"((unsigned short)h), "f"(x));
+    asm("sub.rn.f32.f16 %0, %1, %2;" : "=f"(ey) : "h"((unsigned short)(h >> 16)), "f"(y));
+    *hi = h;
+    *lo = h2bits(__floats2half2_rn(-ex, -ey));
 }
 // The numbers in bits 0-3 (UP: 4-7) of both halves of w, plus `off`, as an fp16 pair.
 template <bool UP>

@@ -12,17 +12,22 @@
 //
 // What bounds it: three products a term, 6 * 128 * 64 * HD multiply-adds a tile
 // for 128 x 64 scores: 1536 cycles of the tensor cores (HD 128), beside which the
-// CTA's four schedulers issue some 500 (softmax) + 600 (numbers to fp16) + 130
+// CTA's four schedulers issue some 400 (softmax) + 750 (numbers to fp16) + 130
 // (sums) instructions each, and shared memory moves 96 KB of operands to the
 // tensor cores and 64 KB from the numbers: q and p come from TMEM, or the
 // operands alone would take all of its bandwidth.
 //
-// Warps (4 warpgroups; registers moved to where they are needed):
+// Work: tiles of (sequence, KV head, 128 rows), numbered through by
+// prompt_plan_kernel and cut into equal runs, one per SM; a run that ends inside an
+// item leaves a partial result for prompt_join_kernel.
+//
+// Warps (5 warpgroups; registers moved to where they are needed):
 //   0       raw tiles of the pages into a ring (bulk copies)
 //   1       TMEM, and the one thread that issues the products
 //   4..7    a row each: softmax with a running reference (kv4_decode.cuh), p to TMEM
 //   8..11   a row each: the fp32 sums of p v, and the output
-//   12..15  numbers and scales to fp16 operands in the 128-byte swizzle
+//   12..15  the keys' numbers and scales to fp16 operands in the 128-byte swizzle
+//   16..19  the values'
 // All waits are bounded; one that expires sets the status, and the CTA runs to its
 // end without waiting.
 #pragma once
@@ -32,9 +37,12 @@
 namespace cllm {
 namespace serve {
 
-constexpr int kPromptThreads = 512;
+constexpr int kPromptThreads = 640;
+constexpr int kPromptUnits = 3;  // an item costs as much again as this many tiles
+constexpr int kPromptMinRun = 6;
 constexpr int kPromptRows = 128, kPromptCols = 64;
 constexpr int kRawStages = 3;
+constexpr int kStats = 8;  // the operands' warps are at most 7 tiles ahead of the softmax (raw ring, then theirs)
 
 template <int HD>
 struct PromptSmem {
@@ -43,22 +51,21 @@ struct PromptSmem {
     uint8_t v[2][2][kOperand];  // [stage][hi, lo]: [value][128 bytes of positions]
     uint8_t raw[kRawStages][4 * Tile<HD>::kBytes];
     float alpha[4][kPromptRows];  // what a tile's new reference leaves of the sums
-    float sum[kPromptRows];
-    uint32_t bad[kPromptRows];    // groups that a NaN of the values reaches
+    float sum[2][kPromptRows], ref[2][kPromptRows];  // of an item: its rows' sums of weights and references
+    uint32_t bad[2][kPromptRows];                    // groups that a NaN of the values reaches
     struct Stat {
         float k_down, v_up;  // 2^-(the keys' power), 2^(the values' power)
         int v_power;
         uint32_t bad;        // 1: a value has a NaN
-    } stat[4];
-    uint32_t top[4][4][2];        // [tile][warp]: largest exponents of keys and values
-    uint32_t warp_bad[4][4];
-    uint8_t nan[4][kPromptCols];  // groups of a position that are NaN
+    } stat[kStats];
+    uint32_t top[2][kStats][4];  // [keys, values][tile][warp]: largest exponent
+    uint32_t warp_bad[kStats][4];
+    uint8_t nan[kStats][kPromptCols];  // groups of a position that are NaN
     uint64_t raw_full[kRawStages], raw_empty[kRawStages];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], o_empty[2];
-    uint64_t alpha_full[4], stat_full[4], q_full, done;
+    uint64_t alpha_full[4], stat_full[kStats], q_full, done;
     uint32_t tmem;
     int abort;
-    int item[4];
 };
 
 __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -107,29 +114,145 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
 
 // Two values as an fp16 pair and what is left of them as another.
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) { split2(x, y, &hi, &lo); }
-
-// The item of CTA blockIdx.x: sequence, KV head, tile of 128 rows (the last, longest, first).
-__device__ __forceinline__ bool prompt_item(const AttnArgs& a, int* out) {
-    int left = blockIdx.x;
-    for (int s = 0; s < a.c.n_seqs; ++s) {
-        int begin, n;
-        seq_rows(a, s, &begin, &n);
-        const int64_t rows = (int64_t)n * a.rep;
-        if (rows <= a.rows_max) continue;
-        const int tiles = (int)((rows + kPromptRows - 1) / kPromptRows);
-        if (left < tiles * a.c.n_kv) {
-            out[0] = s;
-            out[1] = left % a.c.n_kv;
-            out[2] = tiles - 1 - left / a.c.n_kv;
-            return true;
-        }
-        left -= tiles * a.c.n_kv;
-    }
-    return false;
+// n * d + m in fp32 of the halves NI of n and DI of d.
+template <int NI, int DI>
+__device__ __forceinline__ float number_value(uint32_t n, uint32_t d, uint32_t m) {
+    const unsigned short nh = NI ? (unsigned short)(n >> 16) : (unsigned short)n;
+    const unsigned short dh = DI ? (unsigned short)(d >> 16) : (unsigned short)d;
+    float v;
+    asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(v) : "h"(nh), "h"(dh), "f"(__uint_as_float(m)));
+    return v;
+}
+// The values of two numbers, split: SEL 0 and 1, the low and the high halves of
+// nx and ny; 2, both halves of nx.  d in the low halves of dx and dy.
+template <int SEL>
+__device__ __forceinline__ void value_pair(uint32_t nx, uint32_t ny, uint32_t dx, uint32_t dy, uint32_t mx, uint32_t my,
+                                           uint32_t& hi, uint32_t& lo) {
+    const float x = number_value<SEL == 1, 0>(nx, dx, mx), y = number_value<SEL != 0, 0>(ny, dy, my);
+    split_pair(x, y, hi, lo);
 }
 
+// 128 rows of a sequence, for every KV head: its tiles per head, and where its units begin.
+struct PromptItem {
+    int seq, block, tiles, pad;
+    int64_t unit;  // units (tiles + kPromptUnits, times KV heads) of the items before it
+};
+// An item that begins in a CTA's run and ends in another's.
+struct PromptPart {
+    int item, kvh, parts, slot;
+};
+struct PromptArgs {
+    AttnArgs a;
+    int most;            // room for items
+    PromptItem* items;   // [most + 1]; the last one's unit is the total
+    int* seq_items;      // [n_seqs] scratch
+    int* count;          // items
+    PromptPart* last;    // [ctas]
+    float* part_ml;      // [2 * ctas][128][2]
+    uint32_t* part_bad;  // [2 * ctas][128]
+    float* part_o;       // [2 * ctas][128][HD]
+};
+
+__device__ __forceinline__ int prompt_tiles(int len, int n, int rep, int block) {
+    const int last = (int)(min((int64_t)(block + 1) * kPromptRows, (int64_t)n * rep) - 1) / rep;  // token of the last row
+    return (max(0, len - (n - 1 - last)) + kPromptCols - 1) / kPromptCols;
+}
+
+// The list of items, one CTA: items per sequence, their prefix sum, then the
+// tiles of each and theirs.
+constexpr int kPromptPlanThreads = 1024;
+__global__ void __launch_bounds__(kPromptPlanThreads) prompt_plan_kernel(const PromptArgs p) {
+    __shared__ int64_t s_warp[32];
+    const AttnArgs& a = p.a;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto scan = [&](int64_t v, int64_t* total) -> int64_t {  // exclusive
+        int64_t x = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) s_warp[warp] = x;
+        __syncthreads();
+        int64_t w = s_warp[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xFFFFFFFFu, w, o);
+            if (lane >= o) w += y;
+        }
+        *total = __shfl_sync(0xFFFFFFFFu, w, 31);
+        const int64_t before = __shfl_sync(0xFFFFFFFFu, w, max(0, warp - 1));
+        return x - v + (warp ? before : 0);
+    };
+    int64_t count = 0;
+    for (int base = 0; base < a.c.n_seqs; base += kPromptPlanThreads) {
+        const int s = base + threadIdx.x;
+        int64_t blocks = 0, total;
+        if (s < a.c.n_seqs) {
+            int begin, n;
+            seq_rows(a, s, &begin, &n);
+            const int64_t rows = (int64_t)n * a.rep;
+            if (rows > a.rows_max) blocks = (rows + kPromptRows - 1) / kPromptRows;
+        }
+        const int64_t at = count + scan(blocks, &total);
+        if (s < a.c.n_seqs) p.seq_items[s] = (int)min(at, (int64_t)p.most);
+        count += total;
+    }
+    count = min(count, (int64_t)p.most);
+    __syncthreads();
+    int64_t units = 0;
+    for (int64_t base = 0; base < count; base += kPromptPlanThreads) {
+        const int i = (int)base + threadIdx.x;
+        PromptItem it{};
+        int64_t mine = 0, total;
+        if (i < count) {
+            int lo = 0, hi = a.c.n_seqs - 1;  // the last sequence whose first item is at most i
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (p.seq_items[mid] <= i) lo = mid;
+                else hi = mid - 1;
+            }
+            int begin, n;
+            seq_rows(a, lo, &begin, &n);
+            it.seq = lo;
+            it.block = i - p.seq_items[lo];
+            it.tiles = prompt_tiles(a.c.length(lo), n, a.rep, it.block);
+            mine = (int64_t)(it.tiles + kPromptUnits) * a.c.n_kv;
+        }
+        it.unit = units + scan(mine, &total);
+        if (i < count) p.items[i] = it;
+        units += total;
+    }
+    if (threadIdx.x == 0) {
+        p.items[count].unit = units;
+        *p.count = (int)count;
+    }
+}
+
+// A place in the numbered units.
+struct PromptCursor {
+    int item, kvh, unit, tiles;
+    int64_t left;
+    // Step over what the run has of this item; its tiles are [*from, *to).
+    __device__ __forceinline__ void range(int* from, int* to) const {
+        *from = max(0, unit - kPromptUnits);
+        *to = max(0, (int)min((int64_t)unit + left, (int64_t)tiles + kPromptUnits) - kPromptUnits);
+    }
+    __device__ __forceinline__ void next(const PromptArgs& p) {
+        left -= tiles + kPromptUnits - unit;
+        unit = 0;
+        if (left > 0 && ++kvh == p.a.c.n_kv) {
+            kvh = 0;
+            tiles = p.items[++item].tiles;
+        }
+    }
+    // Whether the run has something of this item to do: a tile of it, or an item without any.
+    __device__ __forceinline__ bool here(int from, int to) const { return from < to || (tiles == 0 && unit == 0); }
+};
+
 template <int HD>
-__global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const PromptArgs p) {
     constexpr int G = Tile<HD>::G;
     constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kPromptCols >> 3) << 17) | ((uint32_t)(kPromptRows >> 4) << 24);
     constexpr uint32_t kIdescO = (1u << 4) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPromptRows >> 4) << 24);
@@ -137,15 +260,38 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
     extern __shared__ uint8_t smem_raw[];
     PromptSmem<HD>& sm =
         *reinterpret_cast<PromptSmem<HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const AttnArgs& a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort = &sm.abort;
     auto bar = [](uint64_t& b) { return smem_addr(&b); };
 
+    // this CTA's run of the units
+    const int count = *p.count;
+    const int64_t all = count ? p.items[count].unit : 0;
+    const int ctas = (int)min((int64_t)gridDim.x, (all + kPromptMinRun - 1) / kPromptMinRun);
+    if (threadIdx.x == 0) p.last[blockIdx.x].parts = 0;
+    if ((int)blockIdx.x >= ctas) return;
+    const int64_t run0 = blockIdx.x * all / ctas, run1 = (blockIdx.x + 1) * all / ctas;
+    PromptCursor cur;
+    {
+        int lo = 0, hi = count - 1;  // the last item that begins at or before run0
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (p.items[mid].unit <= run0) lo = mid;
+            else hi = mid - 1;
+        }
+        cur.item = lo;
+        cur.tiles = p.items[lo].tiles;
+        const int64_t at = run0 - p.items[lo].unit;
+        cur.kvh = (int)(at / (cur.tiles + kPromptUnits));
+        cur.unit = (int)(at - (int64_t)cur.kvh * (cur.tiles + kPromptUnits));
+        cur.left = run1 - run0;
+    }
+
     if (threadIdx.x == 0) {
-        sm.item[3] = prompt_item(a, sm.item);
         for (int i = 0; i < kRawStages; ++i) {
             mbar_init(bar(sm.raw_full[i]), 1);
-            mbar_init(bar(sm.raw_empty[i]), 4);
+            mbar_init(bar(sm.raw_empty[i]), 8);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(sm.k_full[i]), 4);
@@ -157,17 +303,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
             mbar_init(bar(sm.o_full[i]), 1);
             mbar_init(bar(sm.o_empty[i]), 4);
         }
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(bar(sm.alpha_full[i]), 4);
-            mbar_init(bar(sm.stat_full[i]), 1);
-        }
+        for (int i = 0; i < 4; ++i) mbar_init(bar(sm.alpha_full[i]), 4);
+        for (int i = 0; i < kStats; ++i) mbar_init(bar(sm.stat_full[i]), 2);
         mbar_init(bar(sm.q_full), 4);
         mbar_init(bar(sm.done), 1);
         sm.abort = 0;
         fence_mbar_init();
     }
-    __syncthreads();
-    if (!sm.item[3]) return;  // fewer items than CTAs
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -177,377 +319,426 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sm.tmem);
 
-    const int seq = sm.item[0], kvh = sm.item[1], row0 = sm.item[2] * kPromptRows;
-    int begin, n;
-    seq_rows(a, seq, &begin, &n);
-    const int len = a.c.length(seq);
-    const int last = (int)(min((int64_t)row0 + kPromptRows, (int64_t)n * a.rep) - 1) / a.rep;  // token of the last row
-    const int tiles = (max(0, len - (n - 1 - last)) + kPromptCols - 1) / kPromptCols;
-
+    // Every role walks the same run; `it` counts its tiles, and barrier phases go by it.
+    int it = 0, from, to;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 0) {
             // ---- raw tiles
-            int issued = 0;
-            for (int i = 0; i < tiles && !*abort; ++i) {
-                const int st = i % kRawStages, tile = 4 * i + lane;
-                if (i >= kRawStages) warp_wait(bar(sm.raw_empty[st]), (uint32_t)(i / kRawStages - 1) & 1u, abort);
-                const bool there = lane < 4 && tile * kTile < len;
-                const uint32_t count = __popc(__ballot_sync(0xFFFFFFFFu, there));
-                if (*abort) break;
-                if (lane == 0) mbar_arrive_expect_tx(bar(sm.raw_full[st]), count * Tile<HD>::kBytes);
-                __syncwarp();
-                if (there) {
-                    const int slot = a.page_of(tile);
-                    const int id = max(0, a.c.page(seq, slot));  // a bad one is flagged; the copy stays inside the pool
-                    bulk_g2s(smem_addr(sm.raw[st]) + lane * Tile<HD>::kBytes,
-                             a.c.pages + (((int64_t)id * a.c.n_kv + kvh) * a.page_tiles + (tile - slot * a.page_tiles)) * Tile<HD>::kBytes,
-                             Tile<HD>::kBytes, bar(sm.raw_full[st]));
+            for (; cur.left > 0; cur.next(p)) {
+                cur.range(&from, &to);
+                if (from >= to) continue;
+                const int seq = p.items[cur.item].seq, len = a.c.length(seq);
+                for (int i = from; i < to && !*abort; ++i) {
+                    const int st = it % kRawStages, tile = 4 * i + lane;
+                    const bool there = lane < 4 && tile * kTile < len;
+                    int64_t src = 0;
+                    if (there) {
+                        const int slot = a.page_of(tile);
+                        const int id = max(0, a.c.page(seq, slot));  // a bad one is flagged; the copy stays inside the pool
+                        src = (((int64_t)id * a.c.n_kv + cur.kvh) * a.page_tiles + (tile - slot * a.page_tiles)) * Tile<HD>::kBytes;
+                    }
+                    if (it >= kRawStages) warp_wait(bar(sm.raw_empty[st]), (uint32_t)(it / kRawStages - 1) & 1u, abort);
+                    const uint32_t n = __popc(__ballot_sync(0xFFFFFFFFu, there));
+                    const int dead = __shfl_sync(0xFFFFFFFFu, *abort, 0);
+                    if (dead) break;
+                    if (lane == 0) mbar_arrive_expect_tx(bar(sm.raw_full[st]), n * Tile<HD>::kBytes);
+                    __syncwarp();
+                    if (there) bulk_g2s(smem_addr(sm.raw[st]) + lane * Tile<HD>::kBytes, a.c.pages + src, Tile<HD>::kBytes, bar(sm.raw_full[st]));
+                    ++it;
                 }
-                issued = i + 1;
             }
             if (*abort)  // let the copies in flight land
-                for (int i = max(0, issued - kRawStages); i < issued; ++i) wait_full(bar(sm.raw_full[i % kRawStages]), (uint32_t)(i / kRawStages) & 1u);
+                for (int i = max(0, it - kRawStages); i < it; ++i) wait_full(bar(sm.raw_full[i % kRawStages]), (uint32_t)(i / kRawStages) & 1u);
         } else if (warp == 1 && lane == 0) {
-            // ---- products
-            wait_or_abort(bar(sm.q_full), 0, abort);
-            tc_fence_after();
-            for (int i = 0; i <= tiles; ++i) {
-                if (i < tiles) {  // S = q k, into the buffer that the products of p(i - 2), issued before, have read
-                    const int st = i & 1;
-                    wait_or_abort(bar(sm.k_full[st]), (uint32_t)(i >> 1) & 1u, abort);
+            // ---- products: S of a tile, then O of the one before it
+            auto values = [&](int j) {
+                const int st = j & 1;
+                wait_or_abort(bar(sm.p_full[st]), (uint32_t)(j >> 1) & 1u, abort);
+                wait_or_abort(bar(sm.v_full[st]), (uint32_t)(j >> 1) & 1u, abort);
+                if (j >= 2) wait_or_abort(bar(sm.o_empty[st]), (uint32_t)((j >> 1) - 1) & 1u, abort);
+                tc_fence_after();
+                const uint32_t d = tmem + kColO + 128 * st;
+                for (int term = 0; term < 3; ++term) {  // lo hi, hi lo, hi hi
+                    const uint32_t w = tmem + kColS + 64 * st + (term == 0 ? 32 : 0), v = smem_addr(sm.v[st][term == 1]);
+                    for (int s = 0; s < kPromptCols / 16; ++s) tc_mma_ts(d, w + 8 * s, umma_desc_sw128(v + s * 32), kIdescO, term | s);
+                }
+                tc_commit(bar(sm.o_full[st]));
+                tc_commit(bar(sm.v_empty[st]));
+            };
+            for (int items = 0; cur.left > 0; cur.next(p)) {
+                cur.range(&from, &to);
+                if (!cur.here(from, to)) continue;
+                wait_or_abort(bar(sm.q_full), (uint32_t)(items++) & 1u, abort);
+                tc_fence_after();
+                for (int i = from; i < to; ++i, ++it) {
+                    // S goes into the buffer that the products of p two tiles ago, issued before, have read
+                    const int st = it & 1;
+                    wait_or_abort(bar(sm.k_full[st]), (uint32_t)(it >> 1) & 1u, abort);
                     tc_fence_after();
                     const uint32_t d = tmem + kColS + 64 * st;
-                    for (int term = 0; term < 3; ++term) {  // lo hi, hi lo, hi hi
+                    for (int term = 0; term < 3; ++term) {
                         const uint32_t q = tmem + kColQ + (term == 0 ? HD / 2 : 0), k = smem_addr(sm.k[st][term == 1]);
                         for (int s = 0; s < HD / 16; ++s)
                             tc_mma_ts(d, q + 8 * s, umma_desc_sw128(k + (s / 4) * (kPromptCols * 128) + (s % 4) * 32), kIdescS, term | s);
                     }
                     tc_commit(bar(sm.s_full[st]));
                     tc_commit(bar(sm.k_empty[st]));
+                    if (i > from) values(it - 1);
                 }
-                if (i > 0) {  // O = p v of the tile before
-                    const int j = i - 1, st = j & 1;
-                    wait_or_abort(bar(sm.p_full[st]), (uint32_t)(j >> 1) & 1u, abort);
-                    wait_or_abort(bar(sm.v_full[st]), (uint32_t)(j >> 1) & 1u, abort);
-                    if (j >= 2) wait_or_abort(bar(sm.o_empty[st]), (uint32_t)((j >> 1) - 1) & 1u, abort);
-                    tc_fence_after();
-                    const uint32_t d = tmem + kColO + 128 * st;
-                    for (int term = 0; term < 3; ++term) {
-                        const uint32_t p = tmem + kColS + 64 * st + (term == 0 ? 32 : 0), v = smem_addr(sm.v[st][term == 1]);
-                        for (int s = 0; s < kPromptCols / 16; ++s) tc_mma_ts(d, p + 8 * s, umma_desc_sw128(v + s * 32), kIdescO, term | s);
-                    }
-                    tc_commit(bar(sm.o_full[st]));
-                    tc_commit(bar(sm.v_empty[st]));
-                }
+                if (from < to) values(it - 1);
             }
             tc_commit(bar(sm.done));
             wait_full(bar(sm.done), 0);
         }
     } else if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
         // ---- softmax: thread = row
-        const int row = 32 * (warp - 4) + lane, j = row0 + row;
+        const int row = 32 * (warp - 4) + lane;
         const uint32_t lanes = (uint32_t)(32 * (warp - 4)) << 16;
-        const bool on = j < n * a.rep;
-        const int tok = j / a.rep, head = kvh * a.rep + j % a.rep;
-        const int sees = on ? max(0, len - (n - 1 - tok)) : 0;
-        const float* src = a.q + (int64_t)(begin + tok) * a.ldq + head * HD;
         const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (a.ldq * 4)) & 15) == 0;
-        float f_log2;
-        {
-            float top = 0.f;
-            if (on) {
-                if (vec) {
-                    for (int i = 0; i < HD; i += 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(src + i);
-                        top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+        for (int items = 0; cur.left > 0; cur.next(p)) {
+            cur.range(&from, &to);
+            if (!cur.here(from, to)) continue;
+            const int seq = p.items[cur.item].seq, j = p.items[cur.item].block * kPromptRows + row, len = a.c.length(seq);
+            int begin, n;
+            seq_rows(a, seq, &begin, &n);
+            const bool on = j < n * a.rep;
+            const int sees = on ? max(0, len - (n - 1 - j / a.rep)) : 0;
+            const float* src = a.q + (int64_t)(begin + j / a.rep) * a.ldq + (cur.kvh * a.rep + j % a.rep) * HD;
+            float f_log2;
+            {
+                float top = 0.f;
+                if (on) {
+                    if (vec) {
+                        for (int i = 0; i < HD; i += 4) {
+                            const float4 x = *reinterpret_cast<const float4*>(src + i);
+                            top = fmaxf(fmaxf(top, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+                        }
+                    } else {
+                        for (int i = 0; i < HD; ++i) top = fmaxf(top, fabsf(src[i]));
                     }
+                }
+                const int e = min(max((int)(__float_as_uint(top) >> 23), 30), 230);
+                const float up = __uint_as_float((uint32_t)(263 - e) << 23);  // the row's largest value to [2^9, 2^10)
+                f_log2 = a.scale * 1.44269504088896340736f * __uint_as_float((uint32_t)(e - 9) << 23);
+#pragma unroll 1
+                for (int i = 0; i < HD; i += 32) {
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (on) {
+                            if (vec) x = *reinterpret_cast<const float4*>(src + i + k);
+                            else x = make_float4(src[i + k], src[i + k + 1], src[i + k + 2], src[i + k + 3]);
+                        }
+                        split_pair(x.x * up, x.y * up, hi[k / 2], lo[k / 2]);
+                        split_pair(x.z * up, x.w * up, hi[k / 2 + 1], lo[k / 2 + 1]);
+                    }
+                    tmem_st16u(tmem + lanes + kColQ + i / 2, hi);
+                    tmem_st16u(tmem + lanes + kColQ + HD / 2 + i / 2, lo);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                warp_arrive(bar(sm.q_full));
+            }
+            float ref = -3.0e38f, l = 0.f;
+            uint32_t bad = 0;
+#pragma unroll 1
+            for (int i = from; i < to; ++i, ++it) {
+                const int st = it & 1, r4 = it & 3, rs = it % kStats;
+                warp_wait(bar(sm.stat_full[rs]), (uint32_t)(it / kStats) & 1u, abort);
+                warp_wait(bar(sm.s_full[st]), (uint32_t)(it >> 1) & 1u, abort);
+                tc_fence_after();
+                const float f = f_log2 * sm.stat[rs].k_down, v_up = sm.stat[rs].v_up;
+                const int v_power = sm.stat[rs].v_power;
+                const uint32_t col = tmem + lanes + kColS + 64 * st;
+                uint32_t x[4][16];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld16_issue(col + 16 * c, x[c]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_wait(x[c]);
+                const int limit = sees - i * kPromptCols;  // columns that the row sees
+                if (__any_sync(0xFFFFFFFFu, limit < kPromptCols)) {
+                    __syncwarp();
+                    const uint32_t none = __float_as_uint(f < 0.f ? INFINITY : -INFINITY);
+#pragma unroll
+                    for (int c = 0; c < kPromptCols; ++c)
+                        if (c >= limit) x[c / 16][c % 16] = none;
+                }
+                if (sm.stat[rs].bad)
+                    for (int c = 0; c < min(limit, kPromptCols); ++c) bad |= sm.nan[rs][c];
+                float m[4];
+                if (f >= 0.f) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        m[c] = __uint_as_float(x[c][0]);
+#pragma unroll
+                        for (int k = 1; k < 16; ++k) m[c] = fmaxf(m[c], __uint_as_float(x[c][k]));
+                    }
+                    m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                 } else {
-                    for (int i = 0; i < HD; ++i) top = fmaxf(top, fabsf(src[i]));
-                }
-            }
-            const int e = min(max((int)(__float_as_uint(top) >> 23), 30), 230);
-            const float up = __uint_as_float((uint32_t)(263 - e) << 23);  // the row's largest value to [2^9, 2^10)
-            f_log2 = a.scale * 1.44269504088896340736f * __uint_as_float((uint32_t)(e - 9) << 23);
-#pragma unroll 1
-            for (int i = 0; i < HD; i += 32) {
-                uint32_t hi[16], lo[16];
 #pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (on) {
-                        if (vec) x = *reinterpret_cast<const float4*>(src + i + k);
-                        else x = make_float4(src[i + k], src[i + k + 1], src[i + k + 2], src[i + k + 3]);
+                    for (int c = 0; c < 4; ++c) {
+                        m[c] = __uint_as_float(x[c][0]);
+#pragma unroll
+                        for (int k = 1; k < 16; ++k) m[c] = fminf(m[c], __uint_as_float(x[c][k]));
                     }
-                    split_pair(x.x * up, x.y * up, hi[k / 2], lo[k / 2]);
-                    split_pair(x.z * up, x.w * up, hi[k / 2 + 1], lo[k / 2 + 1]);
+                    m[0] = fminf(fminf(m[0], m[1]), fminf(m[2], m[3]));
                 }
-                tmem_st16u(tmem + lanes + kColQ + i / 2, hi);
-                tmem_st16u(tmem + lanes + kColQ + HD / 2 + i / 2, lo);
-            }
-            tmem_st_wait();
-            tc_fence_before();
-            warp_arrive(bar(sm.q_full));
-        }
-        float ref = -3.0e38f, l = 0.f;
-        uint32_t bad = 0;
-#pragma unroll 1
-        for (int i = 0; i < tiles; ++i) {
-            const int st = i & 1, r4 = i & 3;
-            warp_wait(bar(sm.stat_full[r4]), (uint32_t)(i >> 2) & 1u, abort);
-            warp_wait(bar(sm.s_full[st]), (uint32_t)(i >> 1) & 1u, abort);
-            tc_fence_after();
-            const float f = f_log2 * sm.stat[r4].k_down, v_up = sm.stat[r4].v_up;
-            const int v_power = sm.stat[r4].v_power;
-            const uint32_t col = tmem + lanes + kColS + 64 * st;
-            uint32_t x[4][16];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld16_issue(col + 16 * c, x[c]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld_wait(x[c]);
-            const int limit = sees - i * kPromptCols;  // columns that the row sees
-            if (__any_sync(0xFFFFFFFFu, limit < kPromptCols)) {
-                const uint32_t none = __float_as_uint(f < 0.f ? INFINITY : -INFINITY);
-#pragma unroll
-                for (int c = 0; c < kPromptCols; ++c)
-                    if (c >= limit) x[c / 16][c % 16] = none;
-            }
-            if (sm.stat[r4].bad)
-                for (int c = 0; c < min(limit, kPromptCols); ++c) bad |= sm.nan[r4][c];
-            float m[4];
-            if (f >= 0.f) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    m[c] = __uint_as_float(x[c][0]);
-#pragma unroll
-                    for (int k = 1; k < 16; ++k) m[c] = fmaxf(m[c], __uint_as_float(x[c][k]));
+                const float top = m[0] * f, room = 14.f + (float)min(0, v_power);
+                float alpha = 1.f;
+                if (top > ref + room) {
+                    const float now = top - (room - 4.f);
+                    alpha = exp2_fast(ref - now);
+                    ref = now;
                 }
-                m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-            } else {
+                sm.alpha[r4][row] = alpha;
+                const float off = -ref - (float)v_power;
+                const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
+                float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    m[c] = __uint_as_float(x[c][0]);
+                for (int c = 0; c < 2; ++c) {  // 32 columns at a time: p hi and lo take the place of the scores
+                    uint32_t hi[16], lo[16];
 #pragma unroll
-                    for (int k = 1; k < 16; ++k) m[c] = fminf(m[c], __uint_as_float(x[c][k]));
-                }
-                m[0] = fminf(fminf(m[0], m[1]), fminf(m[2], m[3]));
-            }
-            const float top = m[0] * f, room = 14.f + (float)min(0, v_power);
-            float alpha = 1.f;
-            if (top > ref + room) {
-                const float to = top - (room - 4.f);
-                alpha = exp2_fast(ref - to);
-                ref = to;
-            }
-            sm.alpha[r4][row] = alpha;
-            const float off = -ref - (float)v_power;
-            const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
-            float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[c][2 * k]), __uint_as_float(x[c][2 * k + 1])), f2, off2);
-                    const float2 p = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                    sum = add2(sum, p);
-                    split_pair(p.x, p.y, hi[k], lo[k]);
-                }
-                // columns 8c.. of hi and of lo take the place of the scores just read
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    x[c][k] = hi[k];
-                    x[c][8 + k] = lo[k];
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    hi[k] = x[2 * c][k];
-                    hi[8 + k] = x[2 * c + 1][k];
-                    lo[k] = x[2 * c][8 + k];
-                    lo[8 + k] = x[2 * c + 1][8 + k];
-                }
-                tmem_st16u(col + 16 * c, hi);
-                tmem_st16u(col + 32 + 16 * c, lo);
-            }
-            l = fmaf(sum.x + sum.y, v_up, l * alpha);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(bar(sm.alpha_full[r4]));
-                mbar_arrive(bar(sm.p_full[st]));
-            }
-        }
-        sm.sum[row] = l;
-        sm.bad[row] = bad;
-        if (on && a.lse)
-            a.lse[(int64_t)(begin + tok) * a.n_head + head] = l == 0.f ? -INFINITY : 0.69314718055994530942f * (ref + log2f(l));
-        asm volatile("bar.sync 2, 256;" ::: "memory");
-    } else if (warp < 12) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        // ---- sums: thread = row
-        const int row = 32 * (warp - 8) + lane, j = row0 + row;
-        const uint32_t lanes = (uint32_t)(32 * (warp - 8)) << 16;
-        float2 acc[HD / 2];
-#pragma unroll
-        for (int i = 0; i < HD / 2; ++i) acc[i] = make_float2(0.f, 0.f);
-#pragma unroll 1
-        for (int i = 0; i < tiles; ++i) {
-            const int st = i & 1, r4 = i & 3;
-            warp_wait(bar(sm.alpha_full[r4]), (uint32_t)(i >> 2) & 1u, abort);
-            const float alpha = sm.alpha[r4][row];
-            warp_wait(bar(sm.o_full[st]), (uint32_t)(i >> 1) & 1u, abort);
-            tc_fence_after();
-            const uint32_t col = tmem + lanes + kColO + 128 * st;
-            const float2 keep = make_float2(alpha, alpha);
-            uint32_t x[2][16];
-            tmem_ld16_issue(col, x[0]);
-#pragma unroll
-            for (int c = 0; c < HD / 16; ++c) {
-                tmem_ld_wait(x[c & 1]);
-                if (c + 1 < HD / 16) tmem_ld16_issue(col + 16 * (c + 1), x[(c + 1) & 1]);
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    acc[8 * c + k] = __ffma2_rn(acc[8 * c + k], keep,
-                                                make_float2(__uint_as_float(x[c & 1][2 * k]), __uint_as_float(x[c & 1][2 * k + 1])));
-            }
-            tc_fence_before();
-            warp_arrive(bar(sm.o_empty[st]));
-        }
-        asm volatile("bar.sync 2, 256;" ::: "memory");
-        if (j < n * a.rep) {
-            const float sum = sm.sum[row], inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-            const uint32_t bad = sm.bad[row];
-            float* out = a.out + ((int64_t)(begin + j / a.rep) * a.n_head + kvh * a.rep + j % a.rep) * HD;
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const float by = bad >> g & 1 ? NAN : inv;
-#pragma unroll
-                for (int i = 16 * g; i < 16 * g + 16; i += 2)
-                    *reinterpret_cast<float4*>(out + 2 * i) =
-                        sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                   : make_float4(acc[i].x * by, acc[i].y * by, acc[i + 1].x * by, acc[i + 1].y * by);
-            }
-        }
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-        // ---- numbers to operands: warp w has the 16 positions of raw tile w
-        const int w = warp - 12, tid = threadIdx.x - 384;
-#pragma unroll 1
-        for (int i = 0; i < tiles; ++i) {
-            const int rs = i % kRawStages, st = i & 1, r4 = i & 3;
-            warp_wait(bar(sm.raw_full[rs]), (uint32_t)(i / kRawStages) & 1u, abort);
-            const uint32_t raw = smem_addr(sm.raw[rs]);
-            // the largest exponents: a value is below 2^(e - 14) for e = max(exponent of m, exponent of d + 4)
-            {
-                const int p = tid >> 1, half = tid & 1;  // position, half of its groups
-                uint32_t ek = 0, ev = 0, nan = 0;
-                if (i * kPromptCols + p < len) {
-                    const uint32_t tile = raw + (p / kTile) * Tile<HD>::kBytes + (p % kTile) * (HD / 8) + half * (HD / 16);
-#pragma unroll
-                    for (int g = 0; g < G / 2; ++g) {
-                        const uint32_t k = lds32(tile + Tile<HD>::kScaleK + 4 * g), v = lds32(tile + Tile<HD>::kScaleV + 4 * g);
-                        const uint32_t kd = k >> 10 & 31, km = k >> 26 & 31, vd = v >> 10 & 31, vm = v >> 26 & 31;
-                        if (max(kd, km) < 31) ek = max(ek, max(km, kd + 4));
-                        if (max(vd, vm) < 31) ev = max(ev, max(vm, vd + 4));
-                        else nan |= 1u << (half * (G / 2) + g);
+                    for (int k = 0; k < 16; ++k) {
+                        const uint32_t* y = &x[2 * c + k / 8][2 * (k % 8)];
+                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), f2, off2);
+                        const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                        sum = add2(sum, w);
+                        split_pair(w.x, w.y, hi[k], lo[k]);
                     }
+                    tmem_st16u(col + 16 * c, hi);
+                    tmem_st16u(col + 32 + 16 * c, lo);
                 }
-                ek = __reduce_max_sync(0xFFFFFFFFu, ek);
-                ev = __reduce_max_sync(0xFFFFFFFFu, ev);
-                const bool any = __any_sync(0xFFFFFFFFu, nan != 0);
-                nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, 1);
-                if (half == 0) sm.nan[r4][p] = (uint8_t)nan;
+                l = fmaf(sum.x + sum.y, v_up, l * alpha);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
                 if (lane == 0) {
-                    sm.top[r4][w][0] = ek;
-                    sm.top[r4][w][1] = ev;
-                    sm.warp_bad[r4][w] = any;
+                    mbar_arrive(bar(sm.alpha_full[r4]));
+                    mbar_arrive(bar(sm.p_full[st]));
                 }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            const int ek = (int)max(max(sm.top[r4][0][0], sm.top[r4][1][0]), max(sm.top[r4][2][0], sm.top[r4][3][0]));
-            const int ev = (int)max(max(sm.top[r4][0][1], sm.top[r4][1][1]), max(sm.top[r4][2][1], sm.top[r4][3][1]));
-            const int kp = min(14, 25 - ek), vp = min(12, 25 - ev);  // powers of two: the largest value to [2^10, 2^11)
-            if (tid == 0) {
-                sm.stat[r4].k_down = __uint_as_float((uint32_t)(127 - kp) << 23);
-                sm.stat[r4].v_up = __uint_as_float((uint32_t)(127 + vp) << 23);
-                sm.stat[r4].v_power = vp;
-                sm.stat[r4].bad = sm.warp_bad[r4][0] | sm.warp_bad[r4][1] | sm.warp_bad[r4][2] | sm.warp_bad[r4][3];
-                mbar_arrive(bar(sm.stat_full[r4]));
-            }
-            const float k_up = __uint_as_float((uint32_t)(127 + kp) << 23), v_up = __uint_as_float((uint32_t)(127 + vp) << 23);
-            const uint32_t tile = raw + w * Tile<HD>::kBytes;
-            const int here = len - i * kPromptCols - w * kTile;  // positions of this tile that are stored
-            // keys: a word of eight numbers is a 16-byte chunk of the operand's row
-            if (i >= 2) warp_wait(bar(sm.k_empty[st]), (uint32_t)((i >> 1) - 1) & 1u, abort);
-            {
-                const int p = lane & 15, row = w * kTile + p;
-                uint32_t sc[G];
-                lds_words<G>(tile + Tile<HD>::kScaleK + p * (HD / 8), sc);
-                const bool live = p < here;
+            const int slot = items++ & 1;
+            sm.sum[slot][row] = l;
+            sm.ref[slot][row] = ref;
+            sm.bad[slot][row] = bad;
+            asm volatile("bar.sync 2, 256;" ::: "memory");
+        }
+    } else if (warp < 12) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        // ---- sums: thread = row
+        const int row = 32 * (warp - 8) + lane;
+        const uint32_t lanes = (uint32_t)(32 * (warp - 8)) << 16;
+        for (int items = 0; cur.left > 0; cur.next(p)) {
+            cur.range(&from, &to);
+            if (!cur.here(from, to)) continue;
+            float2 acc[HD / 2];
 #pragma unroll
-                for (int t2 = 0; t2 < 2; ++t2) {
-                    const int t = 2 * (lane >> 4) + t2;
-                    uint32_t kw[G];
-                    lds_words<G>(tile + p * (HD / 2) + t * (HD / 8), kw);
+            for (int i = 0; i < HD / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+#pragma unroll 1
+            for (int i = from; i < to; ++i, ++it) {
+                const int st = it & 1, r4 = it & 3;
+                warp_wait(bar(sm.alpha_full[r4]), (uint32_t)(it >> 2) & 1u, abort);
+                const float alpha = sm.alpha[r4][row];
+                warp_wait(bar(sm.o_full[st]), (uint32_t)(it >> 1) & 1u, abort);
+                tc_fence_after();
+                const uint32_t col = tmem + lanes + kColO + 128 * st;
+                const float2 keep = make_float2(alpha, alpha);
+                uint32_t x[2][16];
+                tmem_ld16_issue(col, x[0]);
+#pragma unroll
+                for (int c = 0; c < HD / 16; ++c) {
+                    tmem_ld_wait(x[c & 1]);
+                    if (c + 1 < HD / 16) tmem_ld16_issue(col + 16 * (c + 1), x[(c + 1) & 1]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        acc[8 * c + k] = __ffma2_rn(acc[8 * c + k], keep,
+                                                    make_float2(__uint_as_float(x[c & 1][2 * k]), __uint_as_float(x[c & 1][2 * k + 1])));
+                }
+                tc_fence_before();
+                warp_arrive(bar(sm.o_empty[st]));
+            }
+            asm volatile("bar.sync 2, 256;" ::: "memory");
+            const PromptItem item = p.items[cur.item];
+            int begin, n;
+            seq_rows(a, item.seq, &begin, &n);
+            const int j = item.block * kPromptRows + row;
+            const float sum = sm.sum[items & 1][row], ref = sm.ref[items & 1][row];
+            const uint32_t bad = sm.bad[items & 1][row];
+            if (to - from == item.tiles) {
+                if (j < n * a.rep) {
+                    const int64_t at = (int64_t)(begin + j / a.rep) * a.n_head + cur.kvh * a.rep + j % a.rep;
+                    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+                    float* out = a.out + at * HD;
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
-                        const float d = live ? h2f(sc[g]) * k_up : 0.f, m = live ? h2f(sc[g] >> 16) * k_up : 0.f;
-                        const uint32_t word = kw[g], word8 = word >> 8;
-                        const float2 n04 = __half22float2(bits_h2(numbers<false>(word, 0.f))), n15 = __half22float2(bits_h2(numbers<true>(word, 0.f)));
-                        const float2 n26 = __half22float2(bits_h2(numbers<false>(word8, 0.f))), n37 = __half22float2(bits_h2(numbers<true>(word8, 0.f)));
+                        const float by = bad >> g & 1 ? NAN : inv;
+#pragma unroll
+                        for (int i = 16 * g; i < 16 * g + 16; i += 2)
+                            *reinterpret_cast<float4*>(out + 2 * i) =
+                                sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                           : make_float4(acc[i].x * by, acc[i].y * by, acc[i + 1].x * by, acc[i + 1].y * by);
+                    }
+                    if (a.lse) a.lse[at] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (ref + log2f(sum));
+                }
+            } else {
+                const int slot = 2 * blockIdx.x + (items ? 1 : 0);
+                float* out = p.part_o + ((int64_t)slot * kPromptRows + row) * HD;
+#pragma unroll
+                for (int i = 0; i < HD / 2; i += 2)
+                    *reinterpret_cast<float4*>(out + 2 * i) = make_float4(acc[i].x, acc[i].y, acc[i + 1].x, acc[i + 1].y);
+                *reinterpret_cast<float2*>(p.part_ml + 2 * (slot * kPromptRows + row)) = make_float2(ref, sum);
+                p.part_bad[slot * kPromptRows + row] = bad;
+                if (from == 0 && row == 0) {  // it begins here and ends in another CTA
+                    const int64_t end = item.unit + (int64_t)(cur.kvh + 1) * (item.tiles + kPromptUnits);
+                    p.last[blockIdx.x] = PromptPart{cur.item, cur.kvh, (int)((end * ctas - 1) / all) - (int)blockIdx.x + 1, slot};
+                }
+            }
+            ++items;
+        }
+    } else if (warp < 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // ---- keys to operands: warp w has the 16 positions of raw tile w
+        const int w = warp - 12, tid = threadIdx.x - 384;
+        for (; cur.left > 0; cur.next(p)) {
+            cur.range(&from, &to);
+            if (from >= to) continue;
+            const int len = a.c.length(p.items[cur.item].seq);
+#pragma unroll 1
+            for (int i = from; i < to; ++i, ++it) {
+                const int rs = it % kRawStages, st = it & 1, si = it % kStats;
+                warp_wait(bar(sm.raw_full[rs]), (uint32_t)(it / kRawStages) & 1u, abort);
+                const uint32_t raw = smem_addr(sm.raw[rs]), tile = raw + w * Tile<HD>::kBytes;
+                // the largest exponent: a value is below 2^(e - 14) for e = max(exponent of m, exponent of d + 4)
+                uint32_t sc[G], e = 0;
+                const int pos = lane & 15;
+                const bool live = i * kPromptCols + w * kTile + pos < len;
+                lds_words<G>(tile + Tile<HD>::kScaleK + pos * (HD / 8), sc);
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    if (!live) sc[g] = 0u;
+                    const uint32_t d = sc[g] >> 10 & 31, m = sc[g] >> 26 & 31;
+                    if (max(d, m) < 31) e = max(e, max(m, d + 4));
+                }
+                e = __reduce_max_sync(0xFFFFFFFFu, e);
+                if (lane == 0) sm.top[0][si][w] = e;
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                e = max(max(sm.top[0][si][0], sm.top[0][si][1]), max(sm.top[0][si][2], sm.top[0][si][3]));
+                const int power = min(14, 25 - (int)e);  // the largest value to [2^10, 2^11)
+                if (tid == 0) {
+                    sm.stat[si].k_down = __uint_as_float((uint32_t)(127 - power) << 23);
+                    mbar_arrive(bar(sm.stat_full[si]));
+                }
+                const __half2 up = __float2half2_rn(__uint_as_float((uint32_t)(127 + power) << 23));
+#pragma unroll
+                for (int g = 0; g < G; ++g) sc[g] = h2bits(__hmul2(bits_h2(sc[g]), up));
+                if (it >= 2) warp_wait(bar(sm.k_empty[st]), (uint32_t)((it >> 1) - 1) & 1u, abort);
+                const int row = w * kTile + pos;
+                const uint32_t hi_at = smem_addr(sm.k[st][0]) + row * 128, lo_at = smem_addr(sm.k[st][1]) + row * 128;
+#pragma unroll 1
+                for (int t2 = 0; t2 < 2; ++t2) {  // a word of eight numbers is a 16-byte chunk of the operand's row
+                    const int t = 2 * (lane >> 4) + t2;
+                    uint32_t kw[G];
+                    lds_words<G>(tile + pos * (HD / 2) + t * (HD / 8), kw);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const uint32_t m = __float_as_uint(h2f(sc[g] >> 16));
+                        const uint32_t x = kw[g], y = x >> 8;
+                        const uint32_t n04 = numbers<false>(x, 0.f), n15 = numbers<true>(x, 0.f), n26 = numbers<false>(y, 0.f),
+                                       n37 = numbers<true>(y, 0.f);
                         uint32_t hi[4], lo[4];
-                        split_pair(fmaf(n04.x, d, m), fmaf(n15.x, d, m), hi[0], lo[0]);
-                        split_pair(fmaf(n26.x, d, m), fmaf(n37.x, d, m), hi[1], lo[1]);
-                        split_pair(fmaf(n04.y, d, m), fmaf(n15.y, d, m), hi[2], lo[2]);
-                        split_pair(fmaf(n26.y, d, m), fmaf(n37.y, d, m), hi[3], lo[3]);
-                        const uint32_t at = (g >> 1) * (kPromptCols * 128) + row * 128 + ((((g & 1) * 4 + t) ^ (row & 7)) << 4);
-                        sts128u(smem_addr(sm.k[st][0]) + at, hi);
-                        sts128u(smem_addr(sm.k[st][1]) + at, lo);
+                        value_pair<0>(n04, n15, sc[g], sc[g], m, m, hi[0], lo[0]);
+                        value_pair<0>(n26, n37, sc[g], sc[g], m, m, hi[1], lo[1]);
+                        value_pair<1>(n04, n15, sc[g], sc[g], m, m, hi[2], lo[2]);
+                        value_pair<1>(n26, n37, sc[g], sc[g], m, m, hi[3], lo[3]);
+                        const uint32_t at = (g >> 1) * (kPromptCols * 128) + ((((g & 1) * 4 + t) ^ (row & 7)) << 4);
+                        sts128u(hi_at + at, hi);
+                        sts128u(lo_at + at, lo);
                     }
                 }
                 fence_proxy_async_smem();
-                warp_arrive(bar(sm.k_full[st]));
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar(sm.k_full[st]));
+                    mbar_arrive(bar(sm.raw_empty[rs]));
+                }
             }
-            // values: eight positions of one value are a 16-byte chunk
-            if (i >= 2) warp_wait(bar(sm.v_empty[st]), (uint32_t)((i >> 1) - 1) & 1u, abort);
-            {
-                const int r = lane & 7, q = lane >> 3 & 1, h = lane >> 4;
-                constexpr int NG = G / 2;  // groups of a lane
-                float d[NG][8], m[NG][8];
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // ---- values to operands: a lane has a column r of 8 positions and half of the groups
+        constexpr int NG = G / 2;
+        const int w = warp - 16, tid = threadIdx.x - 512, r = lane & 7, q = lane >> 3 & 1, h = lane >> 4;
+        for (; cur.left > 0; cur.next(p)) {
+            cur.range(&from, &to);
+            if (from >= to) continue;
+            const int len = a.c.length(p.items[cur.item].seq);
+#pragma unroll 1
+            for (int i = from; i < to; ++i, ++it) {
+                const int rs = it % kRawStages, st = it & 1, si = it % kStats;
+                warp_wait(bar(sm.raw_full[rs]), (uint32_t)(it / kRawStages) & 1u, abort);
+                const uint32_t raw = smem_addr(sm.raw[rs]), tile = raw + w * Tile<HD>::kBytes;
+                const int here = len - i * kPromptCols - w * kTile;  // positions of this tile that are stored
+                {
+                    const int pos = lane & 15;
+                    uint32_t sc[G], e = 0, nan = 0;
+                    lds_words<G>(tile + Tile<HD>::kScaleV + pos * (HD / 8), sc);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        if (pos >= here) sc[g] = 0u;
+                        const uint32_t d = sc[g] >> 10 & 31, m = sc[g] >> 26 & 31;
+                        if (max(d, m) < 31) e = max(e, max(m, d + 4));
+                        else nan |= 1u << g;
+                    }
+                    e = __reduce_max_sync(0xFFFFFFFFu, e);
+                    const bool any = __any_sync(0xFFFFFFFFu, nan != 0);
+                    if (lane < 16) sm.nan[si][w * kTile + pos] = (uint8_t)nan;
+                    if (lane == 0) {
+                        sm.top[1][si][w] = e;
+                        sm.warp_bad[si][w] = any;
+                    }
+                }
+                asm volatile("bar.sync 3, 128;" ::: "memory");
+                const uint32_t e = max(max(sm.top[1][si][0], sm.top[1][si][1]), max(sm.top[1][si][2], sm.top[1][si][3]));
+                const int power = min(12, 25 - (int)e);
+                if (tid == 0) {
+                    sm.stat[si].v_up = __uint_as_float((uint32_t)(127 + power) << 23);
+                    sm.stat[si].v_power = power;
+                    sm.stat[si].bad = sm.warp_bad[si][0] | sm.warp_bad[si][1] | sm.warp_bad[si][2] | sm.warp_bad[si][3];
+                    mbar_arrive(bar(sm.stat_full[si]));
+                }
+                const __half2 up = __float2half2_rn(__uint_as_float((uint32_t)(127 + power) << 23));
+                if (it >= 2) warp_wait(bar(sm.v_empty[st]), (uint32_t)((it >> 1) - 1) & 1u, abort);
                 uint32_t num[8];
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
-                    const int t = 2 * q + x / 4;
-                    const uint32_t at = tile + Tile<HD>::kV + ((x % 4) / 2) * (4 * HD) + (r * 4 + t) * (HD / 8) + (x & 1) * (HD / 16) + h * (HD / 32);
+                    const uint32_t at = tile + Tile<HD>::kV + ((x % 4) / 2) * (4 * HD) + (r * 4 + 2 * q + x / 4) * (HD / 8) +
+                                        (x & 1) * (HD / 16) + h * (HD / 32);
                     num[x] = HD == 128 ? lds32(at) : lds16(at);
-                    const bool live = 8 * q + x < here;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const uint32_t sc = lds32(tile + Tile<HD>::kScaleV + (8 * q + x) * (HD / 8) + (h * NG + g) * 4);
-                        const bool fine = live && (sc >> 10 & 31) < 31 && (sc >> 26 & 31) < 31;
-                        d[g][x] = fine ? h2f(sc) * v_up : 0.f;
-                        m[g][x] = fine ? h2f(sc >> 16) * v_up : 0.f;
-                    }
                 }
-#pragma unroll
+#pragma unroll 1
                 for (int g = 0; g < NG; ++g) {
-                    uint32_t pair[4];
+                    uint32_t sc[8], m[8], pair[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) pair[x] = __byte_perm(num[2 * x], num[2 * x + 1], g ? 0x7632 : 0x5410);
+                    for (int x = 0; x < 8; ++x) {
+                        uint32_t y = lds32(tile + Tile<HD>::kScaleV + (8 * q + x) * (HD / 8) + (h * NG + g) * 4);
+                        if (8 * q + x >= here || (y >> 10 & 31) == 31 || (y >> 26 & 31) == 31) y = 0u;
+                        sc[x] = h2bits(__hmul2(bits_h2(y), up));
+                        m[x] = __float_as_uint(h2f(sc[x] >> 16));
+                    }
+                    const uint32_t sel = g ? 0x7632u : 0x5410u;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int x = 0; x < 4; ++x) pair[x] = __byte_perm(num[2 * x], num[2 * x + 1], sel);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {  // eight positions of one value are a 16-byte chunk
                         uint32_t hi[4], lo[4];
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
                             const uint32_t y = c < 2 ? pair[x] : pair[x] >> 8;
-                            const float2 f = __half22float2(bits_h2(c & 1 ? numbers<true>(y, 0.f) : numbers<false>(y, 0.f)));
-                            split_pair(fmaf(f.x, d[g][2 * x], m[g][2 * x]), fmaf(f.y, d[g][2 * x + 1], m[g][2 * x + 1]), hi[x], lo[x]);
+                            const uint32_t n = c & 1 ? numbers<true>(y, 0.f) : numbers<false>(y, 0.f);
+                            value_pair<2>(n, n, sc[2 * x], sc[2 * x + 1], m[2 * x], m[2 * x + 1], hi[x], lo[x]);
                         }
                         const uint32_t at = (32 * (h * NG + g) + 8 * c + r) * 128 + (((2 * w + q) ^ r) << 4);
                         sts128u(smem_addr(sm.v[st][0]) + at, hi);
@@ -567,6 +758,44 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Att
     __syncthreads();
     tc_fence_after();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// The parts of the item that begins in CTA blockIdx.x's run and ends in
+// another's, added in their order: a warp per row, 16 rows per CTA.
+template <int HD>
+__global__ void __launch_bounds__(512) prompt_join_kernel(const PromptArgs p) {
+    const AttnArgs& a = p.a;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const PromptPart part = p.last[blockIdx.x];
+    if (!part.parts) return;
+    const int row = blockIdx.y * 16 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const PromptItem item = p.items[part.item];
+    int begin, n;
+    seq_rows(a, item.seq, &begin, &n);
+    const int j = item.block * kPromptRows + row;
+    if (j >= n * a.rep) return;
+    auto at = [&](int i) -> int64_t { return (int64_t)(i ? 2 * ((int)blockIdx.x + i) : part.slot) * kPromptRows + row; };
+    float m = -3.0e38f;
+    for (int i = 0; i < part.parts; ++i) m = fmaxf(m, p.part_ml[2 * at(i)]);
+    float sum = 0.f;
+    uint32_t bad = 0;
+    constexpr int V = HD / 32;
+    float x[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[e] = 0.f;
+    for (int i = 0; i < part.parts; ++i) {
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at(i));
+        const float k = exp2_fast(ml.x - m);
+        sum = fmaf(k, ml.y, sum);
+        bad |= p.part_bad[at(i)];
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = fmaf(k, p.part_o[at(i) * HD + 32 * e + lane], x[e]);
+    }
+    const int64_t to = (int64_t)(begin + j / a.rep) * a.n_head + part.kvh * a.rep + j % a.rep;
+    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+#pragma unroll
+    for (int e = 0; e < V; ++e) a.out[to * HD + 32 * e + lane] = sum == 0.f ? 0.f : x[e] * (bad >> e & 1 ? NAN : inv);
+    if (a.lse && lane == 0) a.lse[to] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (m + log2f(sum));
 }
 
 }  // namespace serve

@@ -42,6 +42,22 @@ int check_geometry(const char* who, int n_pages, int page_len, int n_head_kv, in
 // Rows * heads of a KV head up to which a sequence is kv4_rows_kernel's.
 constexpr int kRowsMax = 64;
 
+// Launch `kern` so that its launch overlaps the kernel before it; it starts with griddepcontrol.wait.
+template <class Args>
+int launch_after(void (*kern)(Args), dim3 grid, int threads, cudaStream_t st, const Args& args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute pdl[1];
+    pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    pdl[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = pdl;
+    cfg.numAttrs = 1;
+    CLLM_HOST_TRY(cudaLaunchKernelEx(&cfg, kern, args));
+    return CLLM_OK;
+}
+
 template <int HD>
 int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
     static std::once_flag once[64];
@@ -53,33 +69,49 @@ int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
                                         sizeof(PromptSmem<HD>) + 1024);
     });
     CLLM_HOST_TRY(attr);
+    const bool prompts = a.q_begin && (int64_t)a.n_tok * a.rep > a.rows_max;
     const int ctas = std::min(kMaxRowCtas, kRowCtasPerSm * sms);
-    const size_t last = align256(sizeof(Part) * ctas), ml = align256((size_t)2 * ctas * kRowTile * 2 * 4);
+    // blocks of rows of sequences with more rows than rows_max: at most
+    const int64_t rows = (int64_t)a.n_tok * a.rep;
+    const int64_t most = prompts ? rows / kPromptRows + std::min<int64_t>(a.c.n_seqs, rows / (a.rows_max + 1)) : 0;
+    if (most > INT_MAX / 2) return host_fail(CLLM_ERR_TOO_LARGE, "kv4_attention: too many rows in one call");
+
+    size_t bytes = 0;
+    auto part = [&](size_t n) {
+        const size_t at = bytes;
+        bytes += align256(n);
+        return at;
+    };
+    const size_t r_last = part(sizeof(Part) * ctas), r_ml = part((size_t)2 * ctas * kRowTile * 2 * 4);
+    const size_t r_o = part((size_t)2 * ctas * kRowTile * HD * 4);
+    const size_t p_items = part(prompts ? sizeof(PromptItem) * (most + 1) : 0), p_seq = part(prompts ? 4 * (size_t)a.c.n_seqs : 0);
+    const size_t p_count = part(256), p_last = part(sizeof(PromptPart) * sms);
+    const size_t p_ml = part(prompts ? (size_t)2 * sms * kPromptRows * 2 * 4 : 0), p_bad = part(prompts ? (size_t)2 * sms * kPromptRows * 4 : 0);
+    const size_t p_o = part(prompts ? (size_t)2 * sms * kPromptRows * HD * 4 : 0);
     uint8_t* ws;
     std::unique_lock<std::mutex> lk;
-    if (int rc = host_workspace(dev, last + ml + (size_t)2 * ctas * kRowTile * HD * 4, &ws, lk)) return rc;
-    RowsArgs ra{a, reinterpret_cast<Part*>(ws), reinterpret_cast<float*>(ws + last), reinterpret_cast<float*>(ws + last + ml)};
+    if (int rc = host_workspace(dev, bytes, &ws, lk)) return rc;
+
+    RowsArgs ra{a, reinterpret_cast<Part*>(ws + r_last), reinterpret_cast<float*>(ws + r_ml), reinterpret_cast<float*>(ws + r_o)};
     kv4_rows_kernel<HD><<<ctas, kRowThreads, sizeof(RowsSmem<HD>), st>>>(ra);
     CLLM_HOST_TRY(cudaGetLastError());
-    if ((int64_t)a.c.max_pages * a.c.page_len > kStepLen) {  // an item can have more than one step
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(ctas);
-        cfg.blockDim = dim3(kJoinThreads);
-        cfg.stream = st;
-        cudaLaunchAttribute pdl[1];
-        pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        pdl[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = pdl;
-        cfg.numAttrs = 1;
-        CLLM_HOST_TRY(cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD>, ra));
-    }
-    if (a.q_begin && (int64_t)a.n_tok * a.rep > a.rows_max) {
-        // as many CTAs as there can be tiles of sequences with more rows than that
-        const int64_t rows = (int64_t)a.n_tok * a.rep, seqs = std::min<int64_t>(a.c.n_seqs, rows / (a.rows_max + 1));
-        const int64_t items = (rows / kPromptRows + seqs) * a.c.n_kv;
-        if (items > INT_MAX) return host_fail(CLLM_ERR_TOO_LARGE, "kv4_attention: too many rows in one call");
-        kv4_prompt_kernel<HD><<<(unsigned)items, kPromptThreads, sizeof(PromptSmem<HD>) + 1024, st>>>(a);
+    if ((int64_t)a.c.max_pages * a.c.page_len > kStepLen)  // an item can have more than one step
+        if (int rc = launch_after(kv4_join_kernel<HD>, dim3(ctas), kJoinThreads, st, ra)) return rc;
+    if (prompts) {
+        PromptArgs pa{};
+        pa.a = a;
+        pa.most = (int)most;
+        pa.items = reinterpret_cast<PromptItem*>(ws + p_items);
+        pa.seq_items = reinterpret_cast<int*>(ws + p_seq);
+        pa.count = reinterpret_cast<int*>(ws + p_count);
+        pa.last = reinterpret_cast<PromptPart*>(ws + p_last);
+        pa.part_ml = reinterpret_cast<float*>(ws + p_ml);
+        pa.part_bad = reinterpret_cast<uint32_t*>(ws + p_bad);
+        pa.part_o = reinterpret_cast<float*>(ws + p_o);
+        prompt_plan_kernel<<<1, kPromptPlanThreads, 0, st>>>(pa);
+        kv4_prompt_kernel<HD><<<sms, kPromptThreads, sizeof(PromptSmem<HD>) + 1024, st>>>(pa);
         CLLM_HOST_TRY(cudaGetLastError());
+        if (int rc = launch_after(prompt_join_kernel<HD>, dim3(sms, kPromptRows / 16), 512, st, pa)) return rc;
     }
     return CLLM_OK;
 }

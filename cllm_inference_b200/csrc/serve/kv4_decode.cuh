@@ -189,11 +189,12 @@ __device__ __forceinline__ __half2 bits_h2(uint32_t b) { return *reinterpret_cas
 // (x, y) = hi + lo, each an fp16 pair, to 22 bits
 __device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t* lo) {
     const uint32_t h = h2bits(__floats2half2_rn(x, y));
-    float ex, ey;  // hi - x, exact
-    asm("sub.rn.f32.f16 %0, %1, %2;" : "=f"(ex) : "h"((unsigned short)h), "f"(x));
-    asm("sub.rn.f32.f16 %0, %1, %2;" : "=f"(ey) : "h"((unsigned short)(h >> 16)), "f"(y));
+    const uint32_t minus = h ^ 0x80008000u;
+    float ex, ey;  // x - hi, exact
+    asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(ex) : "h"((unsigned short)minus), "f"(x));
+    asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(ey) : "h"((unsigned short)(minus >> 16)), "f"(y));
     *hi = h;
-    *lo = h2bits(__floats2half2_rn(-ex, -ey));
+    *lo = h2bits(__floats2half2_rn(ex, ey));
 }
 // The numbers in bits 0-3 (UP: 4-7) of both halves of w, plus `off`, as an fp16 pair.
 template <bool UP>
@@ -227,12 +228,23 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[W]) {
         w[0] = v.x; w[1] = v.y;
     }
 }
+// mbarrier.try_wait that suspends the thread for up to about 2 us: a warp that
+// polls takes issue slots and instruction fetches from the ones it waits for.
+__device__ __forceinline__ bool mbar_try_wait_long(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(2000u)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool wait_full(uint32_t bar, uint32_t parity) {
     if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = global_timer_ns();
     for (uint32_t it = 1;; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 255u) == 0 && global_timer_ns() - t0 > kWaitLimitNs) {
+        if (mbar_try_wait_long(bar, parity)) return true;
+        if ((it & 15u) == 0 && global_timer_ns() - t0 > kWaitLimitNs) {
             atomicOr(&g_serve_status, kServeTimeout);
             return false;
         }

@@ -31,6 +31,8 @@
 // All waits are bounded; one that expires sets the status, and the CTA runs to its
 // end without waiting.
 #pragma once
+#include <type_traits>
+
 #include "../tc_ptx.cuh"
 #include "kv4_decode.cuh"
 
@@ -68,11 +70,24 @@ struct PromptSmem {
     int abort;
 };
 
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// One lane of the warp.  The compiler knows that a branch on this has one thread
+// and passes the products' operands straight to uniform registers; behind a
+// comparison of the lane number it loops over lanes for each of them (170 cycles
+// a product instead of 40).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
+    return ok != 0;
+}
+// One product step, A in TMEM, B the shared-memory operand at byte `at` (128-byte
+// swizzle; the descriptor's upper half is a constant, its lower the address / 16).
+// Few instructions: one thread issues 36 of these per tile.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t at, uint32_t idesc, bool accumulate) {
+    constexpr uint32_t kHigh = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "r"((at >> 4) | (1u << 16)), "r"(idesc), "r"((uint32_t)accumulate), "r"(kHigh)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -92,8 +107,8 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, vol
     if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = global_timer_ns();
     for (uint32_t it = 1;; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 63u) == 0) {
+        if (mbar_try_wait_long(bar, parity)) return true;
+        if ((it & 15u) == 0) {
             if (*abort) return false;
             if (global_timer_ns() - t0 > kWaitLimitNs) {
                 atomicOr(&g_serve_status, kServeTimeout);
@@ -350,8 +365,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
             }
             if (*abort)  // let the copies in flight land
                 for (int i = max(0, it - kRawStages); i < it; ++i) wait_full(bar(sm.raw_full[i % kRawStages]), (uint32_t)(i / kRawStages) & 1u);
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1 && elect_one()) {
             // ---- products: S of a tile, then O of the one before it
+            using Smem = PromptSmem<HD>;
+            const uint32_t k0 = smem_addr(sm.k), v0 = smem_addr(sm.v);
             auto values = [&](int j) {
                 const int st = j & 1;
                 wait_or_abort(bar(sm.p_full[st]), (uint32_t)(j >> 1) & 1u, abort);
@@ -359,10 +376,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 if (j >= 2) wait_or_abort(bar(sm.o_empty[st]), (uint32_t)((j >> 1) - 1) & 1u, abort);
                 tc_fence_after();
                 const uint32_t d = tmem + kColO + 128 * st;
-                for (int term = 0; term < 3; ++term) {  // lo hi, hi lo, hi hi
-                    const uint32_t w = tmem + kColS + 64 * st + (term == 0 ? 32 : 0), v = smem_addr(sm.v[st][term == 1]);
-                    for (int s = 0; s < kPromptCols / 16; ++s) tc_mma_ts(d, w + 8 * s, umma_desc_sw128(v + s * 32), kIdescO, term | s);
-                }
+                const uint32_t w = tmem + kColS + 64 * st, v = v0 + st * (2 * Smem::kOperand);
+#pragma unroll
+                for (int term = 0; term < 3; ++term)  // lo hi, hi lo, hi hi
+#pragma unroll
+                    for (int s = 0; s < kPromptCols / 16; ++s)
+                        tc_mma_ts(d, w + (term == 0 ? 32 : 0) + 8 * s, v + (term == 1 ? Smem::kOperand : 0) + s * 32, kIdescO, term | s);
                 tc_commit(bar(sm.o_full[st]));
                 tc_commit(bar(sm.v_empty[st]));
             };
@@ -377,11 +396,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     wait_or_abort(bar(sm.k_full[st]), (uint32_t)(it >> 1) & 1u, abort);
                     tc_fence_after();
                     const uint32_t d = tmem + kColS + 64 * st;
-                    for (int term = 0; term < 3; ++term) {
-                        const uint32_t q = tmem + kColQ + (term == 0 ? HD / 2 : 0), k = smem_addr(sm.k[st][term == 1]);
+                    const uint32_t q = tmem + kColQ, k = k0 + st * (2 * Smem::kOperand);
+#pragma unroll
+                    for (int term = 0; term < 3; ++term)
+#pragma unroll
                         for (int s = 0; s < HD / 16; ++s)
-                            tc_mma_ts(d, q + 8 * s, umma_desc_sw128(k + (s / 4) * (kPromptCols * 128) + (s % 4) * 32), kIdescS, term | s);
-                    }
+                            tc_mma_ts(d, q + (term == 0 ? HD / 2 : 0) + 8 * s,
+                                      k + (term == 1 ? Smem::kOperand : 0) + (s / 4) * (kPromptCols * 128) + (s % 4) * 32, kIdescS,
+                                      term | s);
                     tc_commit(bar(sm.s_full[st]));
                     tc_commit(bar(sm.k_empty[st]));
                     if (i > from) values(it - 1);
@@ -444,8 +466,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
             }
             float ref = -3.0e38f, l = 0.f;
             uint32_t bad = 0;
-#pragma unroll 1
-            for (int i = from; i < to; ++i, ++it) {
+            // EDGE: some row of the warp does not see all of the tile (a copy of its own, or every tile pays the selects)
+            auto tile = [&](auto edge, int i) {
+                constexpr bool EDGE = decltype(edge)::value;
                 const int st = it & 1, r4 = it & 3, rs = it % kStats;
                 warp_wait(bar(sm.stat_full[rs]), (uint32_t)(it / kStats) & 1u, abort);
                 warp_wait(bar(sm.s_full[st]), (uint32_t)(it >> 1) & 1u, abort);
@@ -459,8 +482,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld_wait(x[c]);
                 const int limit = sees - i * kPromptCols;  // columns that the row sees
-                if (__any_sync(0xFFFFFFFFu, limit < kPromptCols)) {
-                    __syncwarp();
+                if constexpr (EDGE) {
                     const uint32_t none = __float_as_uint(f < 0.f ? INFINITY : -INFINITY);
 #pragma unroll
                     for (int c = 0; c < kPromptCols; ++c)
@@ -519,7 +541,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     mbar_arrive(bar(sm.alpha_full[r4]));
                     mbar_arrive(bar(sm.p_full[st]));
                 }
-            }
+            };
+            const int plain = min(to, __reduce_min_sync(0xFFFFFFFFu, sees) / kPromptCols);
+#pragma unroll 1
+            for (int i = from; i < plain; ++i, ++it) tile(std::false_type{}, i);
+#pragma unroll 1
+            for (int i = max(from, plain); i < to; ++i, ++it) tile(std::true_type{}, i);
             const int slot = items++ & 1;
             sm.sum[slot][row] = l;
             sm.ref[slot][row] = ref;

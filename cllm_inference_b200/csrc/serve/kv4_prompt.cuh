@@ -127,24 +127,13 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// Two values as an fp16 pair and what is left of them as another.
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) { split2(x, y, &hi, &lo); }
-// n * d + m in fp32 of the halves NI of n and DI of d.
-template <int NI, int DI>
-__device__ __forceinline__ float number_value(uint32_t n, uint32_t d, uint32_t m) {
-    const unsigned short nh = NI ? (unsigned short)(n >> 16) : (unsigned short)n;
-    const unsigned short dh = DI ? (unsigned short)(d >> 16) : (unsigned short)d;
-    float v;
-    asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(v) : "h"(nh), "h"(dh), "f"(__uint_as_float(m)));
-    return v;
-}
-// The values of two numbers, split: SEL 0 and 1, the low and the high halves of
-// nx and ny; 2, both halves of nx.  d in the low halves of dx and dy.
-template <int SEL>
-__device__ __forceinline__ void value_pair(uint32_t nx, uint32_t ny, uint32_t dx, uint32_t dy, uint32_t mx, uint32_t my,
-                                           uint32_t& hi, uint32_t& lo) {
-    const float x = number_value<SEL == 1, 0>(nx, dx, mx), y = number_value<SEL != 0, 0>(ny, dy, my);
-    split_pair(x, y, hi, lo);
+// Two values as an fp16 pair and what is left of them as another: hi is the value
+// cut to fp16's 11 bits (the conversion is exact), so lo holds the next 11.
+__device__ __forceinline__ void split_pair(float2 x, uint32_t& hi, uint32_t& lo) {
+    const float2 h = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xFFFFE000u), __uint_as_float(__float_as_uint(x.y) & 0xFFFFE000u));
+    const float2 l = add2(x, make_float2(-h.x, -h.y));
+    hi = h2bits(__floats2half2_rn(h.x, h.y));
+    lo = h2bits(__floats2half2_rn(l.x, l.y));
 }
 
 // 128 rows of a sequence, for every KV head: its tiles per head, and where its units begin.
@@ -271,10 +260,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
     constexpr int G = Tile<HD>::G;
     constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kPromptCols >> 3) << 17) | ((uint32_t)(kPromptRows >> 4) << 24);
     constexpr uint32_t kIdescO = (1u << 4) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPromptRows >> 4) << 24);
-    constexpr uint32_t kColQ = 0, kColS = 128, kColO = 256;  // TMEM: q hi | lo; two S, each overwritten by p hi | lo; two O
+    constexpr uint32_t kColQ = 0, kColS = 128, kColO = 256;  // TMEM: q hi | lo; two S, 16 scores overwritten by p hi | lo; two O
     extern __shared__ uint8_t smem_raw[];
-    PromptSmem<HD>& sm =
-        *reinterpret_cast<PromptSmem<HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    PromptSmem<HD>& sm = *reinterpret_cast<PromptSmem<HD>*>(smem_raw + (-smem_addr(smem_raw) & 1023u));
     const AttnArgs& a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int* abort = &sm.abort;
@@ -377,11 +365,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 tc_fence_after();
                 const uint32_t d = tmem + kColO + 128 * st;
                 const uint32_t w = tmem + kColS + 64 * st, v = v0 + st * (2 * Smem::kOperand);
-#pragma unroll
+#pragma unroll 1
                 for (int term = 0; term < 3; ++term)  // lo hi, hi lo, hi hi
 #pragma unroll
                     for (int s = 0; s < kPromptCols / 16; ++s)
-                        tc_mma_ts(d, w + (term == 0 ? 32 : 0) + 8 * s, v + (term == 1 ? Smem::kOperand : 0) + s * 32, kIdescO, term | s);
+                        tc_mma_ts(d, w + (term == 0 ? 8 : 0) + 16 * s, v + (term == 1 ? Smem::kOperand : 0) + s * 32, kIdescO, term | s);
                 tc_commit(bar(sm.o_full[st]));
                 tc_commit(bar(sm.v_empty[st]));
             };
@@ -397,7 +385,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     tc_fence_after();
                     const uint32_t d = tmem + kColS + 64 * st;
                     const uint32_t q = tmem + kColQ, k = k0 + st * (2 * Smem::kOperand);
-#pragma unroll
+#pragma unroll 1
                     for (int term = 0; term < 3; ++term)
 #pragma unroll
                         for (int s = 0; s < HD / 16; ++s)
@@ -454,8 +442,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                             if (vec) x = *reinterpret_cast<const float4*>(src + i + k);
                             else x = make_float4(src[i + k], src[i + k + 1], src[i + k + 2], src[i + k + 3]);
                         }
-                        split_pair(x.x * up, x.y * up, hi[k / 2], lo[k / 2]);
-                        split_pair(x.z * up, x.w * up, hi[k / 2 + 1], lo[k / 2 + 1]);
+                        split_pair(make_float2(x.x * up, x.y * up), hi[k / 2], lo[k / 2]);
+                        split_pair(make_float2(x.z * up, x.w * up), hi[k / 2 + 1], lo[k / 2 + 1]);
                     }
                     tmem_st16u(tmem + lanes + kColQ + i / 2, hi);
                     tmem_st16u(tmem + lanes + kColQ + HD / 2 + i / 2, lo);
@@ -476,39 +464,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 const float f = f_log2 * sm.stat[rs].k_down, v_up = sm.stat[rs].v_up;
                 const int v_power = sm.stat[rs].v_power;
                 const uint32_t col = tmem + lanes + kColS + 64 * st;
-                uint32_t x[4][16];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld16_issue(col + 16 * c, x[c]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_wait(x[c]);
                 const int limit = sees - i * kPromptCols;  // columns that the row sees
-                if constexpr (EDGE) {
-                    const uint32_t none = __float_as_uint(f < 0.f ? INFINITY : -INFINITY);
-#pragma unroll
-                    for (int c = 0; c < kPromptCols; ++c)
-                        if (c >= limit) x[c / 16][c % 16] = none;
-                }
                 if (sm.stat[rs].bad)
                     for (int c = 0; c < min(limit, kPromptCols); ++c) bad |= sm.nan[rs][c];
-                float m[4];
-                if (f >= 0.f) {
+                // the largest score (f < 0: the smallest product)
+                const float sign = f < 0.f ? -1.f : 1.f;
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < kPromptCols; c += 16) {
+                    uint32_t x[16];
+                    tmem_ld16_issue(col + c, x);
+                    tmem_ld_wait(x);
+                    float m = -INFINITY;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        m[c] = __uint_as_float(x[c][0]);
-#pragma unroll
-                        for (int k = 1; k < 16; ++k) m[c] = fmaxf(m[c], __uint_as_float(x[c][k]));
+                    for (int k = 0; k < 16; ++k) {
+                        const float y = __uint_as_float(x[k]) * sign;
+                        if (!EDGE || c + k < limit) m = fmaxf(m, y);
                     }
-                    m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        m[c] = __uint_as_float(x[c][0]);
-#pragma unroll
-                        for (int k = 1; k < 16; ++k) m[c] = fminf(m[c], __uint_as_float(x[c][k]));
-                    }
-                    m[0] = fminf(fminf(m[0], m[1]), fminf(m[2], m[3]));
+                    top = fmaxf(top, m);
                 }
-                const float top = m[0] * f, room = 14.f + (float)min(0, v_power);
+                top *= f * sign;
+                const float room = 14.f + (float)min(0, v_power);
                 float alpha = 1.f;
                 if (top > ref + room) {
                     const float now = top - (room - 4.f);
@@ -519,19 +495,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 const float off = -ref - (float)v_power;
                 const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
                 float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 1
+                for (int c = 0; c < kPromptCols; c += 16) {  // 16 weights, hi in 8 columns and lo in 8, in place of their scores
+                    uint32_t x[16], w[16];
+                    tmem_ld16_issue(col + c, x);
+                    tmem_ld_wait(x);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {  // 32 columns at a time: p hi and lo take the place of the scores
-                    uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const uint32_t* y = &x[2 * c + k / 8][2 * (k % 8)];
-                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), f2, off2);
-                        const float2 w = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                        sum = add2(sum, w);
-                        split_pair(w.x, w.y, hi[k], lo[k]);
+                    for (int k = 0; k < 8; ++k) {
+                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), f2, off2);
+                        float2 y = make_float2(exp2_fast(e.x), exp2_fast(e.y));
+                        if (EDGE && c + 2 * k >= limit) y.x = 0.f;
+                        if (EDGE && c + 2 * k + 1 >= limit) y.y = 0.f;
+                        sum = add2(sum, y);
+                        split_pair(y, w[k], w[8 + k]);
                     }
-                    tmem_st16u(col + 16 * c, hi);
-                    tmem_st16u(col + 32 + 16 * c, lo);
+                    tmem_st16u(col + c, w);
                 }
                 l = fmaf(sum.x + sum.y, v_up, l * alpha);
                 tmem_st_wait();
@@ -659,31 +637,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     mbar_arrive(bar(sm.stat_full[si]));
                 }
                 const __half2 up = __float2half2_rn(__uint_as_float((uint32_t)(127 + power) << 23));
-#pragma unroll
-                for (int g = 0; g < G; ++g) sc[g] = h2bits(__hmul2(bits_h2(sc[g]), up));
                 if (it >= 2) warp_wait(bar(sm.k_empty[st]), (uint32_t)((it >> 1) - 1) & 1u, abort);
                 const int row = w * kTile + pos;
                 const uint32_t hi_at = smem_addr(sm.k[st][0]) + row * 128, lo_at = smem_addr(sm.k[st][1]) + row * 128;
 #pragma unroll 1
-                for (int t2 = 0; t2 < 2; ++t2) {  // a word of eight numbers is a 16-byte chunk of the operand's row
-                    const int t = 2 * (lane >> 4) + t2;
-                    uint32_t kw[G];
-                    lds_words<G>(tile + pos * (HD / 2) + t * (HD / 8), kw);
+                for (int c = 0; c < 2 * G; ++c) {  // a word of eight numbers is a 16-byte chunk of the operand's row
+                    const int t = 2 * (lane >> 4) + c / G, g = c % G;
+                    uint32_t word = lds32(tile + pos * (HD / 2) + t * (HD / 8) + 4 * g);
+                    const uint32_t y = live ? lds32(tile + Tile<HD>::kScaleK + pos * (HD / 8) + 4 * g) : 0u;
+                    const float2 dm = __half22float2(__hmul2(bits_h2(y), up)), d = make_float2(dm.x, dm.x), m = make_float2(dm.y, dm.y);
+                    float2 n[4];  // numbers j and j + 4
 #pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const uint32_t m = __float_as_uint(h2f(sc[g] >> 16));
-                        const uint32_t x = kw[g], y = x >> 8;
-                        const uint32_t n04 = numbers<false>(x, 0.f), n15 = numbers<true>(x, 0.f), n26 = numbers<false>(y, 0.f),
-                                       n37 = numbers<true>(y, 0.f);
-                        uint32_t hi[4], lo[4];
-                        value_pair<0>(n04, n15, sc[g], sc[g], m, m, hi[0], lo[0]);
-                        value_pair<0>(n26, n37, sc[g], sc[g], m, m, hi[1], lo[1]);
-                        value_pair<1>(n04, n15, sc[g], sc[g], m, m, hi[2], lo[2]);
-                        value_pair<1>(n26, n37, sc[g], sc[g], m, m, hi[3], lo[3]);
-                        const uint32_t at = (g >> 1) * (kPromptCols * 128) + ((((g & 1) * 4 + t) ^ (row & 7)) << 4);
-                        sts128u(hi_at + at, hi);
-                        sts128u(lo_at + at, lo);
-                    }
+                    for (int j = 0; j < 4; ++j) n[j] = __half22float2(bits_h2(numbers<false>(word >> (4 * j), 0.f)));
+                    uint32_t hi[4], lo[4];
+                    split_pair(__ffma2_rn(make_float2(n[0].x, n[1].x), d, m), hi[0], lo[0]);
+                    split_pair(__ffma2_rn(make_float2(n[2].x, n[3].x), d, m), hi[1], lo[1]);
+                    split_pair(__ffma2_rn(make_float2(n[0].y, n[1].y), d, m), hi[2], lo[2]);
+                    split_pair(__ffma2_rn(make_float2(n[2].y, n[3].y), d, m), hi[3], lo[3]);
+                    const uint32_t at = (g >> 1) * (kPromptCols * 128) + ((((g & 1) * 4 + t) ^ (row & 7)) << 4);
+                    sts128u(hi_at + at, hi);
+                    sts128u(lo_at + at, lo);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -747,25 +720,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 }
 #pragma unroll 1
                 for (int g = 0; g < NG; ++g) {
-                    uint32_t sc[8], m[8], pair[4];
+                    float2 d[4], m[4];
+                    uint32_t pair[4];
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        uint32_t y = lds32(tile + Tile<HD>::kScaleV + (8 * q + x) * (HD / 8) + (h * NG + g) * 4);
-                        if (8 * q + x >= here || (y >> 10 & 31) == 31 || (y >> 26 & 31) == 31) y = 0u;
-                        sc[x] = h2bits(__hmul2(bits_h2(y), up));
-                        m[x] = __float_as_uint(h2f(sc[x] >> 16));
+                    for (int x = 0; x < 4; ++x) {
+                        float2 dm[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t y = lds32(tile + Tile<HD>::kScaleV + (8 * q + 2 * x + e) * (HD / 8) + (h * NG + g) * 4);
+                            if (8 * q + 2 * x + e >= here || (y >> 10 & 31) == 31 || (y >> 26 & 31) == 31) y = 0u;
+                            dm[e] = __half22float2(__hmul2(bits_h2(y), up));
+                        }
+                        d[x] = make_float2(dm[0].x, dm[1].x);
+                        m[x] = make_float2(dm[0].y, dm[1].y);
                     }
                     const uint32_t sel = g ? 0x7632u : 0x5410u;
 #pragma unroll
                     for (int x = 0; x < 4; ++x) pair[x] = __byte_perm(num[2 * x], num[2 * x + 1], sel);
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < 4; ++c) {  // eight positions of one value are a 16-byte chunk
                         uint32_t hi[4], lo[4];
 #pragma unroll
                         for (int x = 0; x < 4; ++x) {
-                            const uint32_t y = c < 2 ? pair[x] : pair[x] >> 8;
-                            const uint32_t n = c & 1 ? numbers<true>(y, 0.f) : numbers<false>(y, 0.f);
-                            value_pair<2>(n, n, sc[2 * x], sc[2 * x + 1], m[2 * x], m[2 * x + 1], hi[x], lo[x]);
+                            const float2 n = __half22float2(bits_h2(numbers<false>(pair[x] >> (4 * c), 0.f)));
+                            split_pair(__ffma2_rn(n, d[x], m[x]), hi[x], lo[x]);
                         }
                         const uint32_t at = (32 * (h * NG + g) + 8 * c + r) * 128 + (((2 * w + q) ^ r) << 4);
                         sts128u(smem_addr(sm.v[st][0]) + at, hi);

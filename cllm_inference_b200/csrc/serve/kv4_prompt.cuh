@@ -122,6 +122,13 @@ __device__ __forceinline__ void warp_wait(uint32_t bar, uint32_t parity, volatil
     if ((threadIdx.x & 31) == 0) wait_or_abort(bar, parity, abort);
     __syncwarp();
 }
+// Wait as a warpgroup: its first warp polls, the others sleep in hardware barrier
+// ID (four polling warps took a third of the SM's issue slots and fetches).
+template <int ID>
+__device__ __forceinline__ void group_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+    if (((threadIdx.x >> 5) & 3) == 0) warp_wait(bar, parity, abort);
+    asm volatile("bar.sync %0, 128;" ::"n"(ID) : "memory");
+}
 __device__ __forceinline__ void warp_arrive(uint32_t bar) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
@@ -402,7 +409,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
             wait_full(bar(sm.done), 0);
         }
     } else if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
         // ---- softmax: thread = row
         const int row = 32 * (warp - 4) + lane;
         const uint32_t lanes = (uint32_t)(32 * (warp - 4)) << 16;
@@ -458,8 +465,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
             auto tile = [&](auto edge, int i) {
                 constexpr bool EDGE = decltype(edge)::value;
                 const int st = it & 1, r4 = it & 3, rs = it % kStats;
-                warp_wait(bar(sm.stat_full[rs]), (uint32_t)(it / kStats) & 1u, abort);
-                warp_wait(bar(sm.s_full[st]), (uint32_t)(it >> 1) & 1u, abort);
+                if (warp == 4) warp_wait(bar(sm.stat_full[rs]), (uint32_t)(it / kStats) & 1u, abort);
+                group_wait<4>(bar(sm.s_full[st]), (uint32_t)(it >> 1) & 1u, abort);
                 tc_fence_after();
                 const float f = f_log2 * sm.stat[rs].k_down, v_up = sm.stat[rs].v_up;
                 const int v_power = sm.stat[rs].v_power;
@@ -545,10 +552,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
 #pragma unroll 1
             for (int i = from; i < to; ++i, ++it) {
                 const int st = it & 1, r4 = it & 3;
-                warp_wait(bar(sm.alpha_full[r4]), (uint32_t)(it >> 2) & 1u, abort);
-                const float alpha = sm.alpha[r4][row];
-                warp_wait(bar(sm.o_full[st]), (uint32_t)(it >> 1) & 1u, abort);
+                if (warp == 8) warp_wait(bar(sm.alpha_full[r4]), (uint32_t)(it >> 2) & 1u, abort);
+                group_wait<5>(bar(sm.o_full[st]), (uint32_t)(it >> 1) & 1u, abort);
                 tc_fence_after();
+                const float alpha = sm.alpha[r4][row];
                 const uint32_t col = tmem + lanes + kColO + 128 * st;
                 const float2 keep = make_float2(alpha, alpha);
                 uint32_t x[2][16];
@@ -604,7 +611,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
             ++items;
         }
     } else if (warp < 16) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // ---- keys to operands: warp w has the 16 positions of raw tile w
         const int w = warp - 12, tid = threadIdx.x - 384;
         for (; cur.left > 0; cur.next(p)) {
@@ -614,7 +621,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
 #pragma unroll 1
             for (int i = from; i < to; ++i, ++it) {
                 const int rs = it % kRawStages, st = it & 1, si = it % kStats;
-                warp_wait(bar(sm.raw_full[rs]), (uint32_t)(it / kRawStages) & 1u, abort);
+                group_wait<1>(bar(sm.raw_full[rs]), (uint32_t)(it / kRawStages) & 1u, abort);
                 const uint32_t raw = smem_addr(sm.raw[rs]), tile = raw + w * Tile<HD>::kBytes;
                 // the largest exponent: a value is below 2^(e - 14) for e = max(exponent of m, exponent of d + 4)
                 uint32_t sc[G], e = 0;
@@ -637,7 +644,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     mbar_arrive(bar(sm.stat_full[si]));
                 }
                 const __half2 up = __float2half2_rn(__uint_as_float((uint32_t)(127 + power) << 23));
-                if (it >= 2) warp_wait(bar(sm.k_empty[st]), (uint32_t)((it >> 1) - 1) & 1u, abort);
+                if (it >= 2) group_wait<1>(bar(sm.k_empty[st]), (uint32_t)((it >> 1) - 1) & 1u, abort);
                 const int row = w * kTile + pos;
                 const uint32_t hi_at = smem_addr(sm.k[st][0]) + row * 128, lo_at = smem_addr(sm.k[st][1]) + row * 128;
 #pragma unroll 1
@@ -667,7 +674,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // ---- values to operands: a lane has a column r of 8 positions and half of the groups
         constexpr int NG = G / 2;
         const int w = warp - 16, tid = threadIdx.x - 512, r = lane & 7, q = lane >> 3 & 1, h = lane >> 4;
@@ -678,7 +685,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
 #pragma unroll 1
             for (int i = from; i < to; ++i, ++it) {
                 const int rs = it % kRawStages, st = it & 1, si = it % kStats;
-                warp_wait(bar(sm.raw_full[rs]), (uint32_t)(it / kRawStages) & 1u, abort);
+                group_wait<3>(bar(sm.raw_full[rs]), (uint32_t)(it / kRawStages) & 1u, abort);
                 const uint32_t raw = smem_addr(sm.raw[rs]), tile = raw + w * Tile<HD>::kBytes;
                 const int here = len - i * kPromptCols - w * kTile;  // positions of this tile that are stored
                 {
@@ -710,7 +717,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     mbar_arrive(bar(sm.stat_full[si]));
                 }
                 const __half2 up = __float2half2_rn(__uint_as_float((uint32_t)(127 + power) << 23));
-                if (it >= 2) warp_wait(bar(sm.v_empty[st]), (uint32_t)((it >> 1) - 1) & 1u, abort);
+                if (it >= 2) group_wait<3>(bar(sm.v_empty[st]), (uint32_t)((it >> 1) - 1) & 1u, abort);
                 uint32_t num[8];
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {

@@ -52,6 +52,8 @@ struct PromptSmem {
     uint8_t k[2][2][kOperand];  // [stage][hi, lo]: [64 values][position][128 bytes]
     uint8_t v[2][2][kOperand];  // [stage][hi, lo]: [value][128 bytes of positions]
     uint8_t raw[kRawStages][4 * Tile<HD>::kBytes];
+    float2 k_scale[4][Tile<HD>::G][kTile];    // [raw tile][group][position] (d, m), scaled
+    float v_scale[4][Tile<HD>::G][2][kTile];  // [raw tile][group][d, m][position]
     float alpha[4][kPromptRows];  // what a tile's new reference leaves of the sums
     float sum[2][kPromptRows], ref[2][kPromptRows];  // of an item: its rows' sums of weights and references
     uint32_t bad[2][kPromptRows];                    // groups that a NaN of the values reaches
@@ -437,8 +439,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     }
                 }
                 const int e = min(max((int)(__float_as_uint(top) >> 23), 30), 230);
-                const float up = __uint_as_float((uint32_t)(263 - e) << 23);  // the row's largest value to [2^9, 2^10)
-                f_log2 = a.scale * 1.44269504088896340736f * __uint_as_float((uint32_t)(e - 9) << 23);
+                // the row's largest value to [2^9, 2^10), with the sign of the scale, so that f_log2 is not negative
+                const float up = copysignf(__uint_as_float((uint32_t)(263 - e) << 23), a.scale);
+                f_log2 = fabsf(a.scale) * 1.44269504088896340736f * __uint_as_float((uint32_t)(e - 9) << 23);
 #pragma unroll 1
                 for (int i = 0; i < HD; i += 32) {
                     uint32_t hi[16], lo[16];
@@ -474,8 +477,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 const int limit = sees - i * kPromptCols;  // columns that the row sees
                 if (sm.stat[rs].bad)
                     for (int c = 0; c < min(limit, kPromptCols); ++c) bad |= sm.nan[rs][c];
-                // the largest score (f < 0: the smallest product)
-                const float sign = f < 0.f ? -1.f : 1.f;
                 float top = -INFINITY;
 #pragma unroll 1
                 for (int c = 0; c < kPromptCols; c += 16) {
@@ -485,12 +486,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     float m = -INFINITY;
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const float y = __uint_as_float(x[k]) * sign;
-                        if (!EDGE || c + k < limit) m = fmaxf(m, y);
+                        if (!EDGE || c + k < limit) m = fmaxf(m, __uint_as_float(x[k]));
                     }
                     top = fmaxf(top, m);
                 }
-                top *= f * sign;
+                top *= f;
                 const float room = 14.f + (float)min(0, v_power);
                 float alpha = 1.f;
                 if (top > ref + room) {
@@ -643,16 +643,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     sm.stat[si].k_down = __uint_as_float((uint32_t)(127 - power) << 23);
                     mbar_arrive(bar(sm.stat_full[si]));
                 }
-                const __half2 up = __float2half2_rn(__uint_as_float((uint32_t)(127 + power) << 23));
+                // a NaN stays one (its scores are NaN)
+                if (lane < 16)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float up = __uint_as_float((uint32_t)(127 + power) << 23);
+                        const float2 dm = __half22float2(bits_h2(sc[g]));
+                        sm.k_scale[w][g][pos] = make_float2(dm.x * up, dm.y * up);
+                    }
+                __syncwarp();
                 if (it >= 2) group_wait<1>(bar(sm.k_empty[st]), (uint32_t)((it >> 1) - 1) & 1u, abort);
                 const int row = w * kTile + pos;
                 const uint32_t hi_at = smem_addr(sm.k[st][0]) + row * 128, lo_at = smem_addr(sm.k[st][1]) + row * 128;
 #pragma unroll 1
                 for (int c = 0; c < 2 * G; ++c) {  // a word of eight numbers is a 16-byte chunk of the operand's row
                     const int t = 2 * (lane >> 4) + c / G, g = c % G;
-                    uint32_t word = lds32(tile + pos * (HD / 2) + t * (HD / 8) + 4 * g);
-                    const uint32_t y = live ? lds32(tile + Tile<HD>::kScaleK + pos * (HD / 8) + 4 * g) : 0u;
-                    const float2 dm = __half22float2(__hmul2(bits_h2(y), up)), d = make_float2(dm.x, dm.x), m = make_float2(dm.y, dm.y);
+                    const uint32_t word = lds32(tile + pos * (HD / 2) + t * (HD / 8) + 4 * g);
+                    const float2 dm = sm.k_scale[w][g][pos], d = make_float2(dm.x, dm.x), m = make_float2(dm.y, dm.y);
                     float2 n[4];  // numbers j and j + 4
 #pragma unroll
                     for (int j = 0; j < 4; ++j) n[j] = __half22float2(bits_h2(numbers<false>(word >> (4 * j), 0.f)));
@@ -688,16 +695,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 group_wait<3>(bar(sm.raw_full[rs]), (uint32_t)(it / kRawStages) & 1u, abort);
                 const uint32_t raw = smem_addr(sm.raw[rs]), tile = raw + w * Tile<HD>::kBytes;
                 const int here = len - i * kPromptCols - w * kTile;  // positions of this tile that are stored
+                const int pos = lane & 15;
+                uint32_t sc[G];
                 {
-                    const int pos = lane & 15;
-                    uint32_t sc[G], e = 0, nan = 0;
+                    uint32_t e = 0, nan = 0;
                     lds_words<G>(tile + Tile<HD>::kScaleV + pos * (HD / 8), sc);
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
-                        if (pos >= here) sc[g] = 0u;
                         const uint32_t d = sc[g] >> 10 & 31, m = sc[g] >> 26 & 31;
-                        if (max(d, m) < 31) e = max(e, max(m, d + 4));
-                        else nan |= 1u << g;
+                        if (pos >= here) {
+                            sc[g] = 0u;
+                        } else if (max(d, m) < 31) {
+                            e = max(e, max(m, d + 4));
+                        } else {  // must not reach the sums of the rows that do not see it
+                            nan |= 1u << g;
+                            sc[g] = 0u;
+                        }
                     }
                     e = __reduce_max_sync(0xFFFFFFFFu, e);
                     const bool any = __any_sync(0xFFFFFFFFu, nan != 0);
@@ -716,7 +729,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     sm.stat[si].bad = sm.warp_bad[si][0] | sm.warp_bad[si][1] | sm.warp_bad[si][2] | sm.warp_bad[si][3];
                     mbar_arrive(bar(sm.stat_full[si]));
                 }
-                const __half2 up = __float2half2_rn(__uint_as_float((uint32_t)(127 + power) << 23));
+                if (lane < 16)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float up = __uint_as_float((uint32_t)(127 + power) << 23);
+                        const float2 dm = __half22float2(bits_h2(sc[g]));
+                        sm.v_scale[w][g][0][pos] = dm.x * up;
+                        sm.v_scale[w][g][1][pos] = dm.y * up;
+                    }
+                __syncwarp();
                 if (it >= 2) group_wait<3>(bar(sm.v_empty[st]), (uint32_t)((it >> 1) - 1) & 1u, abort);
                 uint32_t num[8];
 #pragma unroll
@@ -731,15 +752,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     uint32_t pair[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        float2 dm[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            uint32_t y = lds32(tile + Tile<HD>::kScaleV + (8 * q + 2 * x + e) * (HD / 8) + (h * NG + g) * 4);
-                            if (8 * q + 2 * x + e >= here || (y >> 10 & 31) == 31 || (y >> 26 & 31) == 31) y = 0u;
-                            dm[e] = __half22float2(__hmul2(bits_h2(y), up));
-                        }
-                        d[x] = make_float2(dm[0].x, dm[1].x);
-                        m[x] = make_float2(dm[0].y, dm[1].y);
+                        d[x] = *reinterpret_cast<const float2*>(&sm.v_scale[w][h * NG + g][0][8 * q + 2 * x]);
+                        m[x] = *reinterpret_cast<const float2*>(&sm.v_scale[w][h * NG + g][1][8 * q + 2 * x]);
                     }
                     const uint32_t sel = g ? 0x7632u : 0x5410u;
 #pragma unroll

@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 if (it >= 2) group_wait<1>(bar(sm.k_empty[st]), (uint32_t)((it >> 1) - 1) & 1u, abort);
                 const int row = w * kTile + pos;
                 const uint32_t hi_at = smem_addr(sm.k[st][0]) + row * 128, lo_at = smem_addr(sm.k[st][1]) + row * 128;
-#pragma unroll 1
+#pragma unroll 2
                 for (int c = 0; c < 2 * G; ++c) {  // a word of eight numbers is a 16-byte chunk of the operand's row
                     const int t = 2 * (lane >> 4) + c / G, g = c % G;
                     const uint32_t word = lds32(tile + pos * (HD / 2) + t * (HD / 8) + 4 * g);
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     const uint32_t sel = g ? 0x7632u : 0x5410u;
 #pragma unroll
                     for (int x = 0; x < 4; ++x) pair[x] = __byte_perm(num[2 * x], num[2 * x + 1], sel);
-#pragma unroll 1
+#pragma unroll 2
                     for (int c = 0; c < 4; ++c) {  // eight positions of one value are a 16-byte chunk
                         uint32_t hi[4], lo[4];
 #pragma unroll

@@ -1,13 +1,36 @@
-// What a sampler reports of a row of logits (cllm_cuda_token_scores): one CTA
-// per row, one pass for maximum, sum and rank, one for the entropy's sum, and
-// one search per entry of the top list.
+// What a sampler reports of a row of logits (cllm_cuda_token_scores): log
+// probability and rank of a token, entropy, the top_k entries.
+//
+// One pass over the row, which bounds it: 4 bytes a logit from HBM, so an SM has
+// about 21 issue slots per 32 logits; the common path takes 6.
+//   * softmax: each thread keeps a reference instead of the maximum; it moves only
+//     when a logit exceeds it by 14, so the sums are hardly ever rescaled.  With c
+//     = x - reference (exact or nearly so): l += exp(c), lc += exp(c) * c, fp32.
+//   * top_k: an entry can be among the first k only if it is not behind a bound
+//     that k entries are known to reach.  The bound: with j = ceil(k / warps), the
+//     lowest of the warps' j-th best lanes (a lane's best so far), renewed after
+//     every 16 logits of a thread.  What reaches it (about 300 of 128256) goes to
+//     a list; at the end the list is pruned once more and each entry counts the
+//     entries before it.  A list that overflows (logits in ascending order) is
+//     replaced by k searches of the row.
+//   * rank: counted where a group of four reaches the token's logit.
+// Order is a 64-bit key (value, then lower index), so no result depends on the
+// order in which threads append.  Few rows: a cluster of up to 8 CTAs shares a row
+// and rank 0 joins the parts through distributed shared memory.
 #pragma once
+#include <cooperative_groups.h>
+
+#include <cfloat>
+
 #include "kv4_format.cuh"
 
 namespace cllm {
 namespace serve {
 
-constexpr int kScoreThreads = 1024;
+constexpr int kScoreThreads = 512, kScoreWarps = kScoreThreads / 32;
+constexpr int kScoreList = 4096;   // entries of a CTA's list
+constexpr int kScoreGroups = 4;    // groups of four logits a thread has in flight
+constexpr int kMaxTop = 32;
 
 struct ScoreArgs {
     const float* x;
@@ -20,81 +43,302 @@ struct ScoreArgs {
 };
 
 // A logit and its index as one number: larger is earlier in the order (value
-// descending, index ascending); NaN counts as -inf.
+// descending, index ascending); NaN counts as -inf, -0 as 0.
 __device__ __forceinline__ uint64_t order_key(float v, int i) {
     if (v != v) v = -INFINITY;
-    const uint32_t b = __float_as_uint(v == 0.f ? 0.f : v);  // -0 and 0 are equal
+    const uint32_t b = __float_as_uint(v == 0.f ? 0.f : v);
     const uint32_t k = b & 0x80000000u ? ~b : b | 0x80000000u;
     return ((uint64_t)k << 32) | (uint32_t)~i;
 }
-
-__device__ __forceinline__ double block_add(double v, double* s) {
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    double t = 0;
-    for (int i = 0; i < kScoreThreads / 32; ++i) t += s[i];
-    return t;
+// The value of a key; -inf for 0, which every key reaches.
+__device__ __forceinline__ float key_value(uint64_t key) {
+    if (key == 0) return -INFINITY;
+    const uint32_t k = (uint32_t)(key >> 32);
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
-__device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* s) {
-    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    uint64_t t = 0;
-    for (int i = 0; i < kScoreThreads / 32; ++i) t = max(t, s[i]);
-    return t;
+__device__ __forceinline__ float exp2_score(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t warp_max(uint64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max(v, (uint64_t)__shfl_xor_sync(0xFFFFFFFFu, (unsigned long long)v, o));
+    return v;
 }
 
-__global__ void __launch_bounds__(kScoreThreads) token_scores_kernel(const ScoreArgs a) {
-    __shared__ double s_d[32];
-    __shared__ uint64_t s_k[32];
-    const float* x = a.x + (int64_t)blockIdx.x * a.ld;
-    const int token = a.tokens ? a.tokens[blockIdx.x] : -1;
+// Sums around `from` to sums around `to`; nothing is left where they are more than fp32 apart.
+__device__ __forceinline__ void moved(float from, float to, float* l, float* lc) {
+    const float by = fmaxf(from - to, -1e30f), k = exp2_score(by * 1.44269504088896340736f);
+    *lc = *l == 0.f ? 0.f : k * fmaf(*l, by, *lc);
+    *l *= k;
+}
+
+struct ScorePart {  // what a CTA knows of its part of the row
+    float ref, l, lc;
+    int before;
+    uint64_t top[kMaxTop];
+};
+struct ScoreSmem {
+    uint64_t list[kScoreList];
+    uint64_t warp_key[kScoreWarps];
+    float ref[kScoreWarps], l[kScoreWarps], lc[kScoreWarps];
+    int before[kScoreWarps];
+    int count;
+    uint64_t top[kMaxTop];  // of the list, of the joined lists
+    ScorePart part;
+};
+
+// The bound from each lane's best key: the lowest of the warps' j-th best lanes.
+// Whole CTA; 0 (everything reaches it) where a warp has fewer lanes with a key.
+__device__ __forceinline__ uint64_t reach_bound(uint64_t best, int j, ScoreSmem& sm) {
+    uint64_t mine = best, top = 0;
+    for (int i = 0; i < j; ++i) {
+        top = warp_max(mine);
+        if (mine == top) mine = 0;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sm.warp_key[threadIdx.x >> 5] = top;
+    __syncthreads();
+    uint64_t bound = ~0ull;
+#pragma unroll
+    for (int w = 0; w < kScoreWarps; ++w) bound = min(bound, sm.warp_key[w]);
+    return bound;
+}
+
+// The first k of n keys (all different) of `list` into out, in order; entries there are too few of stay 0.
+__device__ __forceinline__ void first_of(const uint64_t* list, int n, int k, uint64_t* out) {
+    if ((int)threadIdx.x < k) out[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kScoreThreads) {
+        const uint64_t key = list[i];
+        int before = 0;
+        for (int m = 0; m < n; ++m) before += list[m] > key;
+        if (before < k) out[before] = key;
+    }
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const ScoreArgs a) {
+    namespace cg = cooperative_groups;
+    __shared__ ScoreSmem sm;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int parts = cluster.num_blocks(), part = cluster.block_rank(), row = blockIdx.x / parts;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float* x = a.x + (int64_t)row * a.ld;
+    const int token = a.tokens ? a.tokens[row] : -1;
     const bool known = token >= 0 && token < a.vocab;
-    const uint64_t mine = known ? order_key(x[token], token) : ~0ull;
-    uint64_t best = 0;
-    double nan = 0, before = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += kScoreThreads) {
-        const uint64_t k = order_key(x[i], i);
-        best = max(best, k);
-        before += k > mine;
-        nan += x[i] != x[i];
-    }
-    best = block_max(best, s_k);
-    before = block_add(before, s_d);
-    nan = block_add(nan, s_d);
-    const float m = nan > 0 ? NAN : x[(uint32_t)~best];
-    double l = 0, lc = 0;
-    for (int i = threadIdx.x; i < a.vocab; i += kScoreThreads) {
-        const float c = x[i] - m, e = expf(c);
+    float xt = known ? x[token] : INFINITY;
+    if (xt != xt) xt = -INFINITY;
+    // groups of four at 16-byte boundaries; up to three logits before and after them
+    const int head = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 4);
+    const int groups = (a.vocab - head) / 4, tail = head + 4 * groups;
+    const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
+    const int j = (a.top_k + kScoreWarps - 1) / kScoreWarps;
+
+    float ref = -FLT_MAX, l = 0.f, lc = 0.f;
+    int before = 0;
+    uint64_t best = 0, bound = a.top_k ? 0 : ~0ull;
+    float reach = a.top_k ? -INFINITY : INFINITY;  // the bound's value
+    if (tid == 0) sm.count = 0;
+    __syncthreads();
+
+    auto consider = [&](float v, int i) {  // for the list
+        const uint64_t key = order_key(v, i);
+        if (key < bound) return;
+        best = max(best, key);
+        const int at = atomicAdd(&sm.count, 1);
+        if (at < kScoreList) sm.list[at] = key;
+    };
+    auto count = [&](float v, int i) {  // for the rank
+        if (v != v) v = -INFINITY;
+        before += v > xt || (v == xt && i < token);
+    };
+    auto weigh = [&](float v) {
+        const float c = v - ref, e = exp2_score(c * 1.44269504088896340736f);
         l += e;
-        if (e > 0) lc += (double)e * c;
-    }
-    l = block_add(l, s_d);
-    lc = block_add(lc, s_d);
-    const bool none = !(m > -INFINITY && m < INFINITY);  // no distribution
-    const float log_l = none ? NAN : (float)log(l);
-    if (threadIdx.x == 0) {
-        if (a.logprob) a.logprob[blockIdx.x] = known ? (x[token] - m) - log_l : NAN;
-        if (a.rank) a.rank[blockIdx.x] = known ? (int)before : -1;
-        if (a.entropy) a.entropy[blockIdx.x] = none ? NAN : (float)(log(l) - lc / l);
-    }
-    uint64_t last = ~0ull;
-    for (int j = 0; j < a.top_k; ++j) {
-        uint64_t k = 0;
-        for (int i = threadIdx.x; i < a.vocab; i += kScoreThreads) {
-            const uint64_t c = order_key(x[i], i);
-            if (c < last) k = max(k, c);
+        lc = fmaf(e, fmaxf(c, -1e30f), lc);  // -inf: 0 * a number
+    };
+    auto raise = [&](float top) {
+        if (top > ref + 14.f) {
+            moved(ref, top, &l, &lc);
+            ref = top;
         }
-        last = block_max(k, s_k);
-        if (threadIdx.x == 0) {
-            const int i = (int)(uint32_t)~last;
-            a.top_ids[(int64_t)blockIdx.x * a.top_k + j] = i;
-            a.top_logprobs[(int64_t)blockIdx.x * a.top_k + j] = (x[i] - m) - log_l;
+    };
+    auto one = [&](int i) {  // a logit outside the groups
+        const float v = x[i];
+        raise(v);
+        weigh(v);
+        if (known) count(v, i);
+        if (a.top_k) consider(v, i);
+    };
+    if (part == 0 && tid < head) one(tid);
+    if (part == parts - 1 && tid < a.vocab - tail) one(tail + tid);
+
+    // two periods in registers: one on its way, one worked on
+    float4 next[kScoreGroups];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < kScoreGroups; ++u) {
+            const int g = base + u * kScoreThreads + tid;
+            if (g < g1) next[u] = __ldcs(reinterpret_cast<const float4*>(x + head) + g);
+        }
+    };
+    load(g0);
+    for (int base = g0; base < g1; base += kScoreGroups * kScoreThreads) {
+        float4 v[kScoreGroups];
+#pragma unroll
+        for (int u = 0; u < kScoreGroups; ++u) v[u] = next[u];
+        load(base + kScoreGroups * kScoreThreads);
+        if (base == g0 && a.top_k) {  // a first bound, from the first period
+            uint64_t first = best;
+#pragma unroll
+            for (int u = 0; u < kScoreGroups; ++u) {
+                const int g = base + u * kScoreThreads + tid, i = head + 4 * g;
+                if (g < g1)
+                    first = max(first, max(max(order_key(v[u].x, i), order_key(v[u].y, i + 1)),
+                                           max(order_key(v[u].z, i + 2), order_key(v[u].w, i + 3))));
+            }
+            bound = reach_bound(first, j, sm);
+            reach = key_value(bound);
+        }
+#pragma unroll
+        for (int u = 0; u < kScoreGroups; ++u) {
+            const int g = base + u * kScoreThreads + tid, i = head + 4 * g;
+            if (g >= g1) continue;
+            const float top = fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w));
+            if (!(top < fminf(fminf(reach, xt), ref + 14.f))) {
+                raise(top);
+                if (!(top < xt)) {
+                    count(v[u].x, i); count(v[u].y, i + 1); count(v[u].z, i + 2); count(v[u].w, i + 3);
+                }
+                if (!(top < reach)) {
+                    consider(v[u].x, i); consider(v[u].y, i + 1); consider(v[u].z, i + 2); consider(v[u].w, i + 3);
+                }
+            }
+            weigh(v[u].x); weigh(v[u].y); weigh(v[u].z); weigh(v[u].w);
+        }
+        if (a.top_k) {
+            bound = max(bound, reach_bound(best, j, sm));
+            reach = key_value(bound);
         }
     }
+
+    // the CTA's sums
+    float m = ref;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    if (lane == 0) sm.ref[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kScoreWarps; ++w) m = fmaxf(m, sm.ref[w]);
+    moved(ref, m, &l, &lc);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+        lc += __shfl_xor_sync(0xFFFFFFFFu, lc, o);
+        before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+    }
+    if (lane == 0) {
+        sm.l[warp] = l;
+        sm.lc[warp] = lc;
+        sm.before[warp] = before;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        float sl = 0.f, slc = 0.f;
+        int sb = 0;
+        for (int w = 0; w < kScoreWarps; ++w) {
+            sl += sm.l[w];
+            slc += sm.lc[w];
+            sb += sm.before[w];
+        }
+        sm.part.ref = m;
+        sm.part.l = sl;
+        sm.part.lc = slc;
+        sm.part.before = sb;
+    }
+    // the CTA's first top_k
+    if (a.top_k) {
+        int n = sm.count;
+        if (n > kScoreList) {  // it overflowed: search the part once for each entry
+            uint64_t last = ~0ull;
+            for (int k = 0; k < a.top_k; ++k) {
+                uint64_t key = 0;
+                auto look = [&](int i) {
+                    const uint64_t c = order_key(x[i], i);
+                    if (c < last) key = max(key, c);
+                };
+                if (part == 0 && tid < head) look(tid);
+                if (part == parts - 1 && tid < a.vocab - tail) look(tail + tid);
+                for (int i = head + 4 * g0 + tid; i < head + 4 * g1; i += kScoreThreads) look(i);
+                key = warp_max(key);
+                __syncthreads();
+                if (lane == 0) sm.warp_key[warp] = key;
+                __syncthreads();
+                last = 0;
+                for (int w = 0; w < kScoreWarps; ++w) last = max(last, sm.warp_key[w]);
+                if (tid == 0) sm.part.top[k] = last;
+            }
+        } else {
+            if (n > kScoreThreads / 4) {  // keep what still reaches the bound
+                uint64_t mine[kScoreList / kScoreThreads], top = 0;
+#pragma unroll
+                for (int i = 0; i < kScoreList / kScoreThreads; ++i) {
+                    const int at = i * kScoreThreads + tid;
+                    mine[i] = at < n ? sm.list[at] : 0;
+                    top = max(top, mine[i]);
+                }
+                bound = max(bound, reach_bound(top, j, sm));
+                __syncthreads();
+                if (tid == 0) sm.count = 0;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < kScoreList / kScoreThreads; ++i)
+                    if (mine[i] && mine[i] >= bound) sm.list[atomicAdd(&sm.count, 1)] = mine[i];
+                __syncthreads();
+                n = sm.count;
+            }
+            first_of(sm.list, n, a.top_k, sm.part.top);
+        }
+    }
+    cluster.sync();
+    if (part == 0) {
+        m = sm.part.ref;
+        for (int p = 1; p < parts; ++p) m = fmaxf(m, cluster.map_shared_rank(&sm.part, p)->ref);
+        l = lc = 0.f;
+        before = 0;
+        for (int p = 0; p < parts; ++p) {
+            const ScorePart* q = cluster.map_shared_rank(&sm.part, p);
+            float pl = q->l, plc = q->lc;
+            moved(q->ref, m, &pl, &plc);
+            l += pl;
+            lc += plc;
+            before += q->before;
+        }
+        const float log_l = l == 0.f ? NAN : logf(l);  // nothing but -inf: no distribution
+        if (tid == 0) {
+            if (a.logprob) a.logprob[row] = known ? (x[token] - m) - log_l : NAN;
+            if (a.rank) a.rank[row] = known ? before : -1;
+            if (a.entropy) a.entropy[row] = log_l - lc / l;
+        }
+        if (a.top_k) {
+            const uint64_t* top = sm.part.top;
+            if (parts > 1) {
+                for (int i = tid; i < parts * a.top_k; i += kScoreThreads)
+                    sm.list[i] = cluster.map_shared_rank(&sm.part, i / a.top_k)->top[i % a.top_k];
+                __syncthreads();
+                first_of(sm.list, parts * a.top_k, a.top_k, sm.top);
+                top = sm.top;
+            }
+            if (tid < a.top_k) {
+                const int i = (int)(uint32_t)~top[tid];  // top_k <= vocab, so there is an entry
+                a.top_ids[(int64_t)row * a.top_k + tid] = i;
+                a.top_logprobs[(int64_t)row * a.top_k + tid] = (unsigned)i < (unsigned)a.vocab ? (x[i] - m) - log_l : NAN;
+            }
+        }
+    }
+    cluster.sync();  // the other parts' memory stays until it has been read
 }
 
 }  // namespace serve

@@ -290,8 +290,21 @@ int cllm_cuda_token_scores(const float* logits, int64_t ld, int rows, int vocab,
     int dev, sms;
     if (int rc = host_device(&dev, &sms)) return rc;
     ScoreArgs a{logits, ld, rows, vocab, top_k, tokens, logprob, entropy, rank, top_ids, top_logprobs};
-    token_scores_kernel<<<rows, kScoreThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-    CLLM_HOST_TRY(cudaGetLastError());
+    // A cluster of CTAs per row until there are some seven CTAs per SM, each with 4096 logits at least.
+    int parts = 1;
+    while (parts < 8 && (int64_t)rows * parts < 7 * (int64_t)sms && vocab / (2 * parts) >= 4096) parts *= 2;
+    if ((int64_t)rows * parts > INT_MAX) return host_fail(CLLM_ERR_TOO_LARGE, "token_scores: too many rows");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * parts));
+    cfg.blockDim = dim3(kScoreThreads);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CLLM_HOST_TRY(cudaLaunchKernelEx(&cfg, token_scores_kernel, a));
     return CLLM_OK;
 }
 

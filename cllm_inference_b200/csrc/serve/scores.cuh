@@ -8,12 +8,13 @@
 //     = x - reference (exact or nearly so): l += exp(c), lc += exp(c) * c, fp32.
 //   * top_k: an entry can be among the first k only if it is not behind a bound
 //     that k entries are known to reach.  The bound: with j = ceil(k / warps), the
-//     lowest of the warps' j-th best lanes (a lane's best so far), renewed after
-//     every 16 logits of a thread.  What reaches it (about 300 of 128256) goes to
+//     lowest of the warps' j-th best lanes (a lane's best so far), renewed whenever
+//     the part read has doubled.  What reaches it (some hundreds of 128256) goes to
 //     a list; at the end the list is pruned once more and each entry counts the
 //     entries before it.  A list that overflows (logits in ascending order) is
 //     replaced by k searches of the row.
-//   * rank: counted where a group of four reaches the token's logit.
+//   * rank: a compare and an add per logit; what equals the token's logit counts
+//     before the token only, i.e. the threshold behind it is the next number up.
 // Order is a 64-bit key (value, then lower index), so no result depends on the
 // order in which threads append.  Few rows: a cluster of up to 8 CTAs shares a row
 // and rank 0 joins the parts through distributed shared memory.
@@ -27,7 +28,7 @@
 namespace cllm {
 namespace serve {
 
-constexpr int kScoreThreads = 512, kScoreWarps = kScoreThreads / 32;
+constexpr int kScoreThreads = 256, kScoreWarps = kScoreThreads / 32;
 constexpr int kScoreList = 4096;   // entries of a CTA's list
 constexpr int kScoreGroups = 4;    // groups of four logits a thread has in flight
 constexpr int kMaxTop = 32;
@@ -119,7 +120,7 @@ __device__ __forceinline__ void first_of(const uint64_t* list, int n, int k, uin
     __syncthreads();
 }
 
-__global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const ScoreArgs a) {
+__global__ void __launch_bounds__(kScoreThreads, 4) token_scores_kernel(const ScoreArgs a) {
     namespace cg = cooperative_groups;
     __shared__ ScoreSmem sm;
     cg::cluster_group cluster = cg::this_cluster();
@@ -136,7 +137,10 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const Sc
     const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
     const int j = (a.top_k + kScoreWarps - 1) / kScoreWarps;
 
+    const bool odd = known && !(fabsf(xt) < INFINITY);  // an infinite logit: count by the order itself
+    const float above = nextafterf(xt, INFINITY);
     float ref = -FLT_MAX, l = 0.f, lc = 0.f;
+    float2 l2 = make_float2(0.f, 0.f), lc2 = make_float2(0.f, 0.f);  // of the groups: even and odd logits
     int before = 0;
     uint64_t best = 0, bound = a.top_k ? 0 : ~0ull;
     float reach = a.top_k ? -INFINITY : INFINITY;  // the bound's value
@@ -159,9 +163,18 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const Sc
         l += e;
         lc = fmaf(e, fmaxf(c, -1e30f), lc);  // -inf: 0 * a number
     };
+    auto weigh2 = [&](float v, float w) {
+        const float2 c = __fadd2_rn(make_float2(v, w), make_float2(-ref, -ref));
+        const float2 t = __fmul2_rn(c, make_float2(1.44269504088896340736f, 1.44269504088896340736f));
+        const float2 e = make_float2(exp2_score(t.x), exp2_score(t.y));
+        l2 = __fadd2_rn(l2, e);
+        lc2 = __ffma2_rn(e, make_float2(fmaxf(c.x, -1e30f), fmaxf(c.y, -1e30f)), lc2);
+    };
     auto raise = [&](float top) {
         if (top > ref + 14.f) {
             moved(ref, top, &l, &lc);
+            moved(ref, top, &l2.x, &lc2.x);
+            moved(ref, top, &l2.y, &lc2.y);
             ref = top;
         }
     };
@@ -185,6 +198,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const Sc
         }
     };
     load(g0);
+    int period = 0;
     for (int base = g0; base < g1; base += kScoreGroups * kScoreThreads) {
         float4 v[kScoreGroups];
 #pragma unroll
@@ -207,24 +221,31 @@ __global__ void __launch_bounds__(kScoreThreads, 2) token_scores_kernel(const Sc
             const int g = base + u * kScoreThreads + tid, i = head + 4 * g;
             if (g >= g1) continue;
             const float top = fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w));
-            if (!(top < fminf(fminf(reach, xt), ref + 14.f))) {
+            if (!(top < fminf(reach, ref + 14.f))) {
                 raise(top);
-                if (!(top < xt)) {
-                    count(v[u].x, i); count(v[u].y, i + 1); count(v[u].z, i + 2); count(v[u].w, i + 3);
-                }
                 if (!(top < reach)) {
                     consider(v[u].x, i); consider(v[u].y, i + 1); consider(v[u].z, i + 2); consider(v[u].w, i + 3);
                 }
             }
-            weigh(v[u].x); weigh(v[u].y); weigh(v[u].z); weigh(v[u].w);
+            if (odd || (unsigned)(token - i) < 4u) {
+                count(v[u].x, i); count(v[u].y, i + 1); count(v[u].z, i + 2); count(v[u].w, i + 3);
+            } else {
+                const float at = i < token ? xt : above;
+                before += (v[u].x >= at) + (v[u].y >= at) + (v[u].z >= at) + (v[u].w >= at);
+            }
+            weigh2(v[u].x, v[u].y);
+            weigh2(v[u].z, v[u].w);
         }
-        if (a.top_k) {
+        ++period;
+        if (a.top_k && (period & (period - 1)) == 0 && base + kScoreGroups * kScoreThreads < g1) {
             bound = max(bound, reach_bound(best, j, sm));
             reach = key_value(bound);
         }
     }
 
     // the CTA's sums
+    l += l2.x + l2.y;
+    lc += lc2.x + lc2.y;
     float m = ref;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));

@@ -7,10 +7,9 @@
 //     when a logit exceeds it by 14, so the sums are hardly ever rescaled.  With c
 //     = x - reference (exact or nearly so): l += exp(c), lc += exp(c) * c, fp32.
 //   * top_k: an entry can be among the first k only if it is not behind a bound
-//     that k entries are known to reach.  The bound: with j = ceil(k / warps), the
-//     lowest of the warps' j-th best lanes (a lane's best so far), renewed whenever
-//     the part read has doubled.  What reaches it (some hundreds of 128256) goes to
-//     a list; at the end the list is pruned once more and each entry counts the
+//     that k entries are known to reach: the k-th of the best lanes (a lane's best
+//     so far) of each warp, renewed whenever the part read has doubled.  What
+//     reaches it (some hundreds of 128256) goes to a list; at the end the list is pruned once more and each entry counts the
 //     entries before it.  A list that overflows (logits in ascending order) is
 //     replaced by k searches of the row.
 //   * rank: a compare and an add per logit; what equals the token's logit counts
@@ -32,6 +31,7 @@ constexpr int kScoreThreads = 256, kScoreWarps = kScoreThreads / 32;
 constexpr int kScoreList = 4096;   // entries of a CTA's list
 constexpr int kScoreGroups = 4;    // groups of four logits a thread has in flight
 constexpr int kMaxTop = 32;
+constexpr int kBestLanes = 10;      // of a warp, at most, that a bound is taken from (80 >= 2 * 32)
 
 struct ScoreArgs {
     const float* x;
@@ -81,8 +81,10 @@ struct ScorePart {  // what a CTA knows of its part of the row
     uint64_t top[kMaxTop];
 };
 struct ScoreSmem {
-    uint64_t list[kScoreList];
+    uint64_t list[kScoreList];  // while reading: logit (low word) and index; then keys
     uint64_t warp_key[kScoreWarps];
+    uint64_t best[kScoreWarps * kBestLanes];
+    uint64_t bound;
     float ref[kScoreWarps], l[kScoreWarps], lc[kScoreWarps];
     int before[kScoreWarps];
     int count;
@@ -90,21 +92,33 @@ struct ScoreSmem {
     ScorePart part;
 };
 
-// The bound from each lane's best key: the lowest of the warps' j-th best lanes.
-// Whole CTA; 0 (everything reaches it) where a warp has fewer lanes with a key.
-__device__ __forceinline__ uint64_t reach_bound(uint64_t best, int j, ScoreSmem& sm) {
-    uint64_t mine = best, top = 0;
-    for (int i = 0; i < j; ++i) {
-        top = warp_max(mine);
-        if (mine == top) mine = 0;
+// A key that k keys reach: the k-th of the best lanes of each warp (`best`: a
+// lane's key, 0 for none).  0 where there are fewer than k.  Whole CTA.
+__device__ __forceinline__ uint64_t reach_bound(uint64_t best, int k, ScoreSmem& sm) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lanes = min(kBestLanes, 2 + 2 * ((k + kScoreWarps - 1) / kScoreWarps));
+    uint32_t value = (uint32_t)(best >> 32), index = (uint32_t)best;
+    __syncthreads();
+    for (int i = 0; i < lanes; ++i) {
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, value);
+        const int from = __ffs(__ballot_sync(0xFFFFFFFFu, value == top)) - 1;
+        const uint32_t at = __shfl_sync(0xFFFFFFFFu, index, from);
+        if (lane == from) {
+            sm.best[warp * lanes + i] = top ? ((uint64_t)top << 32) | at : 0;
+            value = 0;
+        }
+    }
+    if (threadIdx.x == 0) sm.bound = 0;
+    __syncthreads();
+    const int n = kScoreWarps * lanes;
+    if ((int)threadIdx.x < n) {
+        const uint64_t mine = sm.best[threadIdx.x];
+        int before = 0;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) before += sm.best[i] > mine;
+        if (mine && before == k - 1) sm.bound = mine;
     }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) sm.warp_key[threadIdx.x >> 5] = top;
-    __syncthreads();
-    uint64_t bound = ~0ull;
-#pragma unroll
-    for (int w = 0; w < kScoreWarps; ++w) bound = min(bound, sm.warp_key[w]);
-    return bound;
+    return sm.bound;
 }
 
 // The first k of n keys (all different) of `list` into out, in order; entries there are too few of stay 0.
@@ -114,6 +128,7 @@ __device__ __forceinline__ void first_of(const uint64_t* list, int n, int k, uin
     for (int i = threadIdx.x; i < n; i += kScoreThreads) {
         const uint64_t key = list[i];
         int before = 0;
+#pragma unroll 4
         for (int m = 0; m < n; ++m) before += list[m] > key;
         if (before < k) out[before] = key;
     }
@@ -135,25 +150,36 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_scores_kernel(const Sc
     const int head = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 4);
     const int groups = (a.vocab - head) / 4, tail = head + 4 * groups;
     const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
-    const int j = (a.top_k + kScoreWarps - 1) / kScoreWarps;
 
     const bool odd = known && !(fabsf(xt) < INFINITY);  // an infinite logit: count by the order itself
     const float above = nextafterf(xt, INFINITY);
     float ref = -FLT_MAX, l = 0.f, lc = 0.f;
     float2 l2 = make_float2(0.f, 0.f), lc2 = make_float2(0.f, 0.f);  // of the groups: even and odd logits
     int before = 0;
-    uint64_t best = 0, bound = a.top_k ? 0 : ~0ull;
-    float reach = a.top_k ? -INFINITY : INFINITY;  // the bound's value
+    uint64_t bound = 0;
+    float best_value = -INFINITY;  // of the logits considered
+    int best_index = -1;
+    // the bound's value, the next number up for logits behind the bound's index, and that index
+    float reach = a.top_k ? -INFINITY : INFINITY, reach_up = reach;
+    int reach_to = INT_MAX;
+    auto set_bound = [&](uint64_t to) {
+        bound = to;
+        reach = key_value(to);
+        reach_up = to ? nextafterf(reach, INFINITY) : reach;
+        reach_to = to ? (int)(uint32_t)~to : INT_MAX;
+    };
     if (tid == 0) sm.count = 0;
     __syncthreads();
 
     auto consider = [&](float v, int i) {  // for the list
-        const uint64_t key = order_key(v, i);
-        if (key < bound) return;
-        best = max(best, key);
+        if (v > best_value || best_index < 0) {
+            best_value = v;
+            best_index = i;
+        }
         const int at = atomicAdd(&sm.count, 1);
-        if (at < kScoreList) sm.list[at] = key;
+        if (at < kScoreList) sm.list[at] = ((uint64_t)i << 32) | __float_as_uint(v);
     };
+    auto best = [&]() -> uint64_t { return best_index < 0 ? 0 : order_key(best_value, best_index); };  // this lane's
     auto count = [&](float v, int i) {  // for the rank
         if (v != v) v = -INFINITY;
         before += v > xt || (v == xt && i < token);
@@ -198,48 +224,65 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_scores_kernel(const Sc
         }
     };
     load(g0);
+    constexpr int kPeriod = kScoreGroups * kScoreThreads;
     int period = 0;
-    for (int base = g0; base < g1; base += kScoreGroups * kScoreThreads) {
+    auto four = [&](const float4& v, int i) {
+        const float top = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), least = i > reach_to ? reach_up : reach;
+        if (!(top < fminf(least, ref + 14.f))) {
+            raise(top);
+            if (!(v.x < least)) consider(v.x, i);
+            if (!(v.y < least)) consider(v.y, i + 1);
+            if (!(v.z < least)) consider(v.z, i + 2);
+            if (!(v.w < least)) consider(v.w, i + 3);
+        }
+        if (odd || (unsigned)(token - i) < 4u) {
+            count(v.x, i); count(v.y, i + 1); count(v.z, i + 2); count(v.w, i + 3);
+        } else {
+            const float at = i < token ? xt : above;
+            before += (v.x >= at) + (v.y >= at) + (v.z >= at) + (v.w >= at);
+        }
+        weigh2(v.x, v.y);
+        weigh2(v.z, v.w);
+    };
+    for (int base = g0; base < g1; base += kPeriod) {
         float4 v[kScoreGroups];
 #pragma unroll
         for (int u = 0; u < kScoreGroups; ++u) v[u] = next[u];
-        load(base + kScoreGroups * kScoreThreads);
+        load(base + kPeriod);
+        const int g = base + tid;
         if (base == g0 && a.top_k) {  // a first bound, from the first period
-            uint64_t first = best;
+            float most = -INFINITY;
+            int at = g < g1 ? head + 4 * g : -1;
+            auto look = [&](float y, int i) {
+                if (y > most) {
+                    most = y;
+                    at = i;
+                }
+            };
 #pragma unroll
             for (int u = 0; u < kScoreGroups; ++u) {
-                const int g = base + u * kScoreThreads + tid, i = head + 4 * g;
-                if (g < g1)
-                    first = max(first, max(max(order_key(v[u].x, i), order_key(v[u].y, i + 1)),
-                                           max(order_key(v[u].z, i + 2), order_key(v[u].w, i + 3))));
-            }
-            bound = reach_bound(first, j, sm);
-            reach = key_value(bound);
-        }
-#pragma unroll
-        for (int u = 0; u < kScoreGroups; ++u) {
-            const int g = base + u * kScoreThreads + tid, i = head + 4 * g;
-            if (g >= g1) continue;
-            const float top = fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w));
-            if (!(top < fminf(reach, ref + 14.f))) {
-                raise(top);
-                if (!(top < reach)) {
-                    consider(v[u].x, i); consider(v[u].y, i + 1); consider(v[u].z, i + 2); consider(v[u].w, i + 3);
+                const int i = head + 4 * (g + u * kScoreThreads);
+                if (g + u * kScoreThreads < g1) {
+                    look(v[u].x, i); look(v[u].y, i + 1); look(v[u].z, i + 2); look(v[u].w, i + 3);
                 }
             }
-            if (odd || (unsigned)(token - i) < 4u) {
-                count(v[u].x, i); count(v[u].y, i + 1); count(v[u].z, i + 2); count(v[u].w, i + 3);
-            } else {
-                const float at = i < token ? xt : above;
-                before += (v[u].x >= at) + (v[u].y >= at) + (v[u].z >= at) + (v[u].w >= at);
+            set_bound(reach_bound(max(best(), at < 0 ? 0 : order_key(most, at)), a.top_k, sm));
+        }
+        if (base + kPeriod <= g1) {
+#pragma unroll
+            for (int u = 0; u < kScoreGroups; ++u) four(v[u], head + 4 * (g + u * kScoreThreads));
+        } else {
+#pragma unroll 1
+            for (int u = 0; u < kScoreGroups; ++u) {
+                if (g + u * kScoreThreads < g1) four(v[0], head + 4 * (g + u * kScoreThreads));
+#pragma unroll
+                for (int w = 0; w + 1 < kScoreGroups; ++w) v[w] = v[w + 1];
             }
-            weigh2(v[u].x, v[u].y);
-            weigh2(v[u].z, v[u].w);
         }
         ++period;
-        if (a.top_k && (period & (period - 1)) == 0 && base + kScoreGroups * kScoreThreads < g1) {
-            bound = max(bound, reach_bound(best, j, sm));
-            reach = key_value(bound);
+        if (a.top_k && (period & (period - 1)) == 0 && base + kPeriod < g1) {
+            const uint64_t now = reach_bound(best(), a.top_k, sm);
+            if (now > bound) set_bound(now);
         }
     }
 
@@ -302,15 +345,19 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_scores_kernel(const Sc
                 if (tid == 0) sm.part.top[k] = last;
             }
         } else {
-            if (n > kScoreThreads / 4) {  // keep what still reaches the bound
-                uint64_t mine[kScoreList / kScoreThreads], top = 0;
+            uint64_t mine[kScoreList / kScoreThreads], top = 0;
+            for (int i = 0; i * kScoreThreads < n; ++i) {
+                const int at = i * kScoreThreads + tid;
+                if (at < n) top = max(top, sm.list[at] = order_key(__uint_as_float((uint32_t)sm.list[at]), (int)(sm.list[at] >> 32)));
+            }
+            if (n > kScoreThreads / 4) {  // keep what reaches the bound now
+                const uint64_t now = reach_bound(top, a.top_k, sm);
+                bound = max(bound, now);
 #pragma unroll
                 for (int i = 0; i < kScoreList / kScoreThreads; ++i) {
                     const int at = i * kScoreThreads + tid;
                     mine[i] = at < n ? sm.list[at] : 0;
-                    top = max(top, mine[i]);
                 }
-                bound = max(bound, reach_bound(top, j, sm));
                 __syncthreads();
                 if (tid == 0) sm.count = 0;
                 __syncthreads();

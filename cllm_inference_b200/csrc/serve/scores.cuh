@@ -8,7 +8,7 @@
 //     = x - reference (exact or nearly so): l += exp(c), lc += exp(c) * c, fp32.
 //   * top_k: an entry can be among the first k only if it is not behind a bound
 //     that k entries are known to reach: the k-th of the best lanes (a lane's best
-//     so far) of each warp, renewed whenever the part read has doubled.  What
+//     so far) of each warp, renewed after 2, 8 and 32 periods.  What
 //     reaches it (some hundreds of 128256) goes to a list; at the end the list is pruned once more and each entry counts the
 //     entries before it.  A list that overflows (logits in ascending order) is
 //     replaced by k searches of the row.
@@ -31,7 +31,7 @@ constexpr int kScoreThreads = 256, kScoreWarps = kScoreThreads / 32;
 constexpr int kScoreList = 4096;   // entries of a CTA's list
 constexpr int kScoreGroups = 4;    // groups of four logits a thread has in flight
 constexpr int kMaxTop = 32;
-constexpr int kBestLanes = 10;      // of a warp, at most, that a bound is taken from (80 >= 2 * 32)
+constexpr int kBestLanes = 1 + kMaxTop / kScoreWarps;  // of a warp, at most, that a bound is taken from
 
 struct ScoreArgs {
     const float* x;
@@ -81,7 +81,7 @@ struct ScorePart {  // what a CTA knows of its part of the row
     uint64_t top[kMaxTop];
 };
 struct ScoreSmem {
-    uint64_t list[kScoreList];  // while reading: logit (low word) and index; then keys
+    alignas(16) uint64_t list[kScoreList];  // while reading: logit (low word) and index; then keys
     uint64_t warp_key[kScoreWarps];
     uint64_t best[kScoreWarps * kBestLanes];
     uint64_t bound;
@@ -94,8 +94,8 @@ struct ScoreSmem {
 
 // A key that k keys reach: the k-th of the best lanes of each warp (`best`: a
 // lane's key, 0 for none).  0 where there are fewer than k.  Whole CTA.
-__device__ __forceinline__ uint64_t reach_bound(uint64_t best, int k, ScoreSmem& sm) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lanes = min(kBestLanes, 2 + 2 * ((k + kScoreWarps - 1) / kScoreWarps));
+__device__ __noinline__ uint64_t reach_bound(uint64_t best, int k, ScoreSmem& sm) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lanes = 1 + (k + kScoreWarps - 1) / kScoreWarps;
     uint32_t value = (uint32_t)(best >> 32), index = (uint32_t)best;
     __syncthreads();
     for (int i = 0; i < lanes; ++i) {
@@ -122,14 +122,19 @@ __device__ __forceinline__ uint64_t reach_bound(uint64_t best, int k, ScoreSmem&
 }
 
 // The first k of n keys (all different) of `list` into out, in order; entries there are too few of stay 0.
-__device__ __forceinline__ void first_of(const uint64_t* list, int n, int k, uint64_t* out) {
+__device__ __noinline__ void first_of(const uint64_t* list, int n, int k, uint64_t* out) {
     if ((int)threadIdx.x < k) out[threadIdx.x] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kScoreThreads) {
         const uint64_t key = list[i];
         int before = 0;
-#pragma unroll 4
-        for (int m = 0; m < n; ++m) before += list[m] > key;
+        const ulonglong2* two = reinterpret_cast<const ulonglong2*>(list);
+#pragma unroll 8
+        for (int m = 0; m < n / 2; ++m) {
+            const ulonglong2 y = two[m];
+            before += (y.x > key) + (y.y > key);
+        }
+        if (n & 1) before += list[n - 1] > key;
         if (before < k) out[before] = key;
     }
     __syncthreads();
@@ -280,7 +285,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_scores_kernel(const Sc
             }
         }
         ++period;
-        if (a.top_k && (period & (period - 1)) == 0 && base + kPeriod < g1) {
+        if (a.top_k && (period == 2 || period == 8 || period == 32) && base + kPeriod < g1) {
             const uint64_t now = reach_bound(best(), a.top_k, sm);
             if (now > bound) set_bound(now);
         }
@@ -350,7 +355,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_scores_kernel(const Sc
                 const int at = i * kScoreThreads + tid;
                 if (at < n) top = max(top, sm.list[at] = order_key(__uint_as_float((uint32_t)sm.list[at]), (int)(sm.list[at] >> 32)));
             }
-            if (n > kScoreThreads / 4) {  // keep what reaches the bound now
+            if (n > 2 * a.top_k + 16) {  // keep what reaches the bound now
                 const uint64_t now = reach_bound(top, a.top_k, sm);
                 bound = max(bound, now);
 #pragma unroll

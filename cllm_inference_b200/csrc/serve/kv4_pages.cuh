@@ -1,20 +1,23 @@
 // Sequences over shared pages (cllm_cuda_kv4_fork, cllm_cuda_kv4_compact).
 //
 // A page is in use when a sequence names it, so there is no reference count
-// that could drift: each call derives what it needs from the tables.  Fork, in
-// four launches:
-//   memset   all pages free, none whole, no owner
+// that could drift: each call derives what it needs from the tables.
 //   mark     every page the new sequences continue: whole (shared), or the last,
 //            unfinished one of a sequence, whose owner is the lowest sequence
 //            that ends in it
-//   plan     one CTA: which sequences keep their last page, the pages each one
-//            needs, their prefix sum, the free pages in order (prefix sum over
-//            the bitmap), the list of copies
+//   plan     which sequences keep their last page, the pages each one needs,
+//            their prefix sum, the free pages in order (prefix sum over the
+//            bitmap), the list of copies
 //   apply    the table rows, and the copies in every layer, 16 bytes a load
 // The results depend on no order of execution: marks are bits and minima, and
-// pages are handed out by prefix sums.  What bounds the calls: the copies'
-// bytes (read and written once) for large pools, the chain of four launches
-// for small ones.
+// pages are handed out by prefix sums.
+//
+// What bounds the calls: the copies' bytes (read and written once) for large
+// pools, launches and latency for small ones.  So where the tables fit, one
+// launch does it all: every CTA derives the whole plan in shared memory (some
+// thousand table entries, 4 us), writes its share of the rows and copies its
+// share of the pages, and no CTA waits for another.  Larger tables, and compact
+// in place, take four launches through the workspace.
 #pragma once
 #include "kv4_format.cuh"
 
@@ -78,6 +81,21 @@ __device__ __forceinline__ int page_at(const PagesArgs& a, int s, int i) {
     atomicOr(&g_serve_status, kServeBadPage);
     return -1;
 }
+
+// One launch: limits, and what a CTA holds.
+constexpr int kSmallThreads = 1024, kSmallPages = 16384, kSmallSeqs = 1024, kSmallEntries = 65536, kSmallUnroll = 4;
+struct SmallPlan {
+    uint32_t free_bits[kSmallPages / 32], part_bits[kSmallPages / 32];
+    union {
+        uint32_t owner[kSmallPages];  // until the sequences know which last pages they keep
+        uint16_t to[kSmallPages];     // compact: where a page goes
+    };
+    uint16_t ids[kSmallPages];        // free pages / holes
+    int2 copies[kSmallSeqs];          // fork
+    int src[kSmallSeqs], held[kSmallSeqs], want[kSmallSeqs], first[kSmallSeqs];
+    int warp[32];
+    int count;
+};
 
 __device__ __forceinline__ void clear_bit(uint32_t* bits, int i) {
     const uint32_t b = 1u << (i & 31);
@@ -227,31 +245,32 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const PagesA
     }
 }
 
-// The copies of *a.count pages in every layer, spread over CTAs [first, first + ctas).
-__device__ __forceinline__ void copy_pages(const PagesArgs& a, int cta, int ctas) {
-    constexpr int kPiece = kCopyThreads * kCopyUnroll;  // 16-byte units of a piece
+// The copies of `count` pages in every layer, CTA `cta` of `ctas`' share.
+template <int THREADS, int UNROLL>
+__device__ __forceinline__ void copy_pages(const PagesArgs& a, const int2* copies, int count, int cta, int ctas) {
+    constexpr int kPiece = THREADS * UNROLL;  // 16-byte units of a piece
     const int64_t vecs = a.page_bytes / 16;
-    const int64_t pieces = (vecs + kPiece - 1) / kPiece, all = pieces * a.n_layers * (int64_t)*a.count;
+    const int64_t pieces = (vecs + kPiece - 1) / kPiece, all = pieces * a.n_layers * (int64_t)count;
     for (int64_t i = cta; i < all; i += ctas) {
         const int64_t page = i / pieces, at = (i - page * pieces) * kPiece + threadIdx.x;
         const int layer = (int)(page % a.n_layers);
-        const int2 c = a.copies[page / a.n_layers];
+        const int2 c = copies[page / a.n_layers];
         const uint4* from = reinterpret_cast<const uint4*>(a.pages + ((int64_t)layer * a.n_pages + c.x) * a.page_bytes);
         uint4* to = reinterpret_cast<uint4*>(a.pages + ((int64_t)layer * a.n_pages + c.y) * a.page_bytes);
-        uint4 v[kCopyUnroll];
+        uint4 v[UNROLL];
 #pragma unroll
-        for (int u = 0; u < kCopyUnroll; ++u)
-            if (at + u * kCopyThreads < vecs) v[u] = from[at + u * kCopyThreads];
+        for (int u = 0; u < UNROLL; ++u)
+            if (at + u * THREADS < vecs) v[u] = __ldcs(from + at + u * THREADS);
 #pragma unroll
-        for (int u = 0; u < kCopyUnroll; ++u)
-            if (at + u * kCopyThreads < vecs) to[at + u * kCopyThreads] = v[u];
+        for (int u = 0; u < UNROLL; ++u)
+            if (at + u * THREADS < vecs) __stcs(to + at + u * THREADS, v[u]);
     }
 }
 
 // CTAs below n_new write a table row each, the others copy.
 __global__ void __launch_bounds__(kCopyThreads) fork_apply_kernel(const PagesArgs a) {
     if ((int)blockIdx.x >= a.n_new) {
-        copy_pages(a, blockIdx.x - a.n_new, gridDim.x - a.n_new);
+        copy_pages<kCopyThreads, kCopyUnroll>(a, a.copies, *a.count, blockIdx.x - a.n_new, gridDim.x - a.n_new);
         return;
     }
     const int s = blockIdx.x;
@@ -269,7 +288,7 @@ __global__ void __launch_bounds__(kCopyThreads) fork_apply_kernel(const PagesArg
 
 __global__ void __launch_bounds__(kCopyThreads) compact_apply_kernel(const PagesArgs a) {
     if ((int)blockIdx.x >= a.n_new) {
-        copy_pages(a, blockIdx.x - a.n_new, gridDim.x - a.n_new);
+        copy_pages<kCopyThreads, kCopyUnroll>(a, a.copies, *a.count, blockIdx.x - a.n_new, gridDim.x - a.n_new);
         return;
     }
     const int s = blockIdx.x, n = min(a.max_pages, pages_of(a.seq_len[s], a.page_len)), live = *a.n_live;
@@ -281,6 +300,126 @@ __global__ void __launch_bounds__(kCopyThreads) compact_apply_kernel(const Pages
             if (id >= live && id < a.n_pages) id = a.moved[id];
         }
         a.table_out[at] = id;
+    }
+}
+
+// Exclusive prefix sum over the free (or, `used`, the used) pages of the bitmap
+// from page `from` on; each(id, rank) for every one.  Returns their number.
+template <class F>
+__device__ __forceinline__ int each_page(const uint32_t* bits, bool used, int from, int n_pages, int* s_warp, F each) {
+    int total;
+    const int w = threadIdx.x;  // at most kSmallPages / 32 words
+    uint32_t b = 0;
+    if (32 * w < n_pages) {
+        b = (used ? ~bits[w] : bits[w]) & word_mask(n_pages, w);
+        b &= ~word_mask(from, w);
+    }
+    int at = block_scan(__popc(b), s_warp, &total);
+    for (; b; b &= b - 1) each(32 * w + __ffs(b) - 1, at++);
+    return total;
+}
+
+__global__ void __launch_bounds__(kSmallThreads, 1) fork_small_kernel(const PagesArgs a) {
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    SmallPlan& sm = *reinterpret_cast<SmallPlan*>(smem_raw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < kSmallPages / 32; i += kSmallThreads) sm.free_bits[i] = sm.part_bits[i] = ~0u;
+    for (int i = tid; i < a.n_pages; i += kSmallThreads) sm.owner[i] = ~0u;
+    bool fine = false;
+    int src = 0, kept = 0, want = 0;
+    if (tid < a.n_new) {
+        fine = fork_request(a, tid, &src, &kept, &want);
+        sm.src[tid] = src;
+        sm.held[tid] = fine ? kept : 0;
+        sm.want[tid] = want;
+    }
+    if (tid == 0) sm.count = 0;
+    __syncthreads();
+    for (int s = warp; s < a.n_new; s += kSmallThreads / 32) {
+        const int k = sm.held[s], whole = k / a.page_len, n = whole + (k % a.page_len > 0);
+        for (int i = lane; i < n; i += 32) {
+            const int id = page_at(a, sm.src[s], i);
+            if (id < 0) continue;
+            clear_bit(sm.free_bits, id);
+            if (i < whole) clear_bit(sm.part_bits, id);
+            else atomicMin(sm.owner + id, (uint32_t)s);
+        }
+    }
+    __syncthreads();
+    const int room = each_page(sm.free_bits, false, 0, a.n_pages, sm.warp, [&](int id, int rank) { sm.ids[rank] = (uint16_t)id; });
+    int need = 0, held = 0, last = -1;
+    bool copy = false;
+    if (tid < a.n_new) {
+        held = kept / a.page_len;
+        if (kept % a.page_len) {
+            last = page_at(a, src, held);
+            const bool keeps = last >= 0 && (sm.part_bits[last >> 5] >> (last & 31) & 1u) && sm.owner[last] == (uint32_t)tid;
+            held += keeps;
+            copy = !keeps && last >= 0;
+        }
+        need = (fine ? pages_of(want, a.page_len) : 0) - held;
+        if (!fine) need = 0;
+    }
+    int total;
+    const int at = block_scan(need, sm.warp, &total);
+    fine = fine && (int64_t)at + need <= room;
+    const int c = block_scan(fine && copy, sm.warp, &total);
+    if (tid < a.n_new) {
+        if (fine && copy) sm.copies[c] = make_int2(last, sm.ids[at]);
+        sm.first[tid] = at;
+        sm.held[tid] = fine ? held : -1;
+    }
+    __syncthreads();
+    for (int s = blockIdx.x * (kSmallThreads / 32) + warp; s < a.n_new; s += gridDim.x * (kSmallThreads / 32)) {
+        const int h = sm.held[s], goal = h < 0 ? 0 : pages_of(sm.want[s], a.page_len);
+        if (lane == 0) a.len_out[s] = h < 0 ? -1 : sm.want[s];
+        for (int i = lane; i < a.max_pages; i += 32) {
+            int id = -1;
+            if (i < h) id = a.table[(int64_t)sm.src[s] * a.max_pages + i];
+            else if (i < goal) id = sm.ids[sm.first[s] + i - h];
+            a.table_out[(int64_t)s * a.max_pages + i] = id;
+        }
+    }
+    copy_pages<kSmallThreads, kSmallUnroll>(a, sm.copies, total, blockIdx.x, gridDim.x);
+}
+
+__global__ void __launch_bounds__(kSmallThreads, 1) compact_small_kernel(const PagesArgs a) {
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    SmallPlan& sm = *reinterpret_cast<SmallPlan*>(smem_raw);
+    int2* moves = reinterpret_cast<int2*>(sm.copies);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < kSmallPages / 32; i += kSmallThreads) sm.free_bits[i] = ~0u;
+    if (tid < a.n_new) sm.held[tid] = min(a.max_pages, pages_of(a.seq_len[tid], a.page_len));
+    __syncthreads();
+    for (int s = warp; s < a.n_new; s += kSmallThreads / 32)
+        for (int i = lane; i < sm.held[s]; i += 32) {
+            const int id = page_at(a, s, i);
+            if (id >= 0) clear_bit(sm.free_bits, id);
+        }
+    __syncthreads();
+    const int live = each_page(sm.free_bits, true, 0, a.n_pages, sm.warp, [](int, int) {});
+    each_page(sm.free_bits, false, 0, min(live, a.n_pages), sm.warp, [&](int id, int rank) { sm.ids[rank] = (uint16_t)id; });
+    __syncthreads();
+    const int count = each_page(sm.free_bits, true, live, a.n_pages, sm.warp, [&](int id, int rank) { sm.to[id] = sm.ids[rank]; });
+    __syncthreads();
+    if (tid == 0 && blockIdx.x == 0) *a.n_live = live;
+    for (int s = blockIdx.x * (kSmallThreads / 32) + warp; s < a.n_new; s += gridDim.x * (kSmallThreads / 32))
+        for (int i = lane; i < a.max_pages; i += 32) {
+            int id = -1;
+            if (i < sm.held[s]) {
+                id = a.table[(int64_t)s * a.max_pages + i];
+                if (id >= live && id < a.n_pages) id = sm.to[id];
+            }
+            a.table_out[(int64_t)s * a.max_pages + i] = id;
+        }
+    // the moves, as many at a time as the list holds
+    for (int base = 0; base < count; base += kSmallSeqs) {
+        __syncthreads();
+        each_page(sm.free_bits, true, live, a.n_pages, sm.warp, [&](int id, int rank) {
+            if (rank >= base && rank < base + kSmallSeqs) moves[rank - base] = make_int2(id, sm.ids[rank]);
+        });
+        __syncthreads();
+        copy_pages<kSmallThreads, kSmallUnroll>(a, moves, min(kSmallSeqs, count - base), blockIdx.x, gridDim.x);
     }
 }
 

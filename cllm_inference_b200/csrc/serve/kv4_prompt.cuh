@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
     constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kPromptCols >> 3) << 17) | ((uint32_t)(kPromptRows >> 4) << 24);
     constexpr uint32_t kIdescO = (1u << 4) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kPromptRows >> 4) << 24);
     constexpr uint32_t kColQ = 0, kColS = 128, kColO = 256;  // TMEM: q hi | lo; two S, 16 scores overwritten by p hi | lo; two O
-    extern __shared__ uint8_t smem_raw[];
+    extern __shared__ __align__(128) uint8_t smem_raw[];
     PromptSmem<HD>& sm = *reinterpret_cast<PromptSmem<HD>*>(smem_raw + (-smem_addr(smem_raw) & 1023u));
     const AttnArgs& a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

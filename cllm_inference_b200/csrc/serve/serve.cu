@@ -210,6 +210,23 @@ static int pages_call(const char* who, PagesArgs a, void* pages, int64_t page_by
     if (int rc = host_device(&dev, &sms)) return rc;
     a.pages = static_cast<uint8_t*>(pages);
     a.page_bytes = page_bytes;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Tables that a CTA can hold: one launch (192 sequences of 8 pages 12 us less than four launches).
+    if (a.n_pages <= kSmallPages && a.n_new <= kSmallSeqs && (int64_t)a.n_new * a.max_pages <= kSmallEntries &&
+        a.table_out != a.table) {
+        static std::once_flag once[64];
+        cudaError_t attr = cudaSuccess;
+        std::call_once(once[dev], [&] {
+            attr = cudaFuncSetAttribute(fork_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SmallPlan));
+            if (attr == cudaSuccess)
+                attr = cudaFuncSetAttribute(compact_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(SmallPlan));
+        });
+        CLLM_HOST_TRY(attr);
+        if (fork) fork_small_kernel<<<sms, kSmallThreads, sizeof(SmallPlan), st>>>(a);
+        else compact_small_kernel<<<sms, kSmallThreads, sizeof(SmallPlan), st>>>(a);
+        CLLM_HOST_TRY(cudaGetLastError());
+        return CLLM_OK;
+    }
     const size_t words = ((size_t)a.n_pages + 31) / 32, n = (size_t)a.n_pages;
     const size_t bits = align256(4 * words), list = align256(4 * n), pairs = align256(8 * n);
     const size_t seqs = align256(4 * (size_t)a.n_new);
@@ -231,7 +248,6 @@ static int pages_call(const char* who, PagesArgs a, void* pages, int64_t page_by
     a.first = reinterpret_cast<int*>(take(seqs));
     a.held = reinterpret_cast<int*>(take(seqs));
     a.count = reinterpret_cast<int*>(take(256));
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     CLLM_HOST_TRY(cudaMemsetAsync(ones, 0xFF, 2 * bits + list, st));
     const dim3 mark(a.n_new, (a.max_pages + 1023) / 1024);
     if (mark.y > 65535) return host_fail(CLLM_ERR_TOO_LARGE, "%s: %d pages per sequence", who, a.max_pages);

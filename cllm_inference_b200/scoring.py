@@ -30,17 +30,18 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, top_k
     if tokens is not None and (not tokens.is_cuda or tokens.dtype != torch.int32 or tokens.numel() != rows or
                                not tokens.is_contiguous()):
         raise _lib.CudaError(_lib.ERR_INVALID_ARG, "token_scores: tokens must be int32, contiguous, one per row")
-    dev = logits.device
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    k = max(0, top_k)
+    entropy = logits.new_empty(rows)
     logprob = rank = None
+    tp = lp = rp = 0
     if tokens is not None:
-        logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-        rank = torch.empty(rows, dtype=torch.int32, device=dev)
-    ids = torch.empty((rows, max(0, top_k)), dtype=torch.int32, device=dev)
-    logprobs = torch.empty((rows, max(0, top_k)), dtype=torch.float32, device=dev)
-    _lib.check(_lib.load().cllm_cuda_token_scores(
-        logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab,
-        0 if tokens is None else tokens.data_ptr(), top_k, 0 if tokens is None else logprob.data_ptr(),
-        entropy.data_ptr(), 0 if tokens is None else rank.data_ptr(), ids.data_ptr(), logprobs.data_ptr(),
-        torch.cuda.current_stream(dev).cuda_stream))
+        logprob, rank = torch.empty_like(entropy), torch.empty_like(tokens)
+        tp, lp, rp = tokens.data_ptr(), logprob.data_ptr(), rank.data_ptr()
+    logprobs = logits.new_empty((rows, k))
+    ids = torch.empty_like(logprobs, dtype=torch.int32)
+    rc = _lib.load().cllm_cuda_token_scores(
+        logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, tp, top_k, lp, entropy.data_ptr(),
+        rp, ids.data_ptr(), logprobs.data_ptr(), torch._C._cuda_getCurrentRawStream(logits.get_device()))
+    if rc:
+        _lib.check(rc)
     return TokenScores(logprob, rank, entropy, ids, logprobs)

@@ -36,7 +36,7 @@
 //   whatever the lengths are.  A CTA's four
 //   warps take two tiles each, from a ring of their own that one lane fills with
 //   bulk copies across the runs' borders.  A run that ends inside an item leaves a
-//   partial result, which kv4_join_kernel puts together in order.
+//   partial result, which rows_join puts together in order.
 #pragma once
 #include "kv4_format.cuh"
 
@@ -294,6 +294,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     const AttnArgs& a = ra.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
 
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the prompt kernel needs nothing of this one, the join waits
     const uint32_t full = smem_addr(sm.full[warp]), ring = smem_addr(sm.ring[warp]);
     if (lane == 0) {
         for (int i = 0; i < kRowStages; ++i) mbar_init(full + 8 * i, 1);
@@ -730,12 +731,11 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
 // another's, added in their order: 128 threads per row, four values each.
 constexpr int kJoinThreads = 128 * kRowTile;
 template <int HD>
-__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const RowsArgs ra) {
+__device__ __forceinline__ void rows_join(const RowsArgs& ra) {
     constexpr int kLanes = HD / 4, kGroups = 128 / kLanes;
     __shared__ float s_w[kRowTile][kMaxRowCtas], s_max[kRowTile][4], s_sum[kRowTile][4];
     __shared__ __align__(16) float4 s_o[kRowTile][128];
     const AttnArgs& a = ra.a;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const Part part = ra.last[blockIdx.x];
     if (!part.parts) return;
     const SeqWork w = seq_work(a, part.seq);

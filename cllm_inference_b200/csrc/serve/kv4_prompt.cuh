@@ -19,7 +19,7 @@
 //
 // Work: tiles of (sequence, KV head, 128 rows), numbered through by
 // prompt_plan_kernel and cut into equal runs, one per SM; a run that ends inside an
-// item leaves a partial result for prompt_join_kernel.
+// item leaves a partial result for prompt_join.
 //
 // Warps (5 warpgroups; registers moved to where they are needed):
 //   0       raw tiles of the pages into a ring (bulk copies)
@@ -282,7 +282,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
     const int64_t all = count ? p.items[count].unit : 0;
     const int ctas = (int)min((int64_t)gridDim.x, (all + kPromptMinRun - 1) / kPromptMinRun);
     if (threadIdx.x == 0) p.last[blockIdx.x].parts = 0;
-    if ((int)blockIdx.x >= ctas) return;
+    if ((int)blockIdx.x >= ctas) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     const int64_t run0 = blockIdx.x * all / ctas, run1 = (blockIdx.x + 1) * all / ctas;
     PromptCursor cur;
     {
@@ -784,44 +787,58 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
     __syncthreads();
     tc_fence_after();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    // This kernel may have begun before kv4_rows_kernel, of which it needs nothing, was done; the join needs both.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// The parts of the item that begins in CTA blockIdx.x's run and ends in
-// another's, added in their order: a warp per row, 16 rows per CTA.
+// The parts of the item that begins in CTA `cta`'s run and ends in another's,
+// added in their order: a warp per row, four rows each.
 template <int HD>
-__global__ void __launch_bounds__(512) prompt_join_kernel(const PromptArgs p) {
+__device__ __forceinline__ void prompt_join(const PromptArgs& p, int cta) {
     const AttnArgs& a = p.a;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const PromptPart part = p.last[blockIdx.x];
+    const PromptPart part = p.last[cta];
     if (!part.parts) return;
-    const int row = blockIdx.y * 16 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
     const PromptItem item = p.items[part.item];
     int begin, n;
     seq_rows(a, item.seq, &begin, &n);
-    const int j = item.block * kPromptRows + row;
-    if (j >= n * a.rep) return;
-    auto at = [&](int i) -> int64_t { return (int64_t)(i ? 2 * ((int)blockIdx.x + i) : part.slot) * kPromptRows + row; };
-    float m = -3.0e38f;
-    for (int i = 0; i < part.parts; ++i) m = fmaxf(m, p.part_ml[2 * at(i)]);
-    float sum = 0.f;
-    uint32_t bad = 0;
-    constexpr int V = HD / 32;
-    float x[V];
+    for (int row = threadIdx.x >> 5; row < kPromptRows; row += kJoinThreads / 32) {
+        const int j = item.block * kPromptRows + row;
+        if (j >= n * a.rep) return;
+        auto at = [&](int i) -> int64_t { return (int64_t)(i ? 2 * (cta + i) : part.slot) * kPromptRows + row; };
+        float m = -3.0e38f;
+        for (int i = lane; i < part.parts; i += 32) m = fmaxf(m, p.part_ml[2 * at(i)]);
 #pragma unroll
-    for (int e = 0; e < V; ++e) x[e] = 0.f;
-    for (int i = 0; i < part.parts; ++i) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at(i));
-        const float k = exp2_fast(ml.x - m);
-        sum = fmaf(k, ml.y, sum);
-        bad |= p.part_bad[at(i)];
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        float sum = 0.f;
+        uint32_t bad = 0;
+        constexpr int V = HD / 32;
+        float x[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = fmaf(k, p.part_o[at(i) * HD + 32 * e + lane], x[e]);
+        for (int e = 0; e < V; ++e) x[e] = 0.f;
+#pragma unroll 4
+        for (int i = 0; i < part.parts; ++i) {
+            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at(i));
+            const float k = exp2_fast(ml.x - m);
+            sum = fmaf(k, ml.y, sum);
+            bad |= p.part_bad[at(i)];
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = fmaf(k, p.part_o[at(i) * HD + 32 * e + lane], x[e]);
+        }
+        const int64_t to = (int64_t)(begin + j / a.rep) * a.n_head + part.kvh * a.rep + j % a.rep;
+        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+#pragma unroll
+        for (int e = 0; e < V; ++e) a.out[to * HD + 32 * e + lane] = sum == 0.f ? 0.f : x[e] * (bad >> e & 1 ? NAN : inv);
+        if (a.lse && lane == 0) a.lse[to] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (m + log2f(sum));
     }
-    const int64_t to = (int64_t)(begin + j / a.rep) * a.n_head + part.kvh * a.rep + j % a.rep;
-    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-#pragma unroll
-    for (int e = 0; e < V; ++e) a.out[to * HD + 32 * e + lane] = sum == 0.f ? 0.f : x[e] * (bad >> e & 1 ? NAN : inv);
-    if (a.lse && lane == 0) a.lse[to] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (m + log2f(sum));
+}
+
+// CTAs below rows_ctas join kv4_rows_kernel's parts, the others (if any) kv4_prompt_kernel's.
+template <int HD>
+__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const RowsArgs ra, const PromptArgs pa, int rows_ctas) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if ((int)blockIdx.x < rows_ctas) rows_join<HD>(ra);
+    else prompt_join<HD>(pa, blockIdx.x - rows_ctas);
 }
 
 }  // namespace serve

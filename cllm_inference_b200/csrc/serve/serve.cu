@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 #include "kv4_append.cuh"
 #include "kv4_decode.cuh"
@@ -42,19 +43,21 @@ int check_geometry(const char* who, int n_pages, int page_len, int n_head_kv, in
 // Rows * heads of a KV head up to which a sequence is kv4_rows_kernel's.
 constexpr int kRowsMax = 64;
 
-// Launch `kern` so that its launch overlaps the kernel before it; it starts with griddepcontrol.wait.
-template <class Args>
-int launch_after(void (*kern)(Args), dim3 grid, int threads, cudaStream_t st, const Args& args) {
+// Launch `kern` so that it may start before the kernel before it is done (programmatic
+// dependent launch); it waits with griddepcontrol.wait where it needs to.
+template <class... KArgs>
+int launch_early(void (*kern)(KArgs...), int ctas, int threads, size_t smem, cudaStream_t st, const std::common_type_t<KArgs>&... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
+    cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute pdl[1];
     pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     pdl[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = pdl;
     cfg.numAttrs = 1;
-    CLLM_HOST_TRY(cudaLaunchKernelEx(&cfg, kern, args));
+    CLLM_HOST_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
     return CLLM_OK;
 }
 
@@ -93,12 +96,8 @@ int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
     if (int rc = host_workspace(dev, bytes, &ws, lk)) return rc;
 
     RowsArgs ra{a, reinterpret_cast<Part*>(ws + r_last), reinterpret_cast<float*>(ws + r_ml), reinterpret_cast<float*>(ws + r_o)};
-    kv4_rows_kernel<HD><<<ctas, kRowThreads, sizeof(RowsSmem<HD>), st>>>(ra);
-    CLLM_HOST_TRY(cudaGetLastError());
-    if ((int64_t)a.c.max_pages * a.c.page_len > kStepLen)  // an item can have more than one step
-        if (int rc = launch_after(kv4_join_kernel<HD>, dim3(ctas), kJoinThreads, st, ra)) return rc;
+    PromptArgs pa{};
     if (prompts) {
-        PromptArgs pa{};
         pa.a = a;
         pa.most = (int)most;
         pa.items = reinterpret_cast<PromptItem*>(ws + p_items);
@@ -109,10 +108,13 @@ int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
         pa.part_bad = reinterpret_cast<uint32_t*>(ws + p_bad);
         pa.part_o = reinterpret_cast<float*>(ws + p_o);
         prompt_plan_kernel<<<1, kPromptPlanThreads, 0, st>>>(pa);
-        kv4_prompt_kernel<HD><<<sms, kPromptThreads, sizeof(PromptSmem<HD>) + 1024, st>>>(pa);
-        CLLM_HOST_TRY(cudaGetLastError());
-        if (int rc = launch_after(prompt_join_kernel<HD>, dim3(sms, kPromptRows / 16), 512, st, pa)) return rc;
     }
+    kv4_rows_kernel<HD><<<ctas, kRowThreads, sizeof(RowsSmem<HD>), st>>>(ra);
+    CLLM_HOST_TRY(cudaGetLastError());
+    if (prompts)
+        if (int rc = launch_early(kv4_prompt_kernel<HD>, sms, kPromptThreads, sizeof(PromptSmem<HD>) + 1024, st, pa)) return rc;
+    if (prompts || (int64_t)a.c.max_pages * a.c.page_len > kStepLen)  // an item can have more than one step
+        if (int rc = launch_early(kv4_join_kernel<HD>, ctas + (prompts ? sms : 0), kJoinThreads, 0, st, ra, pa, ctas)) return rc;
     return CLLM_OK;
 }
 

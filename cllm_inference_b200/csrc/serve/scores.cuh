@@ -147,15 +147,25 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_scores_kernel(const Sc
     const int parts = cluster.num_blocks(), part = cluster.block_rank(), row = blockIdx.x / parts;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float* x = a.x + (int64_t)row * a.ld;
-    const int token = a.tokens ? a.tokens[row] : -1;
-    const bool known = token >= 0 && token < a.vocab;
-    float xt = known ? x[token] : INFINITY;
-    if (xt != xt) xt = -INFINITY;
     // groups of four at 16-byte boundaries; up to three logits before and after them
     const int head = min(a.vocab, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / 4);
     const int groups = (a.vocab - head) / 4, tail = head + 4 * groups;
     const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
 
+    // two periods in registers: one on its way, one worked on
+    float4 next[kScoreGroups];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < kScoreGroups; ++u) {
+            const int g = base + u * kScoreThreads + tid;
+            if (g < g1) next[u] = __ldcs(reinterpret_cast<const float4*>(x + head) + g);
+        }
+    };
+    load(g0);
+    const int token = a.tokens ? a.tokens[row] : -1;
+    const bool known = token >= 0 && token < a.vocab;
+    float xt = known ? x[token] : INFINITY;
+    if (xt != xt) xt = -INFINITY;
     const bool odd = known && !(fabsf(xt) < INFINITY);  // an infinite logit: count by the order itself
     const float above = nextafterf(xt, INFINITY);
     float ref = -FLT_MAX, l = 0.f, lc = 0.f;
@@ -219,16 +229,6 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_scores_kernel(const Sc
     if (part == 0 && tid < head) one(tid);
     if (part == parts - 1 && tid < a.vocab - tail) one(tail + tid);
 
-    // two periods in registers: one on its way, one worked on
-    float4 next[kScoreGroups];
-    auto load = [&](int base) {
-#pragma unroll
-        for (int u = 0; u < kScoreGroups; ++u) {
-            const int g = base + u * kScoreThreads + tid;
-            if (g < g1) next[u] = __ldcs(reinterpret_cast<const float4*>(x + head) + g);
-        }
-    };
-    load(g0);
     constexpr int kPeriod = kScoreGroups * kScoreThreads;
     int period = 0;
     auto four = [&](const float4& v, int i) {
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kScoreThreads, 4) token_scores_kernel(const Sc
                 const int at = i * kScoreThreads + tid;
                 if (at < n) top = max(top, sm.list[at] = order_key(__uint_as_float((uint32_t)sm.list[at]), (int)(sm.list[at] >> 32)));
             }
-            if (n > 2 * a.top_k + 16) {  // keep what reaches the bound now
+            if (n > kScoreThreads) {  // keep what reaches the bound now
                 const uint64_t now = reach_bound(top, a.top_k, sm);
                 bound = max(bound, now);
 #pragma unroll

@@ -312,10 +312,19 @@ int cllm_cuda_token_scores(const float* logits, int64_t ld, int rows, int vocab,
     int dev, sms;
     if (int rc = host_device(&dev, &sms)) return rc;
     ScoreArgs a{logits, ld, rows, vocab, top_k, tokens, logprob, entropy, rank, top_ids, top_logprobs};
-    // A cluster of CTAs per row until every SM has its four, each with 4096 logits at least (512 rows of
-    // 128256: 2 CTAs a row 1.5 times as fast as 4, which pay twice for bounds and lists).
+    // CTAs per row (a cluster): what makes the slowest SM's share shortest.  Measured, in cycles: 15000 for what a
+    // CTA does besides reading (bounds, list, join), then 0.19 a logit for each of the up to four CTAs that share an
+    // SM's bandwidth, 0.25 at least.  512 rows of 128256: 1 CTA a row 68 us, 2 (two waves) 77.
     int parts = 1;
-    while (parts < 8 && (int64_t)rows * parts < 4 * (int64_t)sms && vocab / (2 * parts) >= 4096) parts *= 2;
+    double best = 0;
+    for (int p = 1; p <= 8 && (p == 1 || vocab / p >= 4096); p *= 2) {
+        const double ctas = (double)rows * p, waves = std::ceil(ctas / (4.0 * sms)), share = std::min(4.0, std::ceil(ctas / sms));
+        const double cycles = waves * (15000 + std::max(0.25, 0.19 * share) * vocab / p);
+        if (p == 1 || cycles < best) {
+            best = cycles;
+            parts = p;
+        }
+    }
     if ((int64_t)rows * parts > INT_MAX) return host_fail(CLLM_ERR_TOO_LARGE, "token_scores: too many rows");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * parts));

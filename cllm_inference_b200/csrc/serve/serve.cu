@@ -160,11 +160,11 @@ int cllm_cuda_kv4_append(const float* q, int64_t ldq, float* q_out, const float*
             ldkv % 4 == 0 && (n_head == 0 || ldq % 4 == 0);
     a.c = Cache{static_cast<uint8_t*>(pages), page_table, nullptr, n_pages, page_len, n_head_kv, n_seqs, max_pages};
     a.rope_vec = aligned16(rope_table);
-    // Steps of a warp: as many as leave 32 warps for every SM, up to 12 (2048 tokens of 48 heads: see kv4_append.cuh).
+    // Vectors of a warp: as many as leave 32 warps for every SM, up to 12 steps' worth.
     const int vecs = 128 / head_dim, warps = kAppendThreads / 32;
-    const int64_t steps = (n_head + 2 * n_head_kv + vecs - 1) / vecs;
-    a.span = (int)std::max<int64_t>(1, std::min<int64_t>(12, n_tok * steps / (32 * (int64_t)sms)));
-    const int64_t ctas = (n_tok * ((steps + a.span - 1) / a.span) + warps - 1) / warps;
+    const int64_t units = n_head + 2 * n_head_kv, steps = (units + vecs - 1) / vecs;
+    a.span = vecs * (int)std::max<int64_t>(1, std::min<int64_t>(12, n_tok * steps / (32 * (int64_t)sms)));
+    const int64_t ctas = (n_tok * ((units + a.span - 1) / a.span) + warps - 1) / warps;
     if (ctas > INT_MAX) return host_fail(CLLM_ERR_TOO_LARGE, "kv4_append: too many tokens in one call");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (head_dim == 128) kv4_append_kernel<128><<<(unsigned)ctas, kAppendThreads, 0, st>>>(a);

@@ -209,7 +209,7 @@ int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int
 
 static int pages_call(const char* who, PagesArgs a, void* pages, int64_t page_bytes, bool fork, void* stream) {
     if (a.n_layers <= 0 || a.n_pages <= 0 || a.page_len <= 0 || a.page_len % kTile || a.max_pages <= 0 ||
-        page_bytes <= 0 || page_bytes % 16 || (int64_t)a.max_pages * a.page_len > INT_MAX)
+        page_bytes <= 0 || page_bytes % 16 || page_bytes > (int64_t(1) << 34) || (int64_t)a.max_pages * a.page_len > INT_MAX)
         return host_fail(CLLM_ERR_INVALID_ARG, "%s: bad sizes", who);
     if (!aligned16(pages)) return host_fail(CLLM_ERR_INVALID_ARG, "%s: pages must be 16-byte aligned", who);
     int dev, sms;

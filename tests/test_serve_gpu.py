@@ -250,6 +250,25 @@ def test_attention_a_nan_stays_with_the_rows_that_see_it(cuda, lib, rows):
     assert not np.isnan(o[0, ~sees]).any() and not np.isnan(o[0, :, 1]).any() and not np.isnan(o[1]).any()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [1, 3, 50])
+def test_attention_a_nan_of_the_values_stays_in_its_group(cuda, lib, rows, hd):
+    rng = np.random.default_rng(rows + hd)
+    cache, p, table = _cache(rng, 1, 12, 64, 2, hd, [200, 210], 4)
+    g = hd // 32 - 1
+    at = p[0, table[0, 190 // 64], 1, 190 % 64 // 16]
+    o = 18 * hd + (190 % 16) * hd // 8 + 4 * g
+    at[o:o + 4] = 0xFF  # value of position 190, head 1, last group, sequence 0
+    cache.pages.copy_(torch.from_numpy(p))
+    q = torch.from_numpy(rng.standard_normal((2 * rows, 4 * hd)).astype(np.float32)).cuda()
+    begin = torch.tensor([0, rows, 2 * rows], dtype=torch.int32, device="cuda")
+    got = cache.attention(0, q, begin=begin).cpu().numpy().reshape(2, rows, 2, 2, hd // 32, 32)
+    sees = 200 - (rows - 1 - np.arange(rows)) > 190
+    assert np.isnan(got[0, sees, 1, :, g]).all()
+    got[0, sees, 1, :, g] = 0
+    assert not np.isnan(got).any()
+
+
 def test_attention_lengths_beyond_the_table_and_bad_pages(cuda, lib):
     hd = 64
     rng = np.random.default_rng(7)
@@ -397,6 +416,24 @@ def test_fork_and_compact_large_tables(cuda, lib, pool, n_seqs, slots):
     np.testing.assert_array_equal(new.pages.cpu().numpy(), pages)
 
 
+@pytest.mark.parametrize("pool,n_seqs", [(500, 30), (40000, 30)])
+def test_compact_in_place(cuda, lib, pool, n_seqs):
+    """The C call may write the table that it reads."""
+    rng = np.random.default_rng(n_seqs)
+    lens = rng.integers(0, 16 * 8 + 1, n_seqs).astype(np.int32)
+    cache, pages, table = _cache(rng, 2, pool, 16, 1, 64, lens.tolist(), 8)
+    want, n_live, moves = O.compact(table, lens, pool, 16)
+    for a, b in moves:
+        pages[:, b] = pages[:, a]
+    live = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _lib.check(lib.cllm_cuda_kv4_compact(cache.pages.data_ptr(), 2, pool, cache.page_bytes, 16, cache.table.data_ptr(),
+                                         cache.lens.data_ptr(), n_seqs, 8, cache.table.data_ptr(), live.data_ptr(),
+                                         torch.cuda.current_stream().cuda_stream))
+    assert int(live[0]) == n_live
+    np.testing.assert_array_equal(cache.table.cpu().numpy(), want)
+    np.testing.assert_array_equal(cache.pages.cpu().numpy(), pages)
+
+
 def test_fork_of_a_bad_page_sets_the_status(cuda, lib):
     rng = np.random.default_rng(1)
     cache, _, table = _cache(rng, 1, 9, 16, 1, 64, [40, 40], 3)
@@ -541,4 +578,45 @@ def test_refusals_of_the_front_ends(cuda, lib):
     assert cache.append(0, f(0, 128), f(0, 128), ints(0), ints(0)) is None
     assert cache.fork(ints(0), ints(0)).n_seqs == 0
     assert token_scores(f(0, 50), ints(0), 3).top_ids.shape == (0, 3)
+    _lib.check(lib.cllm_cuda_check_device_status())
+
+
+# ---- together ---------------------------------------------------------------------------
+
+
+def test_best_of_n_example(cuda, lib):
+    """The example's candidates, taken again in one piece each, get the probabilities that they got step by step.
+
+    Rows of a batch are quantized to Q8_0 before every matmul, and a last-bit difference between the batched and
+    the one-row kernels can move a value by a whole step: the band is the engine's 5 % of the logits' scale
+    (test_engine_gpu.py)."""
+    import importlib.util
+    import os
+
+    from cllm_inference_b200 import gguf
+    from cllm_inference_b200.kv4 import KV4Cache
+    from cllm_inference_b200.scoring import token_scores
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "best_of_n.py")
+    spec = importlib.util.spec_from_file_location("best_of_n", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    model = ex.Model(gguf.LlamaShape(2, 1024, 8, 2, 2048, 5000, 256))
+    prompt = np.random.default_rng(1).integers(0, 5000, 75).tolist()
+    steps = 12
+    tokens, scores, in_use, cache = ex.best_of_n(model, prompt, n=5, steps=steps, keep=2)
+    assert tokens.shape == scores.shape == (2, steps) and cache.n_seqs == 2
+    pages = {int(p) for row in cache.table.tolist() for p in row if p >= 0}
+    assert in_use == len(pages) and pages == set(range(in_use))
+    assert in_use < 2 * -(-(75 + steps) // 16)  # the prompt's whole pages are shared
+    for c in range(2):
+        text = prompt + tokens[c].tolist()[:-1]
+        whole = KV4Cache.empty(2, 8, 16, 2, 128, 1, 8).fork(ex.ints(-1), ex.ints(len(text)))
+        n = len(text)
+        logits = model.rows(whole, torch.tensor(text, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda"),
+                            torch.arange(n, dtype=torch.int32, device="cuda"), begin=ex.ints(0, n),
+                            last=list(range(74, n)))
+        again = token_scores(logits, tokens[c].contiguous()).logprob
+        scale = float(logits.std())
+        assert float((again - scores[c]).abs().max()) <= 0.05 * scale * 4  # logits within 4 deviations
     _lib.check(lib.cllm_cuda_check_device_status())

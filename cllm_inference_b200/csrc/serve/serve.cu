@@ -40,8 +40,18 @@ int check_geometry(const char* who, int n_pages, int page_len, int n_head_kv, in
     return CLLM_OK;
 }
 
-// Rows * heads of a KV head up to which a sequence is kv4_rows_kernel's.
-constexpr int kRowsMax = 64;
+// Rows (of all heads of a KV head) up to which a sequence is kv4_rows_kernel's.  Its time grows with every 8 rows, the
+// prompt kernel's only with every 128.  8 KV heads of 128, us, rows kernel / prompt kernel at 16, 48, 64, 128 rows:
+//   16 sequences of 1024 positions    40/71    71/81    83/83    138/81
+//   64 of 1024                        85/183   194/218  249/220  466/196
+//   16 of 8192                        126/271  318/302  411/304  787/259
+constexpr int kRowsMax = 48;
+// A call of no more rows than this in all is the rows kernel's alone, without the launches that look for prompts.  One
+// sequence at 48, 64, 128 rows:
+//   500 positions    19/44    22/44    26/54
+//   4096             32/56    34/54    46/71
+//   32768            95/114   120/116  216/126
+constexpr int kRowsAlone = 64;
 
 // Launch `kern` so that it may start before the kernel before it is done (programmatic
 // dependent launch); it waits with griddepcontrol.wait where it needs to.
@@ -160,10 +170,13 @@ int cllm_cuda_kv4_append(const float* q, int64_t ldq, float* q_out, const float*
             ldkv % 4 == 0 && (n_head == 0 || ldq % 4 == 0);
     a.c = Cache{static_cast<uint8_t*>(pages), page_table, nullptr, n_pages, page_len, n_head_kv, n_seqs, max_pages};
     a.rope_vec = aligned16(rope_table);
-    // Vectors of a warp: as many as leave 32 warps for every SM, up to 12 steps' worth.
+    // Vectors of a warp: as many as leave 32 warps for every SM, up to 12 steps' worth, in whole rounds of loads.
+    // 32 query and 16 other vectors of 128 a token, us at 1 step a warp / 12 / by the rule: 64 tokens 10/14/8, 512
+    // 20/16/14, 1024 35/18/18, 2048 61/31/31.
     const int vecs = 128 / head_dim, warps = kAppendThreads / 32;
     const int64_t units = n_head + 2 * n_head_kv, steps = (units + vecs - 1) / vecs;
-    a.span = vecs * (int)std::max<int64_t>(1, std::min<int64_t>(12, n_tok * steps / (32 * (int64_t)sms)));
+    const int64_t share = std::min<int64_t>(12, n_tok * steps / (32 * (int64_t)sms));
+    a.span = vecs * (int)(share <= 1 ? 1 : (share + kAppendTogether - 1) / kAppendTogether * kAppendTogether);
     const int64_t ctas = (n_tok * ((units + a.span - 1) / a.span) + warps - 1) / warps;
     if (ctas > INT_MAX) return host_fail(CLLM_ERR_TOO_LARGE, "kv4_append: too many tokens in one call");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -196,7 +209,7 @@ int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int
     if (int rc = host_device(&dev, &sms)) return rc;
     AttnArgs a{};
     a.q = q; a.ldq = ldq; a.q_begin = q_begin; a.n_tok = n_tok; a.n_head = n_head; a.rep = n_head / n_head_kv;
-    a.rows_max = std::max(kRowsMax, a.rep);
+    a.rows_max = std::max((int64_t)n_tok * a.rep <= kRowsAlone ? kRowsAlone : kRowsMax, a.rep);
     a.scale = scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale;
     a.out = out; a.lse = lse;
     a.c = Cache{const_cast<uint8_t*>(static_cast<const uint8_t*>(pages)), page_table, seq_len, n_pages, page_len,
@@ -217,7 +230,8 @@ static int pages_call(const char* who, PagesArgs a, void* pages, int64_t page_by
     a.pages = static_cast<uint8_t*>(pages);
     a.page_bytes = page_bytes;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // Tables that a CTA can hold: one launch (192 sequences of 8 pages 12 us less than four launches).
+    // Tables that a CTA can hold: one launch instead of four.  8 sequences of 17 pages 11.3 us instead of 16.9, 192 of 8
+    // 16.5 instead of 21.3, compact of 96 of 14 in a pool of 2048 55.3 instead of 60.6.
     if (a.n_pages <= kSmallPages && a.n_new <= kSmallSeqs && (int64_t)a.n_new * a.max_pages <= kSmallEntries &&
         a.table_out != a.table) {
         static std::once_flag once[64];

@@ -72,19 +72,22 @@ struct AttnArgs {
     }
 };
 
-// An item that begins in a CTA's run and ends in another's.
-struct Part {
-    int seq, item;  // item: KV head * row groups + row group
-    int parts;      // CTAs that have a part of it, this one first; 0: nothing to join here
-    int slot;       // of this CTA's part (the others': their first slot)
-};
-
+// An item that lies in several CTAs' runs has a part in each.  CTA c keeps the
+// part that the item begins with in slot 2c + 1, another's continuation in 2c.
 struct RowsArgs {
     AttnArgs a;
-    Part* last;      // [ctas]
-    float* part_ml;  // [2 * ctas][kRowTile][2] reference (log2) and sum; slot 2c: first item of CTA c, 2c + 1: last
+    int set;         // of g_rows_arrived, that this call counts in
+    float* part_ml;  // [2 * ctas][kRowTile][2] reference (log2) and sum
     float* part_o;   // [2 * ctas][kRowTile][HD]
 };
+// Parts of the item that begins in CTA c that are there.  The last one to come
+// sets it back to 0.  Every call clears the other set, so a wrong count (calls
+// that overlapped, which their caller must not let happen) does not stay.
+__device__ unsigned g_rows_arrived[2][kMaxRowCtas];
+
+// CTA whose run has unit u: runs begin at floor(c * all / ctas).
+__device__ __forceinline__ int run_of(int64_t u, int ctas, int64_t all) { return (int)(((u + 1) * ctas - 1) / all); }
+__device__ __forceinline__ int part_slot(int c0, int i) { return i ? 2 * (c0 + i) : 2 * c0 + 1; }  // part i of c0's item
 
 // ---- rows of a sequence -------------------------------------------------------
 
@@ -284,6 +287,71 @@ __device__ __forceinline__ uint32_t keep(uint32_t x) {
 // a row group then holds the positions 4t .. 4t+3, whose scale rows lie in different banks for all t.
 __device__ __forceinline__ int tile_pos(int i, int r) { return 4 * (r >> 1) + 2 * i + ((r & 1) ^ (r >> 2)); }
 
+// ---- the parts of an item ------------------------------------------------------------
+
+// Added in their order, whichever CTA does it.  A lane has four values of a row.
+// Other CTAs wrote them during this kernel: read past L1.
+template <int HD>
+__device__ __forceinline__ void rows_join(const RowsArgs& ra, int c0, int parts, const SeqWork& w, int kvh, int row0) {
+    constexpr int kLanes = HD / 4, kPass = kRowWarps * (32 / kLanes), kPasses = kRowTile / kPass;
+    const AttnArgs& a = ra.a;
+    const int d = threadIdx.x % kLanes, r0 = threadIdx.x / kLanes;
+    float m[kPasses], sum[kPasses];
+    float4 x[kPasses];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        m[p] = -3.0e38f;
+        sum[p] = 0.f;
+        x[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    auto ml = [&](int i, int p) {
+        return __ldcg(reinterpret_cast<const float2*>(ra.part_ml) + (int64_t)part_slot(c0, i) * kRowTile + r0 + p * kPass);
+    };
+#pragma unroll 1
+    for (int i = d; i < parts; i += kLanes)
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) m[p] = fmaxf(m[p], ml(i, p).x);
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) m[p] = fmaxf(m[p], __shfl_xor_sync(0xFFFFFFFFu, m[p], o));
+#pragma unroll 1
+    for (int base = 0; base < parts; base += kLanes) {
+        float k[kPasses];  // the weight of part base + d
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+            const float2 z = base + d < parts ? ml(base + d, p) : make_float2(-INFINITY, 0.f);
+            k[p] = exp2_fast(z.x - m[p]);
+            sum[p] = fmaf(k[p], z.y, sum[p]);
+        }
+        const int n = min(kLanes, parts - base);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i)
+#pragma unroll
+            for (int p = 0; p < kPasses; ++p) {
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(
+                    ra.part_o + ((int64_t)part_slot(c0, base + i) * kRowTile + r0 + p * kPass) * HD + 4 * d));
+                const float by = __shfl_sync(0xFFFFFFFFu, k[p], i, kLanes);
+                x[p].x = fmaf(by, y.x, x[p].x); x[p].y = fmaf(by, y.y, x[p].y);
+                x[p].z = fmaf(by, y.z, x[p].z); x[p].w = fmaf(by, y.w, x[p].w);
+            }
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) sum[p] += __shfl_xor_sync(0xFFFFFFFFu, sum[p], o);
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const int row = row0 + r0 + p * kPass;
+        if (row >= w.n * a.rep) break;
+        const int64_t at = (int64_t)(w.begin + row / a.rep) * a.n_head + kvh * a.rep + row % a.rep;
+        const float inv = sum[p] == 0.f ? 0.f : __fdiv_rn(1.f, sum[p]);
+        *reinterpret_cast<float4*>(a.out + at * HD + 4 * d) =
+            sum[p] == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x[p].x * inv, x[p].y * inv, x[p].z * inv, x[p].w * inv);
+        if (a.lse && d == 0) a.lse[at] = sum[p] == 0.f ? -INFINITY : 0.69314718055994530942f * (m[p] + log2f(sum[p]));
+    }
+}
+
 // ---- the kernel --------------------------------------------------------------------
 
 template <int HD>
@@ -294,7 +362,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     const AttnArgs& a = ra.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the prompt kernel needs nothing of this one, the join waits
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the prompt kernel needs nothing of this one
     const uint32_t full = smem_addr(sm.full[warp]), ring = smem_addr(sm.ring[warp]);
     if (lane == 0) {
         for (int i = 0; i < kRowStages; ++i) mbar_init(full + 8 * i, 1);
@@ -321,7 +389,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     int64_t all;
     const int64_t before = cta_scan(mine, sm.scan, &all);
     const int ctas = (int)min((int64_t)gridDim.x, all);
-    if (threadIdx.x == 0) ra.last[blockIdx.x].parts = 0;
+    if (threadIdx.x == 0) g_rows_arrived[ra.set ^ 1][blockIdx.x] = 0;
     if ((int)blockIdx.x >= ctas) return;
     const int64_t run0 = blockIdx.x * all / ctas, run1 = (blockIdx.x + 1) * all / ctas;
     if (mine && before <= run0 && run0 < before + mine) {
@@ -402,7 +470,6 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     const uint32_t at_v = keep(Tile<HD>::kV + lane * (HD / 8));                                       // values' numbers
     const uint32_t low = keep(t < 2 ? 0x5410u : 0x1054u), high = keep(t < 2 ? 0x7632u : 0x3276u);
     constexpr uint32_t kToV = Tile<HD>::kScaleV - Tile<HD>::kScaleK, kTwo = 2 * (HD / 8);             // two rows on
-    bool first = true;  // the run's first item
     while (cur.left > 0) {
         // ---- one item (or the part of it inside the run)
         const int units = min(cur.left, cur.w.units() - cur.unit), groups = cur.w.items / a.c.n_kv;
@@ -687,8 +754,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
         }
         __syncthreads();
         const bool whole = step1 - step0 == cur.w.steps;
-        const int slot = 2 * blockIdx.x + (first ? 0 : 1);
-        first = false;
+        const int slot = 2 * blockIdx.x + (step0 == 0 ? 1 : 0);
         for (int i = threadIdx.x; i < kRowTile * HD / 4; i += kRowThreads) {
             const int rr = i / (HD / 4), d = 4 * (i % (HD / 4));
             float m = sm.ml[0][rr][0];
@@ -716,71 +782,26 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                 if (d == 0) *reinterpret_cast<float2*>(ra.part_ml + (slot * kRowTile + rr) * 2) = make_float2(m, sum);
             }
         }
-        if (!whole && step0 == 0 && threadIdx.x == 0) {  // the item begins here and ends in another CTA
-            const int64_t end = run1 - cur.left + cur.w.units() - cur.unit;  // number of the unit after the item
-            ra.last[blockIdx.x] = Part{cur.s, cur.item, (int)((end * ctas - 1) / all) - (int)blockIdx.x + 1, slot};
+        if (!whole) {  // the CTA whose part is the last to come joins them
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const int64_t unit0 = run1 - cur.left - cur.unit;  // number of the item's first unit
+                const int c0 = run_of(unit0 + kItemUnits, ctas, all), c1 = run_of(unit0 + cur.w.units() - 1, ctas, all);
+                __threadfence();
+                const bool last = atomicAdd(&g_rows_arrived[ra.set][c0], 1u) == (unsigned)(c1 - c0);
+                if (last) g_rows_arrived[ra.set][c0] = 0;
+                __threadfence();
+                sm.start[0] = last ? c1 - c0 + 1 : 0;
+                sm.start[1] = c0;
+            }
+            __syncthreads();
+            if (sm.start[0]) rows_join<HD>(ra, sm.start[1], sm.start[0], cur.w, kvh, row0);
         }
         __syncthreads();
         cur.next(a, units);
     }
     if (!alive)  // let the copies in flight land before the CTA ends
         for (; get.i != put.i || get.parity != put.parity; get.next()) wait_full(full + 8 * get.i, get.parity);
-}
-
-// The parts of the item that begins in CTA blockIdx.x's run and ends in
-// another's, added in their order: 128 threads per row, four values each.
-constexpr int kJoinThreads = 128 * kRowTile;
-template <int HD>
-__device__ __forceinline__ void rows_join(const RowsArgs& ra) {
-    constexpr int kLanes = HD / 4, kGroups = 128 / kLanes;
-    __shared__ float s_w[kRowTile][kMaxRowCtas], s_max[kRowTile][4], s_sum[kRowTile][4];
-    __shared__ __align__(16) float4 s_o[kRowTile][128];
-    const AttnArgs& a = ra.a;
-    const Part part = ra.last[blockIdx.x];
-    if (!part.parts) return;
-    const SeqWork w = seq_work(a, part.seq);
-    const int groups = w.items / a.c.n_kv, kvh = part.item / groups;
-    const int rr = threadIdx.x >> 7, tid = threadIdx.x & 127, row = (part.item - kvh * groups) * kRowTile + rr;
-    auto slot = [&](int i) -> int64_t { return (int64_t)(i ? 2 * ((int)blockIdx.x + i) : part.slot) * kRowTile + rr; };
-    float m = -3.0e38f;
-    for (int i = tid; i < part.parts; i += 128) m = fmaxf(m, ra.part_ml[2 * slot(i)]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if ((tid & 31) == 0) s_max[rr][tid >> 5] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(s_max[rr][0], s_max[rr][1]), fmaxf(s_max[rr][2], s_max[rr][3]));
-    float sum = 0.f;
-    for (int i = tid; i < part.parts; i += 128) {
-        const float2 x = *reinterpret_cast<const float2*>(ra.part_ml + 2 * slot(i));
-        s_w[rr][i] = exp2_fast(x.x - m);
-        sum = fmaf(s_w[rr][i], x.y, sum);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    if ((tid & 31) == 0) s_sum[rr][tid >> 5] = sum;
-    __syncthreads();
-    sum = (s_sum[rr][0] + s_sum[rr][1]) + (s_sum[rr][2] + s_sum[rr][3]);
-    const int d = tid % kLanes, g = tid / kLanes;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = g; i < part.parts; i += kGroups) {
-        const float k = s_w[rr][i];
-        const float4 y = *reinterpret_cast<const float4*>(ra.part_o + slot(i) * HD + 4 * d);
-        x.x = fmaf(k, y.x, x.x); x.y = fmaf(k, y.y, x.y); x.z = fmaf(k, y.z, x.z); x.w = fmaf(k, y.w, x.w);
-    }
-    s_o[rr][tid] = x;
-    __syncthreads();
-    if (g || row >= w.n * a.rep) return;
-#pragma unroll
-    for (int i = 1; i < kGroups; ++i) {
-        const float4 y = s_o[rr][i * kLanes + d];
-        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-    }
-    const int64_t at = (int64_t)(w.begin + row / a.rep) * a.n_head + kvh * a.rep + row % a.rep;
-    const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-    *reinterpret_cast<float4*>(a.out + at * HD + 4 * d) =
-        sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-    if (a.lse && d == 0) a.lse[at] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (m + log2f(sum));
 }
 
 }  // namespace serve

@@ -70,6 +70,7 @@ struct PromptSmem {
     uint64_t alpha_full[4], stat_full[kStats], q_full, done;
     uint32_t tmem;
     int abort;
+    int join[2];
 };
 
 // One lane of the warp.  The compiler knows that a branch on this has one thread
@@ -150,20 +151,17 @@ struct PromptItem {
     int seq, block, tiles, pad;
     int64_t unit;  // units (tiles + kPromptUnits, times KV heads) of the items before it
 };
-// An item that begins in a CTA's run and ends in another's.
-struct PromptPart {
-    int item, kvh, parts, slot;
-};
 struct PromptArgs {
     AttnArgs a;
     int most;            // room for items
     PromptItem* items;   // [most + 1]; the last one's unit is the total
     int* seq_items;      // [n_seqs] scratch
     int* count;          // items
-    PromptPart* last;    // [ctas]
+    int ctas;
+    unsigned* arrived;   // [ctas] parts of the item that begins in CTA c that are there; the plan clears it
     float* part_ml;      // [2 * ctas][128][2]
     uint32_t* part_bad;  // [2 * ctas][128]
-    float* part_o;       // [2 * ctas][128][HD]
+    float* part_o;       // [2 * ctas][HD / 4][128][4]
 };
 
 __device__ __forceinline__ int prompt_tiles(int len, int n, int rep, int block) {
@@ -198,6 +196,7 @@ __global__ void __launch_bounds__(kPromptPlanThreads) prompt_plan_kernel(const P
         const int64_t before = __shfl_sync(0xFFFFFFFFu, w, max(0, warp - 1));
         return x - v + (warp ? before : 0);
     };
+    for (int i = threadIdx.x; i < p.ctas; i += kPromptPlanThreads) p.arrived[i] = 0;
     int64_t count = 0;
     for (int base = 0; base < a.c.n_seqs; base += kPromptPlanThreads) {
         const int s = base + threadIdx.x;
@@ -264,6 +263,58 @@ struct PromptCursor {
     __device__ __forceinline__ bool here(int from, int to) const { return from < to || (tiles == 0 && unit == 0); }
 };
 
+// The parts of an item, added in their order whichever CTA does it: thread =
+// row, 64 values at a time, so that 16 loads are in flight.  Other CTAs wrote
+// them during this kernel: read past L1.
+template <int HD>
+__device__ __forceinline__ void prompt_join(const PromptArgs& p, int c0, int parts, const PromptItem& item, int begin, int n,
+                                            int kvh, int row) {
+    const AttnArgs& a = p.a;
+    auto ml = [&](int i) {
+        return __ldcg(reinterpret_cast<const float2*>(p.part_ml) + (int64_t)part_slot(c0, i) * kPromptRows + row);
+    };
+    float m = -3.0e38f, sum = 0.f;
+    uint32_t bad = 0;
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, ml(i).x);
+    const int j = item.block * kPromptRows + row;
+    const bool live = j < n * a.rep;
+    const int64_t at = (int64_t)(begin + j / a.rep) * a.n_head + kvh * a.rep + j % a.rep;
+#pragma unroll 1
+    for (int h = 0; h < HD; h += 64) {
+        float4 x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        sum = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < parts; ++i) {
+            const float4* from = reinterpret_cast<const float4*>(p.part_o) +
+                                 ((int64_t)part_slot(c0, i) * (HD / 4) + h / 4) * kPromptRows + row;
+            float4 y[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = __ldcg(from + e * kPromptRows);
+            const float2 z = ml(i);
+            bad |= __ldcg(p.part_bad + (int64_t)part_slot(c0, i) * kPromptRows + row);
+            const float k = exp2_fast(z.x - m);
+            sum = fmaf(k, z.y, sum);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                x[e].x = fmaf(k, y[e].x, x[e].x); x[e].y = fmaf(k, y[e].y, x[e].y);
+                x[e].z = fmaf(k, y[e].z, x[e].z); x[e].w = fmaf(k, y[e].w, x[e].w);
+            }
+        }
+        if (!live) continue;
+        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float by = bad >> (h / 32 + e / 8) & 1 ? NAN : inv;
+            *reinterpret_cast<float4*>(a.out + at * HD + h + 4 * e) =
+                sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x[e].x * by, x[e].y * by, x[e].z * by, x[e].w * by);
+        }
+    }
+    if (live && a.lse) a.lse[at] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (m + log2f(sum));
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const PromptArgs p) {
     constexpr int G = Tile<HD>::G;
@@ -281,7 +332,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
     const int count = *p.count;
     const int64_t all = count ? p.items[count].unit : 0;
     const int ctas = (int)min((int64_t)gridDim.x, (all + kPromptMinRun - 1) / kPromptMinRun);
-    if (threadIdx.x == 0) p.last[blockIdx.x].parts = 0;
     if ((int)blockIdx.x >= ctas) {
         asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
@@ -599,17 +649,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     if (a.lse) a.lse[at] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (ref + log2f(sum));
                 }
             } else {
-                const int slot = 2 * blockIdx.x + (items ? 1 : 0);
-                float* out = p.part_o + ((int64_t)slot * kPromptRows + row) * HD;
+                const int slot = 2 * blockIdx.x + (from == 0 ? 1 : 0);
+                float4* out = reinterpret_cast<float4*>(p.part_o) + (int64_t)slot * (kPromptRows * HD / 4) + row;
 #pragma unroll
                 for (int i = 0; i < HD / 2; i += 2)
-                    *reinterpret_cast<float4*>(out + 2 * i) = make_float4(acc[i].x, acc[i].y, acc[i + 1].x, acc[i + 1].y);
+                    out[i / 2 * kPromptRows] = make_float4(acc[i].x, acc[i].y, acc[i + 1].x, acc[i + 1].y);
                 *reinterpret_cast<float2*>(p.part_ml + 2 * (slot * kPromptRows + row)) = make_float2(ref, sum);
                 p.part_bad[slot * kPromptRows + row] = bad;
-                if (from == 0 && row == 0) {  // it begins here and ends in another CTA
-                    const int64_t end = item.unit + (int64_t)(cur.kvh + 1) * (item.tiles + kPromptUnits);
-                    p.last[blockIdx.x] = PromptPart{cur.item, cur.kvh, (int)((end * ctas - 1) / all) - (int)blockIdx.x + 1, slot};
+                // the CTA whose part is the last to come joins them
+                asm volatile("bar.sync 5, 128;" ::: "memory");
+                if (row == 0) {
+                    const int64_t unit0 = item.unit + (int64_t)cur.kvh * (item.tiles + kPromptUnits);
+                    const int c0 = run_of(unit0 + kPromptUnits, ctas, all);
+                    const int c1 = run_of(unit0 + kPromptUnits + item.tiles - 1, ctas, all);
+                    __threadfence();
+                    const bool last = atomicAdd(&p.arrived[c0], 1u) == (unsigned)(c1 - c0);
+                    __threadfence();
+                    sm.join[0] = last ? c1 - c0 + 1 : 0;
+                    sm.join[1] = c0;
                 }
+                asm volatile("bar.sync 5, 128;" ::: "memory");
+                if (sm.join[0]) prompt_join<HD>(p, sm.join[1], sm.join[0], item, begin, n, cur.kvh, row);
             }
             ++items;
         }
@@ -787,58 +847,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
     __syncthreads();
     tc_fence_after();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
-    // This kernel may have begun before kv4_rows_kernel, of which it needs nothing, was done; the join needs both.
+    // This kernel may have begun before kv4_rows_kernel, of which it needs nothing, was done; what follows both waits
+    // for this one.
     asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
-// The parts of the item that begins in CTA `cta`'s run and ends in another's,
-// added in their order: a warp per row, four rows each.
-template <int HD>
-__device__ __forceinline__ void prompt_join(const PromptArgs& p, int cta) {
-    const AttnArgs& a = p.a;
-    const PromptPart part = p.last[cta];
-    if (!part.parts) return;
-    const int lane = threadIdx.x & 31;
-    const PromptItem item = p.items[part.item];
-    int begin, n;
-    seq_rows(a, item.seq, &begin, &n);
-    for (int row = threadIdx.x >> 5; row < kPromptRows; row += kJoinThreads / 32) {
-        const int j = item.block * kPromptRows + row;
-        if (j >= n * a.rep) return;
-        auto at = [&](int i) -> int64_t { return (int64_t)(i ? 2 * (cta + i) : part.slot) * kPromptRows + row; };
-        float m = -3.0e38f;
-        for (int i = lane; i < part.parts; i += 32) m = fmaxf(m, p.part_ml[2 * at(i)]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        float sum = 0.f;
-        uint32_t bad = 0;
-        constexpr int V = HD / 32;
-        float x[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = 0.f;
-#pragma unroll 4
-        for (int i = 0; i < part.parts; ++i) {
-            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at(i));
-            const float k = exp2_fast(ml.x - m);
-            sum = fmaf(k, ml.y, sum);
-            bad |= p.part_bad[at(i)];
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[e] = fmaf(k, p.part_o[at(i) * HD + 32 * e + lane], x[e]);
-        }
-        const int64_t to = (int64_t)(begin + j / a.rep) * a.n_head + part.kvh * a.rep + j % a.rep;
-        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-#pragma unroll
-        for (int e = 0; e < V; ++e) a.out[to * HD + 32 * e + lane] = sum == 0.f ? 0.f : x[e] * (bad >> e & 1 ? NAN : inv);
-        if (a.lse && lane == 0) a.lse[to] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (m + log2f(sum));
-    }
-}
-
-// CTAs below rows_ctas join kv4_rows_kernel's parts, the others (if any) kv4_prompt_kernel's.
-template <int HD>
-__global__ void __launch_bounds__(kJoinThreads) kv4_join_kernel(const RowsArgs ra, const PromptArgs pa, int rows_ctas) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if ((int)blockIdx.x < rows_ctas) rows_join<HD>(ra);
-    else prompt_join<HD>(pa, blockIdx.x - rows_ctas);
 }
 
 }  // namespace serve

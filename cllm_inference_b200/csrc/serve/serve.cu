@@ -71,6 +71,8 @@ int launch_early(void (*kern)(KArgs...), int ctas, int threads, size_t smem, cud
     return CLLM_OK;
 }
 
+int g_set[64];  // of g_rows_arrived, the last call's; host_workspace's lock guards it
+
 template <int HD>
 int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
     static std::once_flag once[64];
@@ -95,17 +97,17 @@ int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
         bytes += align256(n);
         return at;
     };
-    const size_t r_last = part(sizeof(Part) * ctas), r_ml = part((size_t)2 * ctas * kRowTile * 2 * 4);
+    const size_t r_ml = part((size_t)2 * ctas * kRowTile * 2 * 4);
     const size_t r_o = part((size_t)2 * ctas * kRowTile * HD * 4);
     const size_t p_items = part(prompts ? sizeof(PromptItem) * (most + 1) : 0), p_seq = part(prompts ? 4 * (size_t)a.c.n_seqs : 0);
-    const size_t p_count = part(256), p_last = part(sizeof(PromptPart) * sms);
+    const size_t p_count = part(256), p_arrived = part(4 * (size_t)sms);
     const size_t p_ml = part(prompts ? (size_t)2 * sms * kPromptRows * 2 * 4 : 0), p_bad = part(prompts ? (size_t)2 * sms * kPromptRows * 4 : 0);
     const size_t p_o = part(prompts ? (size_t)2 * sms * kPromptRows * HD * 4 : 0);
     uint8_t* ws;
     std::unique_lock<std::mutex> lk;
     if (int rc = host_workspace(dev, bytes, &ws, lk)) return rc;
 
-    RowsArgs ra{a, reinterpret_cast<Part*>(ws + r_last), reinterpret_cast<float*>(ws + r_ml), reinterpret_cast<float*>(ws + r_o)};
+    RowsArgs ra{a, g_set[dev] ^= 1, reinterpret_cast<float*>(ws + r_ml), reinterpret_cast<float*>(ws + r_o)};
     PromptArgs pa{};
     if (prompts) {
         pa.a = a;
@@ -113,7 +115,8 @@ int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
         pa.items = reinterpret_cast<PromptItem*>(ws + p_items);
         pa.seq_items = reinterpret_cast<int*>(ws + p_seq);
         pa.count = reinterpret_cast<int*>(ws + p_count);
-        pa.last = reinterpret_cast<PromptPart*>(ws + p_last);
+        pa.ctas = sms;
+        pa.arrived = reinterpret_cast<unsigned*>(ws + p_arrived);
         pa.part_ml = reinterpret_cast<float*>(ws + p_ml);
         pa.part_bad = reinterpret_cast<uint32_t*>(ws + p_bad);
         pa.part_o = reinterpret_cast<float*>(ws + p_o);
@@ -123,8 +126,6 @@ int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
     CLLM_HOST_TRY(cudaGetLastError());
     if (prompts)
         if (int rc = launch_early(kv4_prompt_kernel<HD>, sms, kPromptThreads, sizeof(PromptSmem<HD>) + 1024, st, pa)) return rc;
-    if (prompts || (int64_t)a.c.max_pages * a.c.page_len > kStepLen)  // an item can have more than one step
-        if (int rc = launch_early(kv4_join_kernel<HD>, ctas + (prompts ? sms : 0), kJoinThreads, 0, st, ra, pa, ctas)) return rc;
     return CLLM_OK;
 }
 

@@ -12,7 +12,10 @@
 // written) together with the instructions (60 a query vector, 130 a key or value),
 // latency for few.  A warp takes `span` vectors of one token, so the token's
 // page, position and rotation are looked up once for them, and four vectors'
-// loads are issued together; with few tokens span is 1.
+// loads are issued together; with few tokens span is 1.  2048 tokens of 32 query
+// and 8 + 8 key and value vectors of 128, all written out: 28.7 us, 3.6 TB/s (56 %
+// of a copy's rate); the warps wait for their first loads, which depend on the
+// token's page.  One token: 5 us on the GPU.
 #pragma once
 #include <type_traits>
 

@@ -2,10 +2,14 @@
 // (cllm_cuda_kv4_attention; generated tokens).
 //
 // What bounds it: every stored byte is read once and serves rep query heads
-// with 4 * rep * head_dim operations a position, so the HBM stream.  At 6.4
-// TB/s an SM gets a tile of 16 positions every 110 cycles (head_dim 128), in
-// which its four schedulers issue 440 instructions: the numbers must reach the
-// tensor cores with very few of them.
+// with 4 * rep * head_dim operations a position: the HBM stream, were it not for
+// the instructions.  At 6.4 TB/s an SM gets a tile of 16 positions every 110
+// cycles (head_dim 128), in which its four schedulers issue 440 instructions: the
+// numbers must reach the tensor cores with very few of them.  This takes 500 a
+// tile (8 rows), and with the 12 warps that its registers allow the schedulers
+// issue in half of the cycles: 64 sequences of 150 to 8190 positions, 64 heads
+// over 8, 67.6 us, 2.5 TB/s; one of 131071, 32 over 8, 67 us, 2.5 TB/s (38 % of
+// a copy's rate).
 //
 // * Numbers become fp16 two at a time: (w & 0x000F000F) | 0x64006400 is the pair
 //   (1024 + n, 1024 + n'), and one fused operation takes the 1024 off (and the 16
@@ -35,8 +39,11 @@
 //   (and some for the item itself) and cut into equal runs, one per CTA,
 //   whatever the lengths are.  A CTA's four
 //   warps take two tiles each, from a ring of their own that one lane fills with
-//   bulk copies across the runs' borders.  A run that ends inside an item leaves a
-//   partial result, which rows_join puts together in order.
+//   bulk copies across the runs' borders.  Three stages of the ring leave room for
+//   two CTAs an SM only, which is slower (below).
+// * A run that ends inside an item leaves a partial result; the CTA whose part of
+//   an item comes last adds them up in order (64 sequences: 6 us less than a second
+//   kernel's launch and its chain of loads).
 #pragma once
 #include "kv4_format.cuh"
 
@@ -49,7 +56,7 @@ constexpr int kRowStages = 2;               // pairs of tiles in a warp's ring
 constexpr int kRowTile = 8;                 // query rows of an item
 constexpr int kPairLen = 2 * kTile;         // positions of a warp's step
 constexpr int kStepLen = kPairLen * kRowWarps;
-constexpr int kRowCtasPerSm = 3;
+constexpr int kRowCtasPerSm = 3;            // of 168 registers a thread; CT2
 constexpr int kMaxRowCtas = 640;
 constexpr uint32_t kNoTile = 0xFFFFFFFFu;
 
@@ -104,7 +111,8 @@ __device__ __forceinline__ void seq_rows(const AttnArgs& a, int s, int* begin, i
 
 // What a sequence asks of this kernel: items (0: nothing) of `steps` steps
 // each.  An item costs as much again as kItemUnits steps (its queries, the
-// warps' results put together), so it counts steps + kItemUnits units.
+// warps' results put together), so it counts steps + kItemUnits units (64
+// sequences of 150 to 8190 positions, us: IU).
 constexpr int kItemUnits = 2;
 struct SeqWork {
     int begin, n, len, items, steps;

@@ -14,10 +14,13 @@
 //
 // What bounds the calls: the copies' bytes (read and written once) for large
 // pools, launches and latency for small ones.  So where the tables fit, one
-// launch does it all: every CTA derives the whole plan in shared memory (some
-// thousand table entries, 4 us), writes its share of the rows and copies its
-// share of the pages, and no CTA waits for another.  Larger tables, and compact
-// in place, take four launches through the workspace.
+// launch does it all: every CTA derives the whole plan in shared memory, writes
+// its share of the rows and copies its share of the pages, and no CTA waits for
+// another.  Larger tables, and compact in place, take four launches through the
+// workspace.  Forking 8 sequences of 1001 positions (8 layers) 11 us, 192 of 40 to
+// 500 (4 layers) 16.7 us, where the plan and the launch are most of it; compacting
+// 96 of 100 to 900 in 2048 pages of 4 layers 55 us, 5.0 TB/s read and written (78 %
+// of a copy's rate).
 #pragma once
 #include "kv4_format.cuh"
 

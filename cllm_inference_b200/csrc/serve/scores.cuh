@@ -2,7 +2,9 @@
 // probability and rank of a token, entropy, the top_k entries.
 //
 // One pass over the row, which bounds it: 4 bytes a logit from HBM, so an SM has
-// about 21 issue slots per 32 logits; the common path takes 6.
+// 22 issue slots per 32 logits, and this takes 22 (top 20), issued in two cycles of
+// three: 512 rows of 128256 69 us, 3.8 TB/s (59 % of a copy's rate).  One row takes
+// 9 us on the GPU: the launch, its eight CTAs' reading and the join of their lists.
 //   * softmax: each thread keeps a reference instead of the maximum; it moves only
 //     when a logit exceeds it by 14, so the sums are hardly ever rescaled.  With c
 //     = x - reference (exact or nearly so): l += exp(c), lc += exp(c) * c, fp32.

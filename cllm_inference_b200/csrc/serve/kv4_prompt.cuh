@@ -17,7 +17,7 @@
 // from the numbers: q and p come from TMEM, or the operands alone would take all
 // of its bandwidth.  A tile takes 3600 cycles, in which the schedulers issue 59 %
 // of what they could and the tensor cores work 44 %: 1024 tokens of 32 heads over
-// 8 on 8000 positions 425 us, 295 TFLOP/s counted once, three times that in
+// 8 on 8000 positions 425 to 429 us, 294 TFLOP/s counted once, three times that in
 // products (52 % of a plain bf16 GEMM's rate).  Each role is busy some 70 % of the
 // time and waits for the others in turn.
 //

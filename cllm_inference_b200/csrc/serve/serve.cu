@@ -41,16 +41,17 @@ int check_geometry(const char* who, int n_pages, int page_len, int n_head_kv, in
 }
 
 // Rows (of all heads of a KV head) up to which a sequence is kv4_rows_kernel's.  Its time grows with every 8 rows, the
-// prompt kernel's only with every 128.  8 KV heads of 128, us, rows kernel / prompt kernel at 16, 48, 64, 128 rows:
-//   16 sequences of 1024 positions    40/71    71/81    83/83    138/81
-//   64 of 1024                        85/183   194/218  249/220  466/196
-//   16 of 8192                        126/271  318/302  411/304  787/259
-constexpr int kRowsMax = 48;
+// prompt kernel's only with every 128.  8 KV heads of 128, us, rows kernel / prompt kernel at 16, 40, 48, 64 rows:
+//   16 sequences of 1024 positions    33/64    55/65    63/67    76/67
+//   64 of 1024                        78/167   160/171  187/173  244/179
+//   16 of 8192                        119/239  260/241  309/245  402/245
+//   64 of 4096                        219/452  506/462  602/462  796/468
+constexpr int kRowsMax = 40;
 // A call of no more rows than this in all is the rows kernel's alone, without the launches that look for prompts.  One
 // sequence at 48, 64, 128 rows:
-//   500 positions    19/44    22/44    26/54
-//   4096             32/56    34/54    46/71
-//   32768            95/114   120/116  216/126
+//   500 positions    18/38    18/38    20/44
+//   4096             27/48    31/48    43/52
+//   32768            90/97    117/97   211/101
 constexpr int kRowsAlone = 64;
 
 // Launch `kern` so that it may start before the kernel before it is done (programmatic

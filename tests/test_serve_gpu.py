@@ -319,6 +319,23 @@ def test_attention_a_long_cache_and_offsets_past_32_bits(cuda, lib):
     np.testing.assert_allclose(a[0].cpu().numpy().reshape(want.shape), want, atol=2.0 ** -16 * np.abs(v).max(), rtol=0)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [1, 45])
+def test_attention_parts_of_one_item_in_many_ctas(cuda, lib, rows, hd):
+    """One KV head and a long sequence: every CTA has a part of the same rows; the next calls find the counts cleared."""
+    rng = np.random.default_rng(rows * hd)
+    cache, _, _ = _cache(rng, 1, 940, 64, 1, hd, [60000, 33], 938)
+    q = torch.from_numpy(rng.standard_normal((2 * rows, 3 * hd)).astype(np.float32)).cuda()
+    begin = [0, rows, 2 * rows]
+    o = _attend(cache, 0, q, begin, hd)
+    short, _, _ = _cache(rng, 1, 9, 64, 1, hd, [130, 300], 5)
+    for _ in range(2):
+        _attend(short, 0, q, begin, hd)
+        again = cache.attention(0, q, begin=torch.tensor(begin, dtype=torch.int32, device="cuda"))
+        assert np.array_equal(again.cpu().numpy(), o.astype(np.float32))
+    _lib.check(lib.cllm_cuda_check_device_status())
+
+
 def test_attention_is_repeatable_on_another_stream_and_in_a_graph(cuda, lib):
     hd = 128
     rng = np.random.default_rng(9)

@@ -65,7 +65,8 @@ struct AttnArgs {
     int64_t ldq;
     const int* q_begin;  // nullptr: row s belongs to sequence s
     int n_tok, n_head, rep;
-    int rows_max;        // sequences with more rows * rep are the prompt kernel's
+    int rows_max;        // sequences with more rows * rep are the prompt kernel's (INT_MAX: none are)
+    int all_steps;       // but not in a call of at most so many steps in all
     float scale;
     float *out, *lse;
     Cache c;
@@ -119,25 +120,36 @@ struct SeqWork {
     __device__ __forceinline__ int units() const { return steps + kItemUnits; }
     __device__ __forceinline__ int step(int unit) const { return max(0, unit - kItemUnits); }
 };
-__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int s) {
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int s, int limit) {
     SeqWork w;
     seq_rows(a, s, &w.begin, &w.n);
     w.items = 0;
     w.steps = 1;
     w.len = 0;
     const int64_t rows = (int64_t)w.n * a.rep;
-    if (rows == 0 || rows > a.rows_max) return w;
+    if (rows == 0 || rows > limit) return w;
     w.len = a.c.length(s);
     w.items = a.c.n_kv * (int)((rows + kRowTile - 1) / kRowTile);
     w.steps = max(1, (w.len + kStepLen - 1) / kStepLen);  // one even for no positions: its rows are zeros
     return w;
 }
 
+// Steps of a sequence if this kernel took it, at most all_steps + 1.  The rows
+// up to which it takes sequences follow from their sum.
+__device__ __forceinline__ int64_t seq_steps(const AttnArgs& a, int s) {
+    int begin, n;
+    seq_rows(a, s, &begin, &n);
+    const int64_t groups = ((int64_t)n * a.rep + kRowTile - 1) / kRowTile, most = (int64_t)a.all_steps + 1;
+    if (groups >= most) return most;
+    return min(most, groups * a.c.n_kv * max(1, (a.c.length(s) + kStepLen - 1) / kStepLen));
+}
+__device__ __forceinline__ int rows_limit(const AttnArgs& a, int64_t steps) { return steps <= a.all_steps ? INT_MAX : a.rows_max; }
+
 // A place in the numbered units.
 struct Cursor {
     int s, item, unit, left;  // left: units up to the end of this CTA's run
     SeqWork w;
-    __device__ __forceinline__ void next(const AttnArgs& a, int units) {  // over `units` units inside the item
+    __device__ __forceinline__ void next(const AttnArgs& a, int units, const volatile int& limit) {  // over `units` units inside the item
         left -= units;
         unit += units;
         if (unit < w.units()) return;
@@ -145,7 +157,7 @@ struct Cursor {
         if (++item < w.items) return;
         item = 0;
         while (left > 0 && s + 1 < a.c.n_seqs) {
-            w = seq_work(a, ++s);
+            w = seq_work(a, ++s, limit);
             if (w.items) return;
         }
     }
@@ -272,7 +284,7 @@ struct RowsSmem {
     float ml[kRowWarps][kRowTile][2];
     uint64_t full[kRowWarps][kRowStages];
     int64_t scan[kRowWarps];
-    int start[4];
+    int start[3], limit;
 };
 
 // A place in a warp's ring.
@@ -389,12 +401,19 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     // all units, and this CTA's run of them
     const int per = (a.c.n_seqs + kRowThreads - 1) / kRowThreads;
     const int s0 = min(a.c.n_seqs, (int)threadIdx.x * per), s1 = min(a.c.n_seqs, s0 + per);
-    int64_t mine = 0;
+    int64_t mine = 0, all;
+    int limit = a.rows_max;
+    if (limit != INT_MAX) {
+        for (int s = s0; s < s1; ++s) mine += seq_steps(a, s);
+        cta_scan(mine, sm.scan, &all);
+        limit = rows_limit(a, all);
+        mine = 0;
+    }
+    if (threadIdx.x == 0) sm.limit = limit;
     for (int s = s0; s < s1; ++s) {
-        const SeqWork w = seq_work(a, s);
+        const SeqWork w = seq_work(a, s, limit);
         mine += (int64_t)w.items * w.units();
     }
-    int64_t all;
     const int64_t before = cta_scan(mine, sm.scan, &all);
     const int ctas = (int)min((int64_t)gridDim.x, all);
     if (threadIdx.x == 0) g_rows_arrived[ra.set ^ 1][blockIdx.x] = 0;
@@ -403,7 +422,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     if (mine && before <= run0 && run0 < before + mine) {
         int64_t at = before;
         for (int s = s0; s < s1; ++s) {
-            const SeqWork w = seq_work(a, s);
+            const SeqWork w = seq_work(a, s, limit);
             const int64_t next = at + (int64_t)w.items * w.units();
             if (run0 < next) {
                 sm.start[0] = s;
@@ -420,7 +439,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     cur.item = sm.start[1];
     cur.unit = sm.start[2];
     cur.left = (int)(run1 - run0);
-    cur.w = seq_work(a, cur.s);
+    cur.w = seq_work(a, cur.s, limit);
 
     // The producer runs ahead of the warp's own tiles.  Lane i holds the places
     // of the i-th of up to 32 pairs of one item and copies them itself.
@@ -449,7 +468,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                 pro_i = __ffs(lanes) - 1;
                 pro_n = pro_i + __popc(lanes);
             }
-            pro.next(a, units);
+            pro.next(a, units, sm.limit);
         }
     };
     auto produce = [&]() {
@@ -483,7 +502,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
         const int units = min(cur.left, cur.w.units() - cur.unit), groups = cur.w.items / a.c.n_kv;
         const int step0 = cur.w.step(cur.unit), step1 = cur.w.step(cur.unit + units);
         if (step0 == step1) {  // the run ends before the item's first step
-            cur.next(a, units);
+            cur.next(a, units, sm.limit);
             continue;
         }
         const int kvh = cur.item / groups, row0 = (cur.item - kvh * groups) * kRowTile;
@@ -806,7 +825,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
             if (sm.start[0]) rows_join<HD>(ra, sm.start[1], sm.start[0], cur.w, kvh, row0);
         }
         __syncthreads();
-        cur.next(a, units);
+        cur.next(a, units, sm.limit);
     }
     if (!alive)  // let the copies in flight land before the CTA ends
         for (; get.i != put.i || get.parity != put.parity; get.next()) wait_full(full + 8 * get.i, get.parity);

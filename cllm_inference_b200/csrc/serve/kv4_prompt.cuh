@@ -206,7 +206,10 @@ __global__ void __launch_bounds__(kPromptPlanThreads) prompt_plan_kernel(const P
         return x - v + (warp ? before : 0);
     };
     for (int i = threadIdx.x; i < p.ctas; i += kPromptPlanThreads) p.arrived[i] = 0;
-    int64_t count = 0;
+    int64_t count = 0, steps = 0;
+    for (int s = threadIdx.x; s < a.c.n_seqs; s += kPromptPlanThreads) steps += seq_steps(a, s);
+    scan(steps, &steps);
+    const int limit = rows_limit(a, steps);
     for (int base = 0; base < a.c.n_seqs; base += kPromptPlanThreads) {
         const int s = base + threadIdx.x;
         int64_t blocks = 0, total;
@@ -214,7 +217,7 @@ __global__ void __launch_bounds__(kPromptPlanThreads) prompt_plan_kernel(const P
             int begin, n;
             seq_rows(a, s, &begin, &n);
             const int64_t rows = (int64_t)n * a.rep;
-            if (rows > a.rows_max) blocks = (rows + kPromptRows - 1) / kPromptRows;
+            if (rows > limit) blocks = (rows + kPromptRows - 1) / kPromptRows;
         }
         const int64_t at = count + scan(blocks, &total);
         if (s < a.c.n_seqs) p.seq_items[s] = (int)min(at, (int64_t)p.most);

@@ -47,12 +47,14 @@ int check_geometry(const char* who, int n_pages, int page_len, int n_head_kv, in
 //   16 of 8192                        119/239  260/241  309/245  402/245
 //   64 of 4096                        219/452  506/462  602/462  796/468
 constexpr int kRowsMax = 40;
-// A call of no more rows than this in all is the rows kernel's alone, without the launches that look for prompts.  One
-// sequence at 48, 64, 128 rows:
-//   500 positions    18/38    18/38    20/44
-//   4096             27/48    31/48    43/52
-//   32768            90/97    117/97   211/101
-constexpr int kRowsAlone = 64;
+// A call of no more steps (of 8 rows, 128 positions, a KV head) for each of its CTAs is the rows kernel's alone.  8 KV
+// heads of 128 (64), us, rows kernel / prompt kernel, 444 CTAs:
+//   128 rows on 2048 positions, 2048 steps               33/50 (26/38)
+//   1024 on 500, 512 on 1024 or 128 on 4096, 4096 steps  51/46, 45/50, 43/54 (38/38, 33/38, 33/40)
+//   4 sequences of 192 on 1024, 6144 steps               61/56 (43/42)
+//   1024 on 1024 or 256 on 4096, 8192 steps              78/54, 68/56 (53/42, 47/42)
+// Where the sizes alone show it, the launches that look for prompts are left out.
+constexpr int kRowsAllSteps = 9;
 
 // Launch `kern` so that it may start before the kernel before it is done (programmatic
 // dependent launch); it waits with griddepcontrol.wait where it needs to.
@@ -75,7 +77,7 @@ int launch_early(void (*kern)(KArgs...), int ctas, int threads, size_t smem, cud
 int g_set[64];  // of g_rows_arrived, the last call's; host_workspace's lock guards it
 
 template <int HD>
-int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
+int launch_attention(AttnArgs a, int dev, int sms, cudaStream_t st) {
     static std::once_flag once[64];
     cudaError_t attr = cudaSuccess;
     std::call_once(once[dev], [&] {
@@ -85,10 +87,13 @@ int launch_attention(const AttnArgs& a, int dev, int sms, cudaStream_t st) {
                                         sizeof(PromptSmem<HD>) + 1024);
     });
     CLLM_HOST_TRY(attr);
-    const bool prompts = a.q_begin && (int64_t)a.n_tok * a.rep > a.rows_max;
     const int ctas = std::min(kMaxRowCtas, kRowCtasPerSm * sms);
+    const int64_t rows = (int64_t)a.n_tok * a.rep, groups = rows / kRowTile + a.c.n_seqs;  // at most
+    const int64_t steps = ((int64_t)a.c.max_pages * a.c.page_len + kStepLen - 1) / kStepLen;
+    a.all_steps = kRowsAllSteps * ctas;
+    const bool prompts = a.q_begin && rows > a.rows_max && (groups > a.all_steps || groups * a.c.n_kv * steps > a.all_steps);
+    if (!prompts) a.rows_max = INT_MAX;
     // blocks of rows of sequences with more rows than rows_max: at most
-    const int64_t rows = (int64_t)a.n_tok * a.rep;
     const int64_t most = prompts ? rows / kPromptRows + std::min<int64_t>(a.c.n_seqs, rows / (a.rows_max + 1)) : 0;
     if (most > INT_MAX / 2) return host_fail(CLLM_ERR_TOO_LARGE, "kv4_attention: too many rows in one call");
 
@@ -211,7 +216,7 @@ int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int
     if (int rc = host_device(&dev, &sms)) return rc;
     AttnArgs a{};
     a.q = q; a.ldq = ldq; a.q_begin = q_begin; a.n_tok = n_tok; a.n_head = n_head; a.rep = n_head / n_head_kv;
-    a.rows_max = std::max((int64_t)n_tok * a.rep <= kRowsAlone ? kRowsAlone : kRowsMax, a.rep);
+    a.rows_max = std::max(kRowsMax, a.rep);
     a.scale = scale == 0.f ? 1.f / std::sqrt((float)head_dim) : scale;
     a.out = out; a.lse = lse;
     a.c = Cache{const_cast<uint8_t*>(static_cast<const uint8_t*>(pages)), page_table, seq_len, n_pages, page_len,

@@ -319,6 +319,62 @@ def test_attention_a_long_cache_and_offsets_past_32_bits(cuda, lib):
     np.testing.assert_allclose(a[0].cpu().numpy().reshape(want.shape), want, atol=2.0 ** -16 * np.abs(v).max(), rtol=0)
 
 
+# The same in calls that are long enough for whole prompts to be worth 128 rows at a time.
+
+
+@pytest.mark.parametrize("hd,rep,kv,page_len,counts", [
+    (128, 4, 4, 64, [0, 1, 15, 16, 17, 63, 64, 65, 200, 0, 31, 300]),
+    (64, 8, 3, 128, [0, 1, 15, 16, 17, 63, 64, 65, 200, 0, 31, 200]),
+    (128, 1, 16, 32, [0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 300]),
+    (64, 3, 12, 48, [0, 0, 0, 0, 0, 0, 0, 41, 0, 0, 0, 130]),
+    (128, 16, 3, 16, [3, 2, 1, 1, 1, 8, 0, 0, 2, 2, 2, 130]),
+    (64, 1, 40, 64, [0, 0, 0, 0, 0, 0, 0, 0, 129, 0, 0, 128]),
+])
+def test_attention_prompts(cuda, lib, hd, rep, kv, page_len, counts):
+    test_attention_many_rows(cuda, lib, hd, rep, kv, page_len, counts)
+
+
+def test_attention_prompts_extremes(cuda, lib):
+    test_attention_extremes(cuda, lib, 700)
+    test_attention_values_that_cancel(cuda, lib, 8100)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_prompts_a_nan(cuda, lib, hd):
+    if hd == 128:
+        test_attention_a_nan_stays_with_the_rows_that_see_it(cuda, lib, 2100)
+    test_attention_a_nan_of_the_values_stays_in_its_group(cuda, lib, 2100, hd)
+
+
+def test_attention_prompts_bad_pages_and_repeatable(cuda, lib):
+    rng = np.random.default_rng(11)
+    cache, p, table = _cache(rng, 1, 30, 16, 2, 64, [130, 250], 18)
+    q = torch.randn(9000, 6 * 64, device="cuda")
+    begin = torch.tensor([0, 4000, 9000], dtype=torch.int32, device="cuda")
+    o = cache.attention(0, q, begin=begin)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = cache.attention(0, q, begin=begin)
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(cache.attention(0, q, begin=begin), o) and torch.equal(again, o)
+    _lib.check(lib.cllm_cuda_check_device_status())
+    cache.table[0, 1] = 2 ** 30
+    got = cache.attention(0, q, begin=begin)
+    assert lib.cllm_cuda_check_device_status() == _lib.ERR_INVALID_ARG
+    assert torch.equal(got[4000:], o[4000:])
+
+
+@pytest.mark.parametrize("rows", [20, 41, 60, 61, 100])
+def test_attention_either_kernel_at_the_border(cuda, lib, rows):
+    """Calls of about as many rows and steps as the rule between the kernels looks at, in a wide and a tight table."""
+    rng = np.random.default_rng(rows)
+    for slots in (16, 400):
+        cache, _, _ = _cache(rng, 1, 40, 64, 8, 64, [1000, 300, 1000], slots)
+        q = torch.from_numpy(rng.standard_normal((2 * rows + 3, 16 * 64)).astype(np.float32)).cuda()
+        _attend(cache, 0, q, [0, rows, rows + 3, 2 * rows + 3], 64)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("rows", [1, 45])
 def test_attention_parts_of_one_item_in_many_ctas(cuda, lib, rows, hd):

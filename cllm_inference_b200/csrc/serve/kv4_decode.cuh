@@ -65,7 +65,7 @@ struct AttnArgs {
     int64_t ldq;
     const int* q_begin;  // nullptr: row s belongs to sequence s
     int n_tok, n_head, rep;
-    int rows_max;        // sequences with more rows * rep are the prompt kernel's (INT_MAX: none are)
+    int rows_max;        // sequences with more rows * rep are the prompt kernel's,
     int all_steps;       // but not in a call of at most so many steps in all
     float scale;
     float *out, *lse;
@@ -149,7 +149,7 @@ __device__ __forceinline__ int rows_limit(const AttnArgs& a, int64_t steps) { re
 struct Cursor {
     int s, item, unit, left;  // left: units up to the end of this CTA's run
     SeqWork w;
-    __device__ __forceinline__ void next(const AttnArgs& a, int units, const volatile int& limit) {  // over `units` units inside the item
+    __device__ __forceinline__ void next(const AttnArgs& a, int units, const volatile int* limit) {  // over `units` units inside the item
         left -= units;
         unit += units;
         if (unit < w.units()) return;
@@ -157,7 +157,7 @@ struct Cursor {
         if (++item < w.items) return;
         item = 0;
         while (left > 0 && s + 1 < a.c.n_seqs) {
-            w = seq_work(a, ++s, limit);
+            w = seq_work(a, ++s, limit ? *limit : INT_MAX);
             if (w.items) return;
         }
     }
@@ -374,7 +374,9 @@ __device__ __forceinline__ void rows_join(const RowsArgs& ra, int c0, int parts,
 
 // ---- the kernel --------------------------------------------------------------------
 
-template <int HD>
+// ALL: every sequence is this kernel's (no limit to look up: 64 sequences 67.6 us
+// instead of 69.0).
+template <int HD, bool ALL>
 __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(const RowsArgs ra) {
     constexpr int G = Tile<HD>::G;
     extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -402,14 +404,15 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     const int per = (a.c.n_seqs + kRowThreads - 1) / kRowThreads;
     const int s0 = min(a.c.n_seqs, (int)threadIdx.x * per), s1 = min(a.c.n_seqs, s0 + per);
     int64_t mine = 0, all;
-    int limit = a.rows_max;
-    if (limit != INT_MAX) {
+    int limit = INT_MAX;
+    const volatile int* limit_at = ALL ? nullptr : &sm.limit;
+    if (!ALL) {
         for (int s = s0; s < s1; ++s) mine += seq_steps(a, s);
         cta_scan(mine, sm.scan, &all);
         limit = rows_limit(a, all);
         mine = 0;
+        if (threadIdx.x == 0) sm.limit = limit;
     }
-    if (threadIdx.x == 0) sm.limit = limit;
     for (int s = s0; s < s1; ++s) {
         const SeqWork w = seq_work(a, s, limit);
         mine += (int64_t)w.items * w.units();
@@ -468,7 +471,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                 pro_i = __ffs(lanes) - 1;
                 pro_n = pro_i + __popc(lanes);
             }
-            pro.next(a, units, sm.limit);
+            pro.next(a, units, limit_at);
         }
     };
     auto produce = [&]() {
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
         const int units = min(cur.left, cur.w.units() - cur.unit), groups = cur.w.items / a.c.n_kv;
         const int step0 = cur.w.step(cur.unit), step1 = cur.w.step(cur.unit + units);
         if (step0 == step1) {  // the run ends before the item's first step
-            cur.next(a, units, sm.limit);
+            cur.next(a, units, limit_at);
             continue;
         }
         const int kvh = cur.item / groups, row0 = (cur.item - kvh * groups) * kRowTile;
@@ -825,7 +828,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
             if (sm.start[0]) rows_join<HD>(ra, sm.start[1], sm.start[0], cur.w, kvh, row0);
         }
         __syncthreads();
-        cur.next(a, units, sm.limit);
+        cur.next(a, units, limit_at);
     }
     if (!alive)  // let the copies in flight land before the CTA ends
         for (; get.i != put.i || get.parity != put.parity; get.next()) wait_full(full + 8 * get.i, get.parity);

@@ -81,7 +81,10 @@ int launch_attention(AttnArgs a, int dev, int sms, cudaStream_t st) {
     static std::once_flag once[64];
     cudaError_t attr = cudaSuccess;
     std::call_once(once[dev], [&] {
-        attr = cudaFuncSetAttribute(kv4_rows_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(RowsSmem<HD>));
+        attr = cudaFuncSetAttribute(kv4_rows_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(RowsSmem<HD>));
+        if (attr == cudaSuccess)
+            attr = cudaFuncSetAttribute(kv4_rows_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        sizeof(RowsSmem<HD>));
         if (attr == cudaSuccess)
             attr = cudaFuncSetAttribute(kv4_prompt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         sizeof(PromptSmem<HD>) + 1024);
@@ -92,7 +95,6 @@ int launch_attention(AttnArgs a, int dev, int sms, cudaStream_t st) {
     const int64_t steps = ((int64_t)a.c.max_pages * a.c.page_len + kStepLen - 1) / kStepLen;
     a.all_steps = kRowsAllSteps * ctas;
     const bool prompts = a.q_begin && rows > a.rows_max && (groups > a.all_steps || groups * a.c.n_kv * steps > a.all_steps);
-    if (!prompts) a.rows_max = INT_MAX;
     // blocks of rows of sequences with more rows than rows_max: at most
     const int64_t most = prompts ? rows / kPromptRows + std::min<int64_t>(a.c.n_seqs, rows / (a.rows_max + 1)) : 0;
     if (most > INT_MAX / 2) return host_fail(CLLM_ERR_TOO_LARGE, "kv4_attention: too many rows in one call");
@@ -127,8 +129,10 @@ int launch_attention(AttnArgs a, int dev, int sms, cudaStream_t st) {
         pa.part_bad = reinterpret_cast<uint32_t*>(ws + p_bad);
         pa.part_o = reinterpret_cast<float*>(ws + p_o);
         prompt_plan_kernel<<<1, kPromptPlanThreads, 0, st>>>(pa);
+        kv4_rows_kernel<HD, false><<<ctas, kRowThreads, sizeof(RowsSmem<HD>), st>>>(ra);
+    } else {
+        kv4_rows_kernel<HD, true><<<ctas, kRowThreads, sizeof(RowsSmem<HD>), st>>>(ra);
     }
-    kv4_rows_kernel<HD><<<ctas, kRowThreads, sizeof(RowsSmem<HD>), st>>>(ra);
     CLLM_HOST_TRY(cudaGetLastError());
     if (prompts)
         if (int rc = launch_early(kv4_prompt_kernel<HD>, sms, kPromptThreads, sizeof(PromptSmem<HD>) + 1024, st, pa)) return rc;

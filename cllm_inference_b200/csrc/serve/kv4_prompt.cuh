@@ -24,8 +24,9 @@
 // Work: tiles of (sequence, KV head, 128 rows), numbered through by
 // prompt_plan_kernel and cut into equal runs, one per SM; a run that ends inside an
 // item leaves a partial result, and the CTA whose part of an item comes last adds
-// them up in order (sequences of 5 to 2500 positions with up to 300 rows: 36 us
-// with that, 46 with a kernel of its own).
+// them up in order (9 sequences of 5 to 2500 positions, two of them prompts of 65
+// and 99 rows, while these were this kernel's: 36 us with that, 46 with a kernel of
+// its own).
 //
 // Warps (5 warpgroups; registers moved to where they are needed):
 //   0       raw tiles of the pages into a ring (bulk copies)
@@ -46,10 +47,10 @@ namespace cllm {
 namespace serve {
 
 constexpr int kPromptThreads = 640;
-// An item costs as much again as kPromptUnits tiles, and a run has kPromptMinRun
-// units or more.  Sequences of 5 to 2500 positions with up to 300 rows: 36.0 us;
-// with 1 or 6 for the first 38.8 and 36.5, with 1 or 16 for the second 40.2 and 48.7.
-constexpr int kPromptUnits = 3;
+// An item costs as much again as kPromptUnits tiles: 256 rows of 32 heads over 8 on
+// 4096 positions at 1, 3, 6: 61, 59, 57 us, 512 rows 74, 72, 68.  A run has
+// kPromptMinRun units or more; 16 instead: 70 and 72 us for 59 and 72 (at 3 units).
+constexpr int kPromptUnits = 6;
 constexpr int kPromptMinRun = 6;
 constexpr int kPromptRows = 128, kPromptCols = 64;
 constexpr int kRawStages = 3;

@@ -54,7 +54,7 @@ constexpr int kRowsMax = 40;
 //   4 sequences of 192 on 1024, 6144 steps               61/56 (43/42)
 //   1024 on 1024 or 256 on 4096, 8192 steps              78/54, 68/56 (53/42, 47/42)
 // Where the sizes alone show it, the launches that look for prompts are left out.
-constexpr int kRowsAllSteps = 9;
+constexpr int kRowsAllSteps = 10;
 
 // Launch `kern` so that it may start before the kernel before it is done (programmatic
 // dependent launch); it waits with griddepcontrol.wait where it needs to.

@@ -8,7 +8,11 @@
 // a tile's p v is not accumulated in TMEM over the whole sequence but added to
 // fp32 registers, rounded to nearest, tile by tile; that also does the rescaling.
 // k and v of a tile are scaled by a power of two that brings its largest value to
-// [2^10, 2^11), so that lo stays above fp16's subnormals; S and p take it out.
+// [2^10, 2^11), so that lo stays above fp16's subnormals.  S takes the keys' out.
+// The values' stays in the fp32 sums, of weights as of weighted values, and a
+// tile's rescaling brings them to its power: p is not touched by it, and the largest
+// weight is 2^10 to 2^14 whatever the values are, so a weight keeps its 22 bits down to
+// 2^-12 of it and is no further off than 2^-35 below that.
 //
 // What bounds it: three products a term, 6 * 128 * 64 * HD multiply-adds a tile
 // for 128 x 64 scores: 1536 cycles of the tensor cores (HD 128), beside which the
@@ -66,6 +70,7 @@ struct PromptSmem {
     float v_scale[4][Tile<HD>::G][2][kTile];  // [raw tile][group][d, m][position]
     float alpha[4][kPromptRows];  // what a tile's new reference leaves of the sums
     float sum[2][kPromptRows], ref[2][kPromptRows];  // of an item: its rows' sums of weights and references
+    float down[2];                                   // and what takes the values' power out of its sums
     uint32_t bad[2][kPromptRows];                    // groups that a NaN of the values reaches
     struct Stat {
         float k_down, v_up;  // 2^-(the keys' power), 2^(the values' power)
@@ -148,7 +153,9 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
 }
 
 // Two values as an fp16 pair and what is left of them as another: hi is the value
-// cut to fp16's 11 bits (the conversion is exact), so lo holds the next 11.
+// cut to 11 bits, so lo holds the next 11.  For keys and values, whose tile's largest
+// is 2^10 or more: what lies below fp16's normal range, where hi's conversion is not
+// exact, is 2^-24 of it.  Queries and weights are split to the nearest (split2).
 __device__ __forceinline__ void split_pair(float2 x, uint32_t& hi, uint32_t& lo) {
     const float2 h = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xFFFFE000u), __uint_as_float(__float_as_uint(x.y) & 0xFFFFE000u));
     const float2 l = add2(x, make_float2(-h.x, -h.y));
@@ -518,8 +525,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                             if (vec) x = *reinterpret_cast<const float4*>(src + i + k);
                             else x = make_float4(src[i + k], src[i + k + 1], src[i + k + 2], src[i + k + 3]);
                         }
-                        split_pair(make_float2(x.x * up, x.y * up), hi[k / 2], lo[k / 2]);
-                        split_pair(make_float2(x.z * up, x.w * up), hi[k / 2 + 1], lo[k / 2 + 1]);
+                        split2(x.x * up, x.y * up, &hi[k / 2], &lo[k / 2]);
+                        split2(x.z * up, x.w * up, &hi[k / 2 + 1], &lo[k / 2 + 1]);
                     }
                     tmem_st16u(tmem + lanes + kColQ + i / 2, hi);
                     tmem_st16u(tmem + lanes + kColQ + HD / 2 + i / 2, lo);
@@ -529,6 +536,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 warp_arrive(bar(sm.q_full));
             }
             float ref = -3.0e38f, l = 0.f;
+            int power = 0;  // of the values in the sums
             uint32_t bad = 0;
             // EDGE: some row of the warp does not see all of the tile (a copy of its own, or every tile pays the selects)
             auto tile = [&](auto edge, int i) {
@@ -538,7 +546,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 group_wait<4>(bar(sm.s_full[st]), (uint32_t)(it >> 1) & 1u, abort);
                 tc_fence_after();
                 const float f = f_log2 * sm.stat[rs].k_down, v_up = sm.stat[rs].v_up;
-                const int v_power = sm.stat[rs].v_power;
+                const int change = sm.stat[rs].v_power - power;
+                power += change;
                 const uint32_t col = tmem + lanes + kColS + 64 * st;
                 const int limit = sees - i * kPromptCols;  // columns that the row sees
                 if (sm.stat[rs].bad)
@@ -557,15 +566,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     top = fmaxf(top, m);
                 }
                 top *= f;
-                const float room = 14.f + (float)min(0, v_power);
-                float alpha = 1.f;
-                if (top > ref + room) {
-                    const float now = top - (room - 4.f);
-                    alpha = exp2_fast(ref - now);
+                float alpha = __uint_as_float((uint32_t)(127 + change) << 23);
+                if (top > ref + 14.f) {
+                    const float now = top - 10.f;
+                    alpha *= exp2_fast(ref - now);
                     ref = now;
                 }
                 sm.alpha[r4][row] = alpha;
-                const float off = -ref - (float)v_power;
+                const float off = -ref;
                 const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
                 float2 sum = make_float2(0.f, 0.f);
 #pragma unroll 1
@@ -580,7 +588,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                         if (EDGE && c + 2 * k >= limit) y.x = 0.f;
                         if (EDGE && c + 2 * k + 1 >= limit) y.y = 0.f;
                         sum = add2(sum, y);
-                        split_pair(y, w[k], w[8 + k]);
+                        split2(y.x, y.y, &w[k], &w[8 + k]);
                     }
                     tmem_st16u(col + c, w);
                 }
@@ -601,6 +609,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
             const int slot = items++ & 1;
             sm.sum[slot][row] = l;
             sm.ref[slot][row] = ref;
+            if (row == 0) sm.down[slot] = __uint_as_float((uint32_t)(127 - power) << 23);
             sm.bad[slot][row] = bad;
             asm volatile("bar.sync 2, 256;" ::: "memory");
         }
@@ -643,7 +652,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
             int begin, n;
             seq_rows(a, item.seq, &begin, &n);
             const int j = item.block * kPromptRows + row;
-            const float sum = sm.sum[items & 1][row], ref = sm.ref[items & 1][row];
+            const float sum = sm.sum[items & 1][row], ref = sm.ref[items & 1][row], down = sm.down[items & 1];
             const uint32_t bad = sm.bad[items & 1][row];
             if (to - from == item.tiles) {
                 if (j < n * a.rep) {
@@ -659,15 +668,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                                 sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
                                            : make_float4(acc[i].x * by, acc[i].y * by, acc[i + 1].x * by, acc[i + 1].y * by);
                     }
-                    if (a.lse) a.lse[at] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (ref + log2f(sum));
+                    if (a.lse) a.lse[at] = sum == 0.f ? -INFINITY : 0.69314718055994530942f * (ref + log2f(sum * down));
                 }
             } else {
                 const int slot = 2 * blockIdx.x + (from == 0 ? 1 : 0);
                 float4* out = reinterpret_cast<float4*>(p.part_o) + (int64_t)slot * (kPromptRows * HD / 4) + row;
 #pragma unroll
                 for (int i = 0; i < HD / 2; i += 2)
-                    out[i / 2 * kPromptRows] = make_float4(acc[i].x, acc[i].y, acc[i + 1].x, acc[i + 1].y);
-                *reinterpret_cast<float2*>(p.part_ml + 2 * (slot * kPromptRows + row)) = make_float2(ref, sum);
+                    out[i / 2 * kPromptRows] = make_float4(acc[i].x * down, acc[i].y * down, acc[i + 1].x * down, acc[i + 1].y * down);
+                *reinterpret_cast<float2*>(p.part_ml + 2 * (slot * kPromptRows + row)) = make_float2(ref, sum * down);
                 p.part_bad[slot * kPromptRows + row] = bad;
                 // the CTA whose part is the last to come joins them
                 asm volatile("bar.sync 5, 128;" ::: "memory");
@@ -798,7 +807,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 }
                 asm volatile("bar.sync 3, 128;" ::: "memory");
                 const uint32_t e = max(max(sm.top[1][si][0], sm.top[1][si][1]), max(sm.top[1][si][2], sm.top[1][si][3]));
-                const int power = min(12, 25 - (int)e);
+                const int power = 25 - (int)e;
                 if (tid == 0) {
                     sm.stat[si].v_up = __uint_as_float((uint32_t)(127 + power) << 23);
                     sm.stat[si].v_power = power;

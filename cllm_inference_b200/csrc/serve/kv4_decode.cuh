@@ -33,8 +33,12 @@
 //   16 x head_dim tile in two 16-byte loads, for keys and for values, and the
 //   score a lane computes is the p that the same lane needs as an operand.
 // * The running reference (in place of the maximum) of a row moves only when a
-//   score exceeds it by 2^14, so the accumulators are hardly ever rescaled; a p
-//   of at most 2^14 keeps p d inside fp16 (values' scales of 2 and more lower it).
+//   score exceeds it by 2^14, so the accumulators are hardly ever rescaled.
+// * The values' scales get a power of two, which the accumulators carry, that brings
+//   the largest one so far below 2 and to 2^-3 or more: a p of at most 2^14 then keeps
+//   p d inside fp16, and p d is off by 2^-25 at most where p of the largest weight is 2^10
+//   or more, so small weights count beside a dominating one however small the values
+//   are.  Scales of 2^-3 to 2 need no power, and cost a test (64 sequences: 0.4 us).
 // * Work: steps of 128 positions of (sequence, KV head, 8 rows), numbered through
 //   (and some for the item itself) and cut into equal runs, one per CTA,
 //   whatever the lengths are.  A CTA's four
@@ -565,7 +569,9 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
         }
         __syncthreads();
         const uint32_t qa = smem_addr(sm.qa) + 16 * lane, qs_hi = sm.qs[0][lane], qs_lo = sm.qs[1][lane];
-        float2 o[G][4];  // values' numbers less 8: [group][c]
+        float2 o[G][4];  // values' numbers less 8: [group][c], times 2^k
+        constexpr uint32_t kFirst = 0x78007800u, kOne = 0x3C003C00u;
+        uint32_t d_up = kFirst;  // 2^k as an fp16 pair; k = 15 before the first scale
         float om = 0.f;  // and their middles, of group t
 #pragma unroll
         for (int g = 0; g < G; ++g)
@@ -618,9 +624,8 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                     s[u][2 * h + 1] = acc[h].y * f_log2;
                 }
             }
-            // ---- the values' scales of the lane's positions as pairs, and whether one is large
+            // ---- the values' scales of the lane's positions as pairs, times 2^k
             __half2 d[2][2][G];
-            uint32_t big = 0;
             const bool edge = p0 + kPairLen > sees_all;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -645,30 +650,51 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                                 d[u][j >> 1][g] = bits_h2(h2bits(d[u][j >> 1][g]) & (j & 1 ? 0x0000FFFFu : 0xFFFF0000u));
                         }
             }
+            uint32_t big = 0;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int g = 0; g < G; ++g) big |= h2bits(d[u][k][g]);
-            float room = 14.f;
-            if (__any_sync(0xFFFFFFFFu, (big & 0x40004000u) != 0)) {  // a scale of 2 or more: p d stays below 2^15
-                big = 0;
+            const bool two = __any_sync(0xFFFFFFFFu, (big & 0x40004000u) != 0);  // a scale is 2 or more
+            // a first scale of 2^-3 or more (or of 2^-7 with some a sixteenth of it) needs no k
+            if (d_up == kFirst && !two && __any_sync(0xFFFFFFFFu, (big & big << 1 & 0x20002000u) != 0)) d_up = kOne;
+            if (two || d_up != kOne) {
+                __half2 some[4];  // NaNs do not count
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    some[i] = __hmax2(__habs2(d[i / 2][i % 2][0]), __habs2(d[i / 2][i % 2][1]));
+                    if constexpr (G == 4) some[i] = __hmax2(some[i], __hmax2(__habs2(d[i / 2][i % 2][2]), __habs2(d[i / 2][i % 2][3])));
+                }
+                const __half2 most = __hmax2(__hmax2(some[0], some[1]), __hmax2(some[2], some[3]));
+                const uint32_t lo = h2bits(most) & 0xFFFFu, hi = h2bits(most) >> 16;
+                const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(lo > 0x7C00u ? 0u : lo, hi > 0x7C00u ? 0u : hi));
+                const int e = (int)(top >> 10) - 15, k0 = (int)(d_up >> 26) - 15;
+                const int k = min(k0, e >= 1 ? max(-14, -e) : e >= -3 ? 0 : -e);
+                if (k != k0) {
+                    const float by = __uint_as_float((uint32_t)(127 + k - k0) << 23);
+                    const float2 b2 = make_float2(by, by);
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[g][c] = __fmul2_rn(o[g][c], b2);
+                    d_up = (uint32_t)(15 + k) * 0x04000400u;
+                }
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int k = 0; k < 2; ++k)
 #pragma unroll
-                        for (int g = 0; g < G; ++g) big = max(big, max(h2bits(d[u][k][g]) & 0x7FFFu, h2bits(d[u][k][g]) >> 16 & 0x7FFFu));
-                room = 14.f - (float)((int)(__reduce_max_sync(0xFFFFFFFFu, big) >> 10) - 15);
+                        for (int g = 0; g < G; ++g) d[u][k][g] = __hmul2(d[u][k][g], bits_h2(d_up));
             }
             // ---- weights
             const float smax = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                                      fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-            if (__any_sync(0xFFFFFFFFu, smax > ref + room)) {
+            if (__any_sync(0xFFFFFFFFu, smax > ref + 14.f)) {
                 float m = fmaxf(smax, __shfl_xor_sync(0xFFFFFFFFu, smax, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-                const float to = m > ref + room ? m - (room - 4.f) : ref;
+                const float to = m > ref + 14.f ? m - 10.f : ref;
                 const float keep = exp2_fast(ref - to);
                 ref = to;
                 l *= keep;
@@ -769,13 +795,14 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
         {
             // sums of p (m / 2 + 4 d): column 2g, i.e. lane t = g, element 0
+            const float down = __uint_as_float((127 + 15 - (d_up >> 26)) << 23);  // 2^-k
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const float mid = __shfl_sync(0xFFFFFFFFu, om, (lane & ~3) + g);
+                const float mid = 2.f * __shfl_sync(0xFFFFFFFFu, om, (lane & ~3) + g);
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     *reinterpret_cast<float2*>(&sm.o[warp][r][32 * g + 8 * c + 2 * t]) =
-                        make_float2(fmaf(2.f, mid, o[g][c].x), fmaf(2.f, mid, o[g][c].y));
+                        make_float2(fmaf(o[g][c].x, down, mid), fmaf(o[g][c].y, down, mid));
             }
             if (t == 0) {
                 sm.ml[warp][r][0] = ref;

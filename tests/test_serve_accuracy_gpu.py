@@ -85,3 +85,11 @@ def _check(hd, kv, rep, rows, n, size):
 def test_small_weights_beside_a_dominating_position_prompts(cuda, lib, hd, kv, rep, rows, n, size):
     _check(hd, kv, rep, rows, n, size)
     _lib.check(lib.cllm_cuda_check_device_status())
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -8])
+@pytest.mark.parametrize("hd,kv,rep,rows,n", [(128, 1, 4, 1, 8000), (64, 2, 2, 1, 8000), (128, 1, 3, 1, 100000),
+                                              (64, 1, 1, 1, 100000)])
+def test_small_weights_beside_a_dominating_position_one_row(cuda, lib, hd, kv, rep, rows, n, size):
+    _check(hd, kv, rep, rows, n, size)
+    _lib.check(lib.cllm_cuda_check_device_status())

@@ -11,7 +11,8 @@ pages that takes 1.25 bytes per key/value pair of numbers instead of 8:
     o = cache.attention(layer, q)            # one new row per sequence
     cache, live = cache.compact()
 
-Everything runs on torch's current stream, reads nothing back to the host and
+Everything runs on torch's current stream of the cache's device, whichever device
+is current, with tensors of that device; it reads nothing back to the host and
 can be captured into a CUDA graph.  fork and compact move pages in place and
 return a cache with a new table; the old one must not be used after them.
 There is no fallback: without the CUDA library the calls fail.
@@ -36,25 +37,26 @@ def page_bytes(page_len: int, n_head_kv: int, head_dim: int) -> int:
 
 _I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 _raw_stream = torch._C._cuda_getCurrentRawStream  # torch's current stream of a device, as an integer
+_current_device = torch._C._cuda_getDevice
 
 
 def _refuse(what: str):
     raise _lib.CudaError(_lib.ERR_INVALID_ARG, "kv4: " + what)
 
 
-def _ready(t: torch.Tensor, dtype, what: str) -> None:
-    if t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
-        _refuse(f"{what} must be a contiguous CUDA tensor of {dtype}")
+def _ready(t: torch.Tensor, dtype, what: str, device: int) -> None:
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        _refuse(f"{what} must be a contiguous tensor of {dtype} on cuda:{device}")
 
 
-def _rows(t: torch.Tensor, what: str) -> tuple[int, int, int]:
+def _rows(t: torch.Tensor, what: str, device: int) -> tuple[int, int, int]:
     """(rows, values in a row, row stride) of a 2-D fp32 tensor whose rows are dense."""
-    if t.dtype is not _F32 or not t.is_cuda or t.dim() != 2:
-        _refuse(f"{what} must be a 2-D fp32 CUDA tensor with dense rows")
+    if t.dtype is not _F32 or t.get_device() != device or t.dim() != 2:
+        _refuse(f"{what} must be a 2-D fp32 tensor with dense rows on cuda:{device}")
     n, width = t.shape
     ld, step = t.stride()
     if step != 1 and width > 1:
-        _refuse(f"{what} must be a 2-D fp32 CUDA tensor with dense rows")
+        _refuse(f"{what} must be a 2-D fp32 tensor with dense rows on cuda:{device}")
     return n, width, ld if n > 1 else width
 
 
@@ -74,9 +76,12 @@ class KV4Cache:
                  "n_seqs", "max_pages", "page_bytes", "device")
 
     def __init__(self, pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor):
-        _ready(pages, _U8, "pages")
-        _ready(table, _I32, "table")
-        _ready(lens, _I32, "lens")
+        self.device = device = pages.get_device()
+        if device < 0:
+            _refuse("pages must be a CUDA tensor")
+        _ready(pages, _U8, "pages", device)
+        _ready(table, _I32, "table", device)
+        _ready(lens, _I32, "lens", device)
         shape, slots = pages.shape, table.shape
         if len(shape) != 5 or len(slots) != 2 or lens.shape[0] != slots[0] or shape[4] not in (1280, 2560):
             _refuse("pages [layer][page][kv head][page_len/16][20 head_dim], table [sequence][slot], lens [sequence]")
@@ -86,7 +91,6 @@ class KV4Cache:
         self.page_len, self.head_dim = tiles * TILE, tile_bytes // 20
         self.n_seqs, self.max_pages = slots
         self.page_bytes = self.n_head_kv * tiles * tile_bytes
-        self.device = pages.get_device()
 
     @classmethod
     def empty(cls, n_layers: int, n_pages: int, page_len: int, n_head_kv: int, head_dim: int, n_seqs: int,
@@ -107,17 +111,21 @@ class KV4Cache:
         """Write the rows of k and v (rotated by `rope`, the table of cllm_cuda_rope_table, where given) as the
         positions `pos` of the sequences `seq`.  Returns the rotated q (None without q); with `values` also the
         keys and values that the cache now holds: (q, k, v)."""
-        _ready(seq, _I32, "seq")
-        _ready(pos, _I32, "pos")
-        n, kv_dim, ldkv = _rows(k, "k")
-        if (n, kv_dim, ldkv) != _rows(v, "v") or kv_dim != self.n_head_kv * self.head_dim or seq.numel() != n or \
+        device = self.device
+        if _current_device() != device:  # the C calls launch on the current device
+            with torch.cuda.device(device):
+                return self.append(layer, k, v, seq, pos, q, rope, values)
+        _ready(seq, _I32, "seq", device)
+        _ready(pos, _I32, "pos", device)
+        n, kv_dim, ldkv = _rows(k, "k", device)
+        if (n, kv_dim, ldkv) != _rows(v, "v", device) or kv_dim != self.n_head_kv * self.head_dim or seq.numel() != n or \
                 pos.numel() != n:
             _refuse(f"k and v are rows of {self.n_head_kv * self.head_dim} values with one stride, seq and pos one "
                     "entry a row")
         qp = ldq = heads = qo = 0
         q_out = None
         if q is not None:
-            nq, width, ldq = _rows(q, "q")
+            nq, width, ldq = _rows(q, "q", device)
             heads = width // self.head_dim
             if nq != n or width % self.head_dim:
                 _refuse(f"q has a row per token, of heads of {self.head_dim}")
@@ -125,7 +133,7 @@ class KV4Cache:
             qp, qo = q.data_ptr(), q_out.data_ptr()
         table = n_pos = 0
         if rope is not None:
-            _ready(rope, _F32, "rope")
+            _ready(rope, _F32, "rope", device)
             n_pos, rest = divmod(rope.numel(), self.head_dim)
             if rest:
                 _refuse("rope is [position][head_dim / 2][2]")
@@ -138,7 +146,7 @@ class KV4Cache:
         rc = self.lib.cllm_cuda_kv4_append(
             qp, ldq, qo, k.data_ptr(), v.data_ptr(), ldkv, n, heads, table, n_pos, seq.data_ptr(), pos.data_ptr(),
             self._layer(layer), self.n_pages, self.page_len, self.n_head_kv, self.head_dim, self.table.data_ptr(),
-            self.n_seqs, self.max_pages, ko, vo, _raw_stream(self.device))
+            self.n_seqs, self.max_pages, ko, vo, _raw_stream(device))
         if rc:
             _lib.check(rc)
         return (q_out, k_out, v_out) if values else q_out
@@ -148,13 +156,17 @@ class KV4Cache:
         """Attention of the newest rows of every sequence: sequence s brings the rows begin[s] .. begin[s+1] of q
         (one each without `begin`), the last of which sees all its positions.  Returns [rows][heads * head_dim];
         with `lse` also [rows][heads], the log of the softmax's sum."""
-        n, width, ldq = _rows(q, "q")
+        device = self.device
+        if _current_device() != device:
+            with torch.cuda.device(device):
+                return self.attention(layer, q, begin, scale, lse)
+        n, width, ldq = _rows(q, "q", device)
         heads = width // self.head_dim
         if width % self.head_dim:
             _refuse(f"q has rows of heads of {self.head_dim}")
         first = 0
         if begin is not None:
-            _ready(begin, _I32, "begin")
+            _ready(begin, _I32, "begin", device)
             if begin.numel() != self.n_seqs + 1:
                 _refuse("begin has an entry more than there are sequences")
             first = begin.data_ptr()
@@ -163,7 +175,7 @@ class KV4Cache:
         rc = self.lib.cllm_cuda_kv4_attention(
             q.data_ptr(), ldq, first, n, heads, self._layer(layer), self.n_pages, self.page_len, self.n_head_kv,
             self.head_dim, self.table.data_ptr(), self.lens.data_ptr(), self.n_seqs, self.max_pages, scale,
-            out.data_ptr(), logs.data_ptr() if lse else 0, _raw_stream(self.device))
+            out.data_ptr(), logs.data_ptr() if lse else 0, _raw_stream(device))
         if rc:
             _lib.check(rc)
         return (out, logs) if lse else out
@@ -180,8 +192,12 @@ class KV4Cache:
     def fork(self, source: torch.Tensor, new_len: torch.Tensor) -> "KV4Cache":
         """New sequence s continues old sequence source[s] (-1: none) and has room for new_len[s] positions; old
         sequences that none continues are freed.  A sequence that finds no room has length -1 afterwards."""
-        _ready(source, _I32, "source")
-        _ready(new_len, _I32, "new_len")
+        device = self.device
+        if _current_device() != device:
+            with torch.cuda.device(device):
+                return self.fork(source, new_len)
+        _ready(source, _I32, "source", device)
+        _ready(new_len, _I32, "new_len", device)
         n = source.numel()
         if new_len.numel() != n:
             _refuse("source and new_len have one entry per new sequence")
@@ -190,19 +206,23 @@ class KV4Cache:
         rc = self.lib.cllm_cuda_kv4_fork(
             self.pages.data_ptr(), self.n_layers, self.n_pages, self.page_bytes, self.page_len,
             self.table.data_ptr(), self.lens.data_ptr(), self.n_seqs, source.data_ptr(), new_len.data_ptr(), n,
-            self.max_pages, table.data_ptr(), lens.data_ptr(), _raw_stream(self.device))
+            self.max_pages, table.data_ptr(), lens.data_ptr(), _raw_stream(device))
         if rc:
             _lib.check(rc)
         return self._with(table, lens, n)
 
     def compact(self) -> tuple["KV4Cache", torch.Tensor]:
         """Move the pages in use to the lowest ids; returns the cache and their number (int32 [1])."""
+        device = self.device
+        if _current_device() != device:
+            with torch.cuda.device(device):
+                return self.compact()
         table = torch.empty_like(self.table)
         live = self.lens.new_empty(1)
         rc = self.lib.cllm_cuda_kv4_compact(
             self.pages.data_ptr(), self.n_layers, self.n_pages, self.page_bytes, self.page_len,
             self.table.data_ptr(), self.lens.data_ptr(), self.n_seqs, self.max_pages, table.data_ptr(),
-            live.data_ptr(), _raw_stream(self.device))
+            live.data_ptr(), _raw_stream(device))
         if rc:
             _lib.check(rc)
         return self._with(table, self.lens, self.n_seqs), live

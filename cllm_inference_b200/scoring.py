@@ -12,6 +12,9 @@ import torch
 
 from . import _lib
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch's current stream of a device, as an integer
+_current_device = torch._C._cuda_getDevice
+
 
 class TokenScores(NamedTuple):
     logprob: torch.Tensor | None  # fp32 [rows], None without tokens
@@ -22,14 +25,19 @@ class TokenScores(NamedTuple):
 
 
 def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, top_k: int = 0) -> TokenScores:
-    """Scores of fp32 CUDA logits [rows][vocab] (any row stride), on torch's current stream."""
-    if not logits.is_cuda or logits.dtype != torch.float32 or logits.dim() != 2 or (
+    """Scores of fp32 CUDA logits [rows][vocab] (any row stride) and int32 tokens of one device, on torch's
+    current stream of it."""
+    device = logits.get_device()
+    if device < 0 or logits.dtype != torch.float32 or logits.dim() != 2 or (
             logits.shape[1] > 1 and logits.stride(1) != 1):
         raise _lib.CudaError(_lib.ERR_INVALID_ARG, "token_scores: logits must be a 2-D fp32 CUDA tensor with dense rows")
+    if _current_device() != device:  # the C call launches on the current device
+        with torch.cuda.device(device):
+            return token_scores(logits, tokens, top_k)
     rows, vocab = logits.shape
-    if tokens is not None and (not tokens.is_cuda or tokens.dtype != torch.int32 or tokens.numel() != rows or
+    if tokens is not None and (tokens.get_device() != device or tokens.dtype != torch.int32 or tokens.numel() != rows or
                                not tokens.is_contiguous()):
-        raise _lib.CudaError(_lib.ERR_INVALID_ARG, "token_scores: tokens must be int32, contiguous, one per row")
+        raise _lib.CudaError(_lib.ERR_INVALID_ARG, "token_scores: tokens must be int32, contiguous, one per row, beside the logits")
     k = max(0, top_k)
     entropy = logits.new_empty(rows)
     logprob = rank = None
@@ -41,7 +49,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, top_k
     ids = torch.empty_like(logprobs, dtype=torch.int32)
     rc = _lib.load().cllm_cuda_token_scores(
         logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, tp, top_k, lp, entropy.data_ptr(),
-        rp, ids.data_ptr(), logprobs.data_ptr(), torch._C._cuda_getCurrentRawStream(logits.get_device()))
+        rp, ids.data_ptr(), logprobs.data_ptr(), _raw_stream(device))
     if rc:
         _lib.check(rc)
     return TokenScores(logprob, rank, entropy, ids, logprobs)

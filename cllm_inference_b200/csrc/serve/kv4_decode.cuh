@@ -38,7 +38,7 @@
 //   the largest one so far below 2 and to 2^-3 or more: a p of at most 2^14 then keeps
 //   p d inside fp16, and p d is off by 2^-25 at most where p of the largest weight is 2^10
 //   or more, so small weights count beside a dominating one however small the values
-//   are.  Scales of 2^-3 to 2 need no power, and cost a test (64 sequences: 0.4 us).
+//   are.  Scales of 2^-3 to 2 need no power and take no time.
 // * Work: steps of 128 positions of (sequence, KV head, 8 rows), numbered through
 //   (and some for the item itself) and cut into equal runs, one per CTA,
 //   whatever the lengths are.  A CTA's four
@@ -657,36 +657,40 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int g = 0; g < G; ++g) big |= h2bits(d[u][k][g]);
-            const bool two = __any_sync(0xFFFFFFFFu, (big & 0x40004000u) != 0);  // a scale is 2 or more
-            // a first scale of 2^-3 or more (or of 2^-7 with some a sixteenth of it) needs no k
-            if (d_up == kFirst && !two && __any_sync(0xFFFFFFFFu, (big & big << 1 & 0x20002000u) != 0)) d_up = kOne;
-            if (two || d_up != kOne) {
-                __half2 some[4];  // NaNs do not count
+            if (__any_sync(0xFFFFFFFFu, d_up != kOne || (big & 0x40004000u) != 0)) {  // k is not 0, or a scale is 2 or more
+                // a first scale of 2^-3 or more (or of 2^-7 with some a sixteenth of it) needs no k
+                const bool plain = d_up == kFirst && !__any_sync(0xFFFFFFFFu, (big & 0x40004000u) != 0) &&
+                                   __any_sync(0xFFFFFFFFu, (big & big << 1 & 0x20002000u) != 0);
+                if (plain) {
+                    d_up = kOne;
+                } else {
+                    __half2 some[4];  // NaNs do not count
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    some[i] = __hmax2(__habs2(d[i / 2][i % 2][0]), __habs2(d[i / 2][i % 2][1]));
-                    if constexpr (G == 4) some[i] = __hmax2(some[i], __hmax2(__habs2(d[i / 2][i % 2][2]), __habs2(d[i / 2][i % 2][3])));
+                    for (int i = 0; i < 4; ++i) {
+                        some[i] = __hmax2(__habs2(d[i / 2][i % 2][0]), __habs2(d[i / 2][i % 2][1]));
+                        if constexpr (G == 4) some[i] = __hmax2(some[i], __hmax2(__habs2(d[i / 2][i % 2][2]), __habs2(d[i / 2][i % 2][3])));
+                    }
+                    const __half2 most = __hmax2(__hmax2(some[0], some[1]), __hmax2(some[2], some[3]));
+                    const uint32_t lo = h2bits(most) & 0xFFFFu, hi = h2bits(most) >> 16;
+                    const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(lo > 0x7C00u ? 0u : lo, hi > 0x7C00u ? 0u : hi));
+                    const int e = (int)(top >> 10) - 15, k0 = (int)(d_up >> 26) - 15;
+                    const int k = min(k0, e >= 1 ? max(-14, -e) : e >= -3 ? 0 : -e);
+                    if (k != k0) {
+                        const float by = __uint_as_float((uint32_t)(127 + k - k0) << 23);
+                        const float2 b2 = make_float2(by, by);
+#pragma unroll
+                        for (int g = 0; g < G; ++g)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) o[g][c] = __fmul2_rn(o[g][c], b2);
+                        d_up = (uint32_t)(15 + k) * 0x04000400u;
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int g = 0; g < G; ++g) d[u][k][g] = __hmul2(d[u][k][g], bits_h2(d_up));
                 }
-                const __half2 most = __hmax2(__hmax2(some[0], some[1]), __hmax2(some[2], some[3]));
-                const uint32_t lo = h2bits(most) & 0xFFFFu, hi = h2bits(most) >> 16;
-                const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, max(lo > 0x7C00u ? 0u : lo, hi > 0x7C00u ? 0u : hi));
-                const int e = (int)(top >> 10) - 15, k0 = (int)(d_up >> 26) - 15;
-                const int k = min(k0, e >= 1 ? max(-14, -e) : e >= -3 ? 0 : -e);
-                if (k != k0) {
-                    const float by = __uint_as_float((uint32_t)(127 + k - k0) << 23);
-                    const float2 b2 = make_float2(by, by);
-#pragma unroll
-                    for (int g = 0; g < G; ++g)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) o[g][c] = __fmul2_rn(o[g][c], b2);
-                    d_up = (uint32_t)(15 + k) * 0x04000400u;
-                }
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int g = 0; g < G; ++g) d[u][k][g] = __hmul2(d[u][k][g], bits_h2(d_up));
             }
             // ---- weights
             const float smax = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),

@@ -62,7 +62,6 @@ constexpr int kPairLen = 2 * kTile;         // positions of a warp's step
 constexpr int kStepLen = kPairLen * kRowWarps;
 constexpr int kRowCtasPerSm = 3;            // of 168 registers a thread: 64 sequences 67.6 us, 2 of 255 registers 73.3
 constexpr int kMaxRowCtas = 640;
-constexpr uint32_t kNoTile = 0xFFFFFFFFu;
 
 struct AttnArgs {
     const float* q;
@@ -74,6 +73,7 @@ struct AttnArgs {
     float scale;
     float *out, *lse;
     Cache c;
+    const uint8_t* nan_tile;  // g_nan_tile
     int page_tiles;        // tiles of a page and head
     uint32_t page_magic;   // ceil(2^32 / page_tiles), 0 where that is 2^32
     // Slot of the page that holds a tile (< 2^27): the product is at most one too large.
@@ -451,14 +451,14 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     // The producer runs ahead of the warp's own tiles.  Lane i holds the places
     // of the i-th of up to 32 pairs of one item and copies them itself.
     Cursor pro = cur;
-    uint32_t pro_a = 0, pro_b = kNoTile;  // tiles of the pool, counted from the layer's first
+    const uint8_t *pro_a = nullptr, *pro_b = nullptr;  // no second tile: nullptr
     int pro_i = 0, pro_n = 0;
     Stage put, get;
-    auto place = [&](int tile) -> uint32_t {
+    auto place = [&](int tile) -> const uint8_t* {
         const int slot = a.page_of(tile);
-        int id = a.c.page(pro.s, slot);
-        if (id < 0) id = 0;  // flagged; the copy has to stay inside the pool
-        return ((uint32_t)id * a.c.n_kv + pro.item / (pro.w.items / a.c.n_kv)) * a.page_tiles + (tile - slot * a.page_tiles);
+        const int id = a.c.page(pro.s, slot);
+        const uint32_t at = ((uint32_t)id * a.c.n_kv + pro.item / (pro.w.items / a.c.n_kv)) * a.page_tiles + (tile - slot * a.page_tiles);
+        return id < 0 ? a.nan_tile : a.c.pages + (uint64_t)at * Tile<HD>::kBytes;
     };
     auto refill = [&]() {
         pro_i = pro_n = 0;
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
             const bool there = lane < units && step >= 0 && tile * kTile < pro.w.len;
             if (there) {
                 pro_a = place(tile);
-                pro_b = (tile + 1) * kTile < pro.w.len ? place(tile + 1) : kNoTile;
+                pro_b = (tile + 1) * kTile < pro.w.len ? place(tile + 1) : nullptr;
             }
             const uint32_t lanes = __ballot_sync(0xFFFFFFFFu, there);  // consecutive
             if (lanes) {
@@ -485,10 +485,10 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
         }
         if (lane == pro_i) {
             const uint32_t bar = full + 8 * put.i, to = ring + put.i * (2 * Tile<HD>::kBytes);
-            const bool two = pro_b != kNoTile;
+            const bool two = pro_b != nullptr;
             mbar_arrive_expect_tx(bar, two ? 2 * Tile<HD>::kBytes : Tile<HD>::kBytes);
-            bulk_g2s(to, a.c.pages + (uint64_t)pro_a * Tile<HD>::kBytes, Tile<HD>::kBytes, bar);
-            if (two) bulk_g2s(to + Tile<HD>::kBytes, a.c.pages + (uint64_t)pro_b * Tile<HD>::kBytes, Tile<HD>::kBytes, bar);
+            bulk_g2s(to, pro_a, Tile<HD>::kBytes, bar);
+            if (two) bulk_g2s(to + Tile<HD>::kBytes, pro_b, Tile<HD>::kBytes, bar);
         }
         ++pro_i;
         put.next();

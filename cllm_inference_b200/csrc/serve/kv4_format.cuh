@@ -27,6 +27,16 @@ struct Tile {
     static constexpr uint32_t kBytes = 20 * HD;
 };
 
+// What attention reads for a page that does not exist: a tile whose scales are
+// all NaN, so the rows that see it are NaN.  All bits set, for either head_dim.
+struct NanTile {
+    uint64_t bits[Tile<128>::kBytes / 8];
+    constexpr NanTile() : bits() {
+        for (uint64_t& b : bits) b = ~0ull;
+    }
+};
+__device__ const NanTile g_nan_tile alignas(128);
+
 // One layer's pool and the sequences in it.
 struct Cache {
     uint8_t* pages;

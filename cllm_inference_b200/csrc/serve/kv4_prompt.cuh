@@ -417,11 +417,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                 for (int i = from; i < to && !*abort; ++i) {
                     const int st = it % kRawStages, tile = 4 * i + lane;
                     const bool there = lane < 4 && tile * kTile < len;
-                    int64_t src = 0;
+                    const uint8_t* src = a.nan_tile;
                     if (there) {
                         const int slot = a.page_of(tile);
-                        const int id = max(0, a.c.page(seq, slot));  // a bad one is flagged; the copy stays inside the pool
-                        src = (((int64_t)id * a.c.n_kv + cur.kvh) * a.page_tiles + (tile - slot * a.page_tiles)) * Tile<HD>::kBytes;
+                        const int id = a.c.page(seq, slot);
+                        if (id >= 0)
+                            src = a.c.pages + (((int64_t)id * a.c.n_kv + cur.kvh) * a.page_tiles + (tile - slot * a.page_tiles)) * Tile<HD>::kBytes;
                     }
                     if (it >= kRawStages) warp_wait(bar(sm.raw_empty[st]), (uint32_t)(it / kRawStages - 1) & 1u, abort);
                     const uint32_t n = __popc(__ballot_sync(0xFFFFFFFFu, there));
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) kv4_prompt_kernel(const Pro
                     if (dead) break;
                     if (lane == 0) mbar_arrive_expect_tx(bar(sm.raw_full[st]), n * Tile<HD>::kBytes);
                     __syncwarp();
-                    if (there) bulk_g2s(smem_addr(sm.raw[st]) + lane * Tile<HD>::kBytes, a.c.pages + src, Tile<HD>::kBytes, bar(sm.raw_full[st]));
+                    if (there) bulk_g2s(smem_addr(sm.raw[st]) + lane * Tile<HD>::kBytes, src, Tile<HD>::kBytes, bar(sm.raw_full[st]));
                     ++it;
                 }
             }

@@ -79,9 +79,13 @@ int g_set[64];  // of g_rows_arrived, the last call's; host_workspace's lock gua
 template <int HD>
 int launch_attention(AttnArgs a, int dev, int sms, cudaStream_t st) {
     static std::once_flag once[64];
-    cudaError_t attr = cudaSuccess;
-    std::call_once(once[dev], [&] {
-        attr = cudaFuncSetAttribute(kv4_rows_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(RowsSmem<HD>));
+    static void* nan_tile[64];
+    static cudaError_t ready[64];
+    std::call_once(once[dev], [dev] {
+        cudaError_t& attr = ready[dev];
+        attr = cudaGetSymbolAddress(&nan_tile[dev], g_nan_tile);
+        if (attr == cudaSuccess)
+            attr = cudaFuncSetAttribute(kv4_rows_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(RowsSmem<HD>));
         if (attr == cudaSuccess)
             attr = cudaFuncSetAttribute(kv4_rows_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         sizeof(RowsSmem<HD>));
@@ -89,7 +93,8 @@ int launch_attention(AttnArgs a, int dev, int sms, cudaStream_t st) {
             attr = cudaFuncSetAttribute(kv4_prompt_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         sizeof(PromptSmem<HD>) + 1024);
     });
-    CLLM_HOST_TRY(attr);
+    CLLM_HOST_TRY(ready[dev]);
+    a.nan_tile = static_cast<const uint8_t*>(nan_tile[dev]);
     const int ctas = std::min(kMaxRowCtas, kRowCtasPerSm * sms);
     const int64_t rows = (int64_t)a.n_tok * a.rep, groups = rows / kRowTile + a.c.n_seqs;  // at most
     const int64_t steps = ((int64_t)a.c.max_pages * a.c.page_len + kStepLen - 1) / kStepLen;

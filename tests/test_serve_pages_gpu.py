@@ -1,0 +1,35 @@
+"""Page tables that name pages which do not exist, and pools that are too small."""
+import numpy as np
+import pytest
+import torch
+
+from cllm_inference_b200 import _lib
+from tests import serve_oracle as O
+from tests.test_serve_gpu import _cache
+
+pytestmark = pytest.mark.gpu
+
+
+def _ints(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+# (hd, KV heads, heads a KV head, rows of the first sequence): one row, a few (rows kernel), many (prompt kernel)
+@pytest.mark.parametrize("hd,kv,rep,rows", [(128, 2, 4, 1), (64, 1, 3, 1), (128, 1, 2, 30), (64, 2, 2, 30),
+                                            (128, 1, 1, 9000), (64, 2, 3, 3000)])
+@pytest.mark.parametrize("bad", [12, -1, 2 ** 30])
+def test_rows_that_see_a_page_outside_the_pool_are_nan(cuda, lib, hd, kv, rep, rows, bad):
+    rng = np.random.default_rng(rows + hd)
+    cache, _, _ = _cache(rng, 1, 12, 32, kv, hd, [150, 77], 5)
+    q = torch.randn(rows + 3, kv * rep * hd, device="cuda")
+    begin = _ints(0, rows, rows + 3)
+    want, want_lse = cache.attention(0, q, begin=begin, lse=True)
+    cache.table[0, 4] = bad  # positions 128 to 149
+    got, lse = cache.attention(0, q, begin=begin, lse=True)
+    assert lib.cllm_cuda_check_device_status() == _lib.ERR_INVALID_ARG
+    sees = 150 - (rows - 1 - torch.arange(rows, device="cuda")) > 128
+    assert torch.isnan(got[:rows][sees]).all() and torch.isnan(lse[:rows][sees]).all()
+    assert not torch.isnan(got[:rows][~sees]).any() and torch.equal(got[rows:], want[rows:])
+    torch.testing.assert_close(got[:rows][~sees], want[:rows][~sees], rtol=2.0 ** -16, atol=2.0 ** -16)
+    torch.testing.assert_close(lse[rows:], want_lse[rows:], rtol=0, atol=0)
+    _lib.check(lib.cllm_cuda_check_device_status())

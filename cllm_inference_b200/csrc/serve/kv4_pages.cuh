@@ -185,9 +185,10 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const PagesArgs
             held = kept / a.page_len;
             if (kept % a.page_len) {
                 last = page_at(a, src, held);
-                const bool keeps = last >= 0 && (a.part_bits[last >> 5] >> (last & 31) & 1u) && a.owner[last] == (uint32_t)s;
+                // an id outside the pool stays in the table, where every reader finds it
+                const bool keeps = last < 0 || ((a.part_bits[last >> 5] >> (last & 31) & 1u) && a.owner[last] == (uint32_t)s);
                 held += keeps;
-                copy = !keeps && last >= 0;
+                copy = !keeps;
             }
             need = goal - held;
         }
@@ -356,9 +357,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) fork_small_kernel(const Page
         held = kept / a.page_len;
         if (kept % a.page_len) {
             last = page_at(a, src, held);
-            const bool keeps = last >= 0 && (sm.part_bits[last >> 5] >> (last & 31) & 1u) && sm.owner[last] == (uint32_t)tid;
+            const bool keeps = last < 0 || ((sm.part_bits[last >> 5] >> (last & 31) & 1u) && sm.owner[last] == (uint32_t)tid);
             held += keeps;
-            copy = !keeps && last >= 0;
+            copy = !keeps;
         }
         need = (fine ? pages_of(want, a.page_len) : 0) - held;
         if (!fine) need = 0;

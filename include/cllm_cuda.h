@@ -390,7 +390,8 @@ int cllm_cuda_attention(const float* q, const float* k_cache, const float* v_cac
  * never followed; it sets the device status, which
  * cllm_cuda_check_device_status reports as CLLM_ERR_INVALID_ARG.  append then
  * stores nothing (k_out and v_out are 0); attention reads the positions of such
- * a page as NaN, and leaves out those past max_pages * page_len. */
+ * a page as NaN, and leaves out those past max_pages * page_len; fork and compact
+ * carry its id along. */
 
 /* Bytes of one page of one layer; 0 for a geometry that is not supported. */
 int64_t cllm_cuda_kv4_page_bytes(int page_len, int n_head_kv, int head_dim);

@@ -33,3 +33,23 @@ def test_rows_that_see_a_page_outside_the_pool_are_nan(cuda, lib, hd, kv, rep, r
     torch.testing.assert_close(got[:rows][~sees], want[:rows][~sees], rtol=2.0 ** -16, atol=2.0 ** -16)
     torch.testing.assert_close(lse[rows:], want_lse[rows:], rtol=0, atol=0)
     _lib.check(lib.cllm_cuda_check_device_status())
+
+
+@pytest.mark.parametrize("pool", [9, 20000])  # one launch, four launches
+@pytest.mark.parametrize("bad", [20000, -7])
+def test_fork_and_compact_carry_a_page_outside_the_pool_along(cuda, lib, pool, bad):
+    """A sequence whose unfinished page does not exist gets no other page's content for it."""
+    rng = np.random.default_rng(pool)
+    cache, _, _ = _cache(rng, 1, pool, 16, 1, 64, [40, 40], 3)
+    cache.table[0, 2] = bad  # positions 32 to 39
+    new = cache.fork(_ints(0, 0, 1, 0), _ints(41, 48, 41, 32))
+    assert lib.cllm_cuda_check_device_status() == _lib.ERR_INVALID_ARG
+    assert new.lens.tolist() == [41, 48, 41, 32]
+    assert new.table[0, 2] == bad and new.table[1, 2] == bad and new.table[3, 2] == -1
+    assert torch.equal(new.table[2], cache.table[1])
+    packed, live = new.compact()
+    assert lib.cllm_cuda_check_device_status() == _lib.ERR_INVALID_ARG
+    assert int(live[0]) == 5 and packed.table[0, 2] == bad and packed.table[1, 2] == bad
+    o = packed.attention(0, torch.randn(4, 64, device="cuda"))
+    assert lib.cllm_cuda_check_device_status() == _lib.ERR_INVALID_ARG
+    assert torch.isnan(o[:2]).all() and torch.isfinite(o[2:]).all()

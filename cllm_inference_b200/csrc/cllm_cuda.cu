@@ -110,6 +110,7 @@ DeviceInfo g_dev[64];
 struct Workspace {
     void* ptr = nullptr;
     size_t cap = 0;
+    bool captured = false;  // a call that was being captured has got it: a graph may hold its address
 };
 Workspace g_ws[64];
 std::mutex g_ws_mu[64];  // one per device: held from workspace() until the call's kernels are enqueued
@@ -172,20 +173,27 @@ void* mapped_host(const void* p) {
 // (free and reallocate) the buffer between this call and those launches.
 // What the lock cannot order is work already enqueued on other streams:
 // calls that may overlap on the GPU must be serialised by the caller.
-int workspace(int dev, size_t bytes, uint8_t** out, std::unique_lock<std::mutex>& lk) {
+// A buffer that a call under capture was given is kept when the workspace
+// grows, since the caller's graph goes on using it: each such buffer is at
+// least a quarter larger than the one before.
+int workspace(int dev, size_t bytes, cudaStream_t st, uint8_t** out, std::unique_lock<std::mutex>& lk) {
     lk = std::unique_lock<std::mutex>(g_ws_mu[dev]);
     Workspace& ws = g_ws[dev];
     if (ws.cap < bytes) {
-        if (ws.ptr) {
+        if (ws.ptr && !ws.captured) {
             CLLM_CUDA_TRY(cudaDeviceSynchronize());  // a previous call may still use it
             CLLM_CUDA_TRY(cudaFree(ws.ptr));
-            ws.ptr = nullptr;
-            ws.cap = 0;
         }
+        ws = Workspace{};
         const size_t cap = std::max<size_t>(bytes + (bytes >> 2), size_t(4) << 20);
         CLLM_CUDA_TRY(cudaMalloc(&ws.ptr, cap));
         ws.cap = cap;
         g_memory_gen.fetch_add(1);
+    }
+    if (!ws.captured) {
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(st, &cs) != cudaSuccess) (void)cudaGetLastError();  // the default stream, beside a capture
+        ws.captured = cs != cudaStreamCaptureStatusNone;
     }
     *out = static_cast<uint8_t*>(ws.ptr);
     return CLLM_OK;
@@ -806,7 +814,7 @@ int matmul_quant_impl(const float* x, const void* w, int type, const float* bias
     if (scratch) {
         if (total > scratch_cap)
             return fail(CLLM_ERR_TOO_LARGE, "%s: %zu bytes of scratch needed, %zu given", fname, total, scratch_cap);
-    } else if (int rc = workspace(dev, total, &ws, ws_lock)) {
+    } else if (int rc = workspace(dev, total, st, &ws, ws_lock)) {
         return rc;
     }
 
@@ -932,7 +940,7 @@ int host_graph_call(const float* x, const void* w, int type, const float* bias, 
     if (int rc = matmul_quant_impl(x, w, type, bias, in_dim, out_dim, n_rows, y, flags, st, nullptr, 0, &total))
         return rc;
     uint8_t* ws = nullptr;
-    if (int rc = workspace(dev, total, &ws, ws_lock)) return rc;  // may move the workspace (new generation)
+    if (int rc = workspace(dev, total, st, &ws, ws_lock)) return rc;  // may move the workspace (new generation)
     const uint64_t gen = g_memory_gen.load();
     it = cache.find(key);
     if (it != cache.end()) {
@@ -1112,7 +1120,7 @@ int cllm_cuda_matmul_q8(const float* scales, const int8_t* qs, const int32_t* bs
     const int64_t nb = in_dim / 32;
     uint8_t* ws;
     std::unique_lock<std::mutex> ws_lock;
-    if (int rc = workspace(dev, align256((size_t)n_rows * nb) + 256, &ws, ws_lock)) return rc;
+    if (int rc = workspace(dev, align256((size_t)n_rows * nb) + 256, st, &ws, ws_lock)) return rc;
     const int64_t total = nb * n_rows;
     if (total > 0) {
         const int64_t grid = std::min<int64_t>((total + 7) / 8, 16LL * di.sms);
@@ -1163,7 +1171,7 @@ int cllm_cuda_row_partials(const int8_t* qs, const void* w, int type, int in_dim
     const ActLayout L = act_layout(1, in_dim, 0);
     uint8_t* ws;
     std::unique_lock<std::mutex> ws_lock;
-    if (int rc = workspace(dev, L.end, &ws, ws_lock)) return rc;
+    if (int rc = workspace(dev, L.end, st, &ws, ws_lock)) return rc;
     CLLM_CUDA_TRY(cudaMemsetAsync(ws + L.dx, 0, L.fl - L.dx, st));
     CLLM_CUDA_TRY(cudaMemsetAsync(ws + L.fl, 1, L.end - L.fl, st));
     for (int t = 0; t < n_rows; ++t) {
@@ -1203,7 +1211,7 @@ int cllm_cuda_matmul_partials(const float* x, const void* w, int type, int in_di
     if (want_image) total = align256(total + image_bytes(mchunk, in_dim));
     uint8_t* ws;
     std::unique_lock<std::mutex> ws_lock;
-    if (int rc = workspace(dev, total, &ws, ws_lock)) return rc;
+    if (int rc = workspace(dev, total, static_cast<cudaStream_t>(stream), &ws, ws_lock)) return rc;
     return run_decode(type, static_cast<const uint8_t*>(w), row_bytes, x, nullptr, in_dim, out_dim, n_rows,
                       nullptr, partials, ws, L, want_image ? ws + off_img : nullptr, g_dev[dev],
                       static_cast<cudaStream_t>(stream));
@@ -1400,9 +1408,9 @@ int cllm_cuda_matmul_quant_rowshard(const float* x, const void* w_shard, int typ
     uint8_t* ws = nullptr;
     std::unique_lock<std::mutex> ws_lock;
     if (!pl.fused) {
-        if (int rc = workspace(dev, L.end, &ws, ws_lock)) return rc;
+        if (int rc = workspace(dev, L.end, st, &ws, ws_lock)) return rc;
     } else if (use_image) {
-        if (int rc = workspace(dev, image_bytes(n_rows, in_dim), &ws, ws_lock)) return rc;
+        if (int rc = workspace(dev, image_bytes(n_rows, in_dim), st, &ws, ws_lock)) return rc;
     }
     GemvParams p{};
     p.w = wd;
@@ -1559,8 +1567,8 @@ int host_device(int* dev, int* sms) {
     return CLLM_OK;
 }
 
-int host_workspace(int dev, size_t bytes, uint8_t** out, std::unique_lock<std::mutex>& lk) {
-    return workspace(dev, bytes, out, lk);
+int host_workspace(int dev, size_t bytes, cudaStream_t st, uint8_t** out, std::unique_lock<std::mutex>& lk) {
+    return workspace(dev, bytes, st, out, lk);
 }
 
 }  // namespace cllm

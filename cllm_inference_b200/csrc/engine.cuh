@@ -999,12 +999,12 @@ int cllm_cuda_attention(const float* q, const float* k_cache, const float* v_cac
     if (int rc = ensure_device(&dev)) return rc;
     const int chunks = (pos0 + n_tok + eng::kAttnChunk - 1) / eng::kAttnChunk;
     const size_t parts = (size_t)n_tok * n_head * chunks;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
     uint8_t* ws;
     std::unique_lock<std::mutex> ws_lock;
-    if (int rc = workspace(dev, align256(parts * 2 * 4) + parts * head_dim * 4, &ws, ws_lock)) return rc;
+    if (int rc = workspace(dev, align256(parts * 2 * 4) + parts * head_dim * 4, st, &ws, ws_lock)) return rc;
     float* ml = reinterpret_cast<float*>(ws);
     float* acc = reinterpret_cast<float*>(ws + align256(parts * 2 * 4));
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     const float scale = 1.0f / std::sqrt((float)head_dim);
     const dim3 grid(n_head_kv, chunks, n_tok);
 #define CLLM_ATTN_OP(HD, R) eng::attn_chunk_kernel<HD, R><<<grid, eng::kAttnThreads, 0, st>>>(q, k_cache, v_cache, n_head_kv, nullptr, pos0, scale, ml, acc)

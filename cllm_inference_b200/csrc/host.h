@@ -2,6 +2,7 @@
 // units: the calling thread's error message, the device check and the
 // per-device workspace (one workspace and one lock for the whole library).
 #pragma once
+#include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
 
@@ -17,9 +18,9 @@ int host_fail(int code, const char* fmt, ...);
 // The current device, checked for sm_100, and its SM count.
 int host_device(int* dev, int* sms);
 
-// The device's workspace of at least `bytes`; keep `lk` until every kernel
-// that uses it is enqueued.
-int host_workspace(int dev, size_t bytes, uint8_t** out, std::unique_lock<std::mutex>& lk);
+// The device's workspace of at least `bytes` for kernels on `st`; keep `lk`
+// until every one that uses it is enqueued.
+int host_workspace(int dev, size_t bytes, cudaStream_t st, uint8_t** out, std::unique_lock<std::mutex>& lk);
 
 // Device status bits of the serving operators' translation unit.
 constexpr int kServeTimeout = 1;   // a bounded wait expired

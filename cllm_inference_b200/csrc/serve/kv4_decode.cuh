@@ -93,8 +93,10 @@ struct RowsArgs {
     float* part_o;   // [2 * ctas][kRowTile][HD]
 };
 // Parts of the item that begins in CTA c that are there.  The last one to come
-// sets it back to 0.  Every call clears the other set, so a wrong count (calls
-// that overlapped, which their caller must not let happen) does not stay.
+// sets it back to 0.  Calls take the two sets in turn, and each clears the other
+// one: a wrong count (of calls that overlapped, which their caller must not let
+// happen) does not reach later calls.  A captured call has the same set in every
+// replay; in a graph with one such call a wrong count stays until a call outside of it.
 __device__ unsigned g_rows_arrived[2][kMaxRowCtas];
 
 // CTA whose run has unit u: runs begin at floor(c * all / ctas).

@@ -118,7 +118,7 @@ int launch_attention(AttnArgs a, int dev, int sms, cudaStream_t st) {
     const size_t p_o = part(prompts ? (size_t)2 * sms * kPromptRows * HD * 4 : 0);
     uint8_t* ws;
     std::unique_lock<std::mutex> lk;
-    if (int rc = host_workspace(dev, bytes, &ws, lk)) return rc;
+    if (int rc = host_workspace(dev, bytes, st, &ws, lk)) return rc;
 
     RowsArgs ra{a, g_set[dev] ^= 1, reinterpret_cast<float*>(ws + r_ml), reinterpret_cast<float*>(ws + r_o)};
     PromptArgs pa{};
@@ -268,7 +268,7 @@ static int pages_call(const char* who, PagesArgs a, void* pages, int64_t page_by
     const size_t seqs = align256(4 * (size_t)a.n_new);
     uint8_t* ws;
     std::unique_lock<std::mutex> lk;
-    if (int rc = host_workspace(dev, 2 * bits + 3 * list + pairs + 2 * seqs + 256, &ws, lk)) return rc;
+    if (int rc = host_workspace(dev, 2 * bits + 3 * list + pairs + 2 * seqs + 256, st, &ws, lk)) return rc;
     auto take = [&](size_t bytes) {
         uint8_t* p = ws;
         ws += bytes;

@@ -12,9 +12,12 @@ pages that takes 1.25 bytes per key/value pair of numbers instead of 8:
     cache, live = cache.compact()
 
 Everything runs on torch's current stream of the cache's device, whichever device
-is current, with tensors of that device; it reads nothing back to the host and
-can be captured into a CUDA graph.  fork and compact move pages in place and
-return a cache with a new table; the old one must not be used after them.
+is current, with tensors of that device, and reads nothing back to the host.  It
+can be captured into a CUDA graph, after a call of that size outside of it.  The
+library has one workspace for a device: attention, fork and compact on several
+streams, or in graphs, must not overlap on the GPU (order them with events).
+fork and compact move pages in place and return a cache with a new table; the old
+one must not be used after them.
 There is no fallback: without the CUDA library the calls fail.
 """
 from __future__ import annotations

@@ -112,8 +112,9 @@ int cllm_cuda_quantize_q8_0(const float* x, int64_t n, int rows, float* scales, 
  * `stream`; the flags above switch x/bias, y and w to host memory.  Scratch
  * for the quantized activations comes from one workspace per device that the
  * library grows on demand (cudaDeviceSynchronize, cudaFree, cudaMalloc) and
- * keeps until exit; make a first call of the largest size before capturing
- * calls into a CUDA graph.  Host threads may call concurrently (a per-device
+ * keeps until exit; a call under capture cannot grow it, so make a first call of
+ * that size before capturing calls into a CUDA graph (larger calls may follow:
+ * a graph keeps the workspace it was captured with).  Host threads may call concurrently (a per-device
  * lock is held until the call's kernels are enqueued), but calls whose GPU
  * work can overlap -- on different streams of one device -- share that
  * workspace and race on it: order them (one stream, or events). */
@@ -367,9 +368,10 @@ int cllm_cuda_attention(const float* q, const float* k_cache, const float* v_cac
  * No counterpart in the reference, whose engine serves one sequence from a
  * contiguous fp32 cache (engine.cpp:119-146).  Device pointers, fp32 in and
  * out, asynchronous on `stream`, no host read of anything on the device: every
- * call can be captured into a CUDA graph (make a first call of the largest
- * size before, as for cllm_cuda_matmul_quant: attention, fork and compact use
- * the library's workspace, so calls that can overlap must be ordered).
+ * call can be captured into a CUDA graph.  attention, fork and compact use the
+ * library's workspace, as cllm_cuda_matmul_quant does: make a first call of that
+ * size before a capture, and order calls, and replays of graphs that hold them,
+ * that could overlap on the GPU.
  *
  * Pool.  `pages` (16-byte aligned) holds n_layers x n_pages pages of
  * cllm_cuda_kv4_page_bytes bytes; the calls that work on one layer get that

@@ -7,7 +7,8 @@
 //            that ends in it
 //   plan     which sequences keep their last page, the pages each one needs,
 //            their prefix sum, the free pages in order (prefix sum over the
-//            bitmap), the list of copies
+//            bitmap), the list of copies.  The sum goes on past the pages there
+//            are, so the first sequence without room and all after it get none
 //   apply    the table rows, and the copies in every layer, 16 bytes a load
 // The results depend on no order of execution: marks are bits and minima, and
 // pages are handed out by prefix sums.

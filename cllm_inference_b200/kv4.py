@@ -17,7 +17,7 @@ can be captured into a CUDA graph, after a call of that size outside of it.  The
 library has one workspace for a device: attention, fork and compact on several
 streams, or in graphs, must not overlap on the GPU (order them with events).
 fork and compact move pages in place and return a cache with a new table; the old
-one must not be used after them.
+one must not be used after them (but see fork, where the pool is too small).
 There is no fallback: without the CUDA library the calls fail.
 """
 from __future__ import annotations
@@ -194,7 +194,9 @@ class KV4Cache:
 
     def fork(self, source: torch.Tensor, new_len: torch.Tensor) -> "KV4Cache":
         """New sequence s continues old sequence source[s] (-1: none) and has room for new_len[s] positions; old
-        sequences that none continues are freed.  A sequence that finds no room has length -1 afterwards."""
+        sequences that none continues are freed.  The first sequence that finds no room and all after it have length -1
+        afterwards.  Then this cache can be forked again, before anything is appended, with fewer or smaller requests
+        that continue no more of a sequence; the first result is void."""
         device = self.device
         if _current_device() != device:
             with torch.cuda.device(device):

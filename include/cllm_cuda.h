@@ -439,8 +439,13 @@ int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int
  * whole; every other one gets a copy, made in all n_layers layers.  Free pages
  * are those no new sequence holds, given out lowest id first in order of s.  A
  * sequence that finds no room (or whose new_len needs more than max_pages
- * pages, or whose source is out of range) gets len_out -1 and no pages; what
- * the first kind continued counts as held in this call.
+ * pages, or whose source is out of range) gets len_out -1 and no pages.  The
+ * first that finds no room ends the giving out: all after it get len_out -1 too,
+ * whatever they ask for, so put those that must not fail first.  What they
+ * continued counts as held in this call, which writes to free pages only: before
+ * anything is appended, the old table can be forked again in place of the result,
+ * with fewer or smaller requests that continue no more of a source than this
+ * call's.
  * table_out and len_out may not be page_table and seq_len; page_bytes: of one
  * page of one layer, a multiple of 16. */
 int cllm_cuda_kv4_fork(void* pages, int n_layers, int n_pages, int64_t page_bytes, int page_len,

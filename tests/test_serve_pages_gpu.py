@@ -53,3 +53,37 @@ def test_fork_and_compact_carry_a_page_outside_the_pool_along(cuda, lib, pool, b
     o = packed.attention(0, torch.randn(4, 64, device="cuda"))
     assert lib.cllm_cuda_check_device_status() == _lib.ERR_INVALID_ARG
     assert torch.isnan(o[:2]).all() and torch.isfinite(o[2:]).all()
+
+
+@pytest.mark.parametrize("slots", [16, 20000])  # one launch, four launches
+def test_fork_without_room_for_all_can_be_made_again(cuda, lib, slots):
+    """The first request that finds no room takes what comes after it along, even what needs no page; the old
+    sequences are still whole and can be forked anew."""
+    rng = np.random.default_rng(slots)
+    cache, pages, table = _cache(rng, 2, 16, 16, 1, 64, [40, 48, 20, 7], slots)  # 3 + 3 + 2 + 1 pages, 7 free
+    lens = [40, 48, 20, 7]
+    source, want = [3, 0, 0, 1, 2], [8, 41 + 16 * 5, 41, 48, 21]  # s 1 needs 5, s 2 a copy, the others nothing
+    new = cache.fork(_ints(*source), _ints(*want))
+    assert new.lens.tolist() == [8, 121, 41, 48, 21]  # 6 of 7
+    want[1] += 32
+    table_want, lens_want, _ = O.fork(table, lens, source, want, 16, 16)
+    new = cache.fork(_ints(*source), _ints(*want))
+    assert new.lens.tolist() == lens_want.tolist() == [8, 153, -1, -1, -1]  # all 7: s 2's copy has no page
+    want[1] += 16
+    table_want, lens_want, _ = O.fork(table, lens, source, want, 16, 16)
+    new = cache.fork(_ints(*source), _ints(*want))
+    assert new.lens.tolist() == lens_want.tolist() == [8, -1, -1, -1, -1]  # 8
+    assert (new.table[1:] == -1).all() and torch.equal(new.table, torch.from_numpy(table_want).cuda())
+    # again, the small ones first
+    source, want = [0, 3, 2, 1, 0], [41, 8, 21, 48, 41 + 16 * 5]
+    table_want, lens_want, copies = O.fork(table, lens, source, want, 16, 16)
+    new = cache.fork(_ints(*source), _ints(*want))
+    assert new.lens.tolist() == lens_want.tolist() == want
+    assert torch.equal(new.table, torch.from_numpy(table_want).cuda())
+    have = new.pages.cpu().numpy()
+    for s, old in enumerate(source):
+        for layer in range(2):
+            for x, y in zip(O.sequence(have[layer], table_want[s], lens[old], 64),
+                            O.sequence(pages[layer], table[old], lens[old], 64)):
+                np.testing.assert_array_equal(x, y)
+    _lib.check(lib.cllm_cuda_check_device_status())

@@ -456,6 +456,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
     const uint8_t *pro_a = nullptr, *pro_b = nullptr;  // no second tile: nullptr
     int pro_i = 0, pro_n = 0;
     Stage put, get;
+    bool alive = true;  // no wait has expired
     auto place = [&](int tile) -> const uint8_t* {
         const int slot = a.page_of(tile);
         const int id = a.c.page(pro.s, slot);
@@ -485,7 +486,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
             refill();
             if (pro_n == 0) return;
         }
-        if (lane == pro_i) {
+        if (lane == pro_i && alive) {
             const uint32_t bar = full + 8 * put.i, to = ring + put.i * (2 * Tile<HD>::kBytes);
             const bool two = pro_b != nullptr;
             mbar_arrive_expect_tx(bar, two ? 2 * Tile<HD>::kBytes : Tile<HD>::kBytes);
@@ -498,7 +499,6 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
 #pragma unroll 1
     for (int i = 0; i < kRowStages; ++i) produce();
 
-    bool alive = true;
     const uint32_t at_k = keep(tile_pos(0, r) * (HD / 2) + t * (HD / 8));                             // keys' numbers
     const uint32_t at_m = keep(Tile<HD>::kScaleK + tile_pos(0, r) * (HD / 8) + t * 4);                // word (d, m) t
     const uint32_t at_d0 = keep(Tile<HD>::kScaleK + (4 * t + (t >> 1)) * (HD / 8));                   // scale rows of
@@ -585,7 +585,11 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
         for (int i = step0; i < step1; ++i) {
             const int p0 = (i * kRowWarps + warp) * kPairLen;
             if (p0 >= cur.w.len) break;  // and so are the warp's further tiles
-            if (alive) alive = wait_full(full + 8 * get.i, get.parity);
+            if (alive && !wait_full(full + 8 * get.i, get.parity)) {
+                // no copies from here on; those in flight have to land before the CTA ends
+                for (Stage s = get; s.i != put.i || s.parity != put.parity; s.next()) wait_full(full + 8 * s.i, s.parity);
+                alive = false;
+            }
             const uint32_t pair = ring + get.i * (2 * Tile<HD>::kBytes);
             get.next();
             // ---- scores of positions 4t .. 4t+3 of both tiles for row r
@@ -863,8 +867,6 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
         __syncthreads();
         cur.next(a, units, limit_at);
     }
-    if (!alive)  // let the copies in flight land before the CTA ends
-        for (; get.i != put.i || get.parity != put.parity; get.next()) wait_full(full + 8 * get.i, get.parity);
 }
 
 }  // namespace serve

@@ -308,7 +308,7 @@ int cllm_cuda_kv4_fork(void* pages, int n_layers, int n_pages, int64_t page_byte
     if (n_new == 0) return CLLM_OK;
     if (!pages || !page_table || !seq_len || !source || !new_len || !table_out || !len_out)
         return host_fail(CLLM_ERR_INVALID_ARG, "kv4_fork: null argument");
-    if (table_out == page_table || len_out == seq_len)
+    if (table_out == page_table || len_out == seq_len || len_out == source || len_out == new_len)
         return host_fail(CLLM_ERR_INVALID_ARG, "kv4_fork: the new table and lengths need buffers of their own");
     PagesArgs a{};
     a.n_layers = n_layers; a.n_pages = n_pages; a.page_len = page_len; a.max_pages = max_pages;

@@ -446,8 +446,8 @@ int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int
  * anything is appended, the old table can be forked again in place of the result,
  * with fewer or smaller requests that continue no more of a source than this
  * call's.
- * table_out and len_out may not be page_table and seq_len; page_bytes: of one
- * page of one layer, a multiple of 16. */
+ * table_out may not be page_table, nor len_out seq_len, source or new_len;
+ * page_bytes: of one page of one layer, a multiple of 16. */
 int cllm_cuda_kv4_fork(void* pages, int n_layers, int n_pages, int64_t page_bytes, int page_len,
                        const int* page_table, const int* seq_len, int n_old, const int* source, const int* new_len,
                        int n_new, int max_pages, int* table_out, int* len_out, void* stream);

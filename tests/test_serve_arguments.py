@@ -1,0 +1,19 @@
+"""Arguments of the serving operators that the first refusal tests (test_serve.py) leave out; no GPU."""
+import ctypes
+
+import pytest
+
+from cllm_inference_b200 import _lib
+
+
+def _at(i):
+    return ctypes.c_void_p(256 * i)
+
+
+@pytest.mark.parametrize("alias", ["source", "new_len"])
+def test_fork_refuses_lengths_written_over_its_request(lib, alias):
+    """Every CTA of the one-launch form reads the request while others write the lengths."""
+    request = {"source": _at(4), "new_len": _at(5)}
+    rc = lib.cllm_cuda_kv4_fork(_at(1), 1, 4, 1280, 16, _at(2), _at(3), 1, request["source"], request["new_len"], 1, 1,
+                                _at(6), request[alias], None)
+    assert rc == _lib.ERR_INVALID_ARG and "buffers of their own" in _lib.last_error()

@@ -332,7 +332,7 @@ int cllm_cuda_kv4_compact(void* pages, int n_layers, int n_pages, int64_t page_b
 int cllm_cuda_token_scores(const float* logits, int64_t ld, int rows, int vocab, const int* tokens, int top_k,
                            float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprobs,
                            void* stream) {
-    if (rows < 0 || vocab <= 0 || ld < vocab) return host_fail(CLLM_ERR_INVALID_ARG, "token_scores: bad sizes");
+    if (rows < 0 || vocab <= 0 || (ld < vocab && ld != 0)) return host_fail(CLLM_ERR_INVALID_ARG, "token_scores: bad sizes");
     if (top_k < 0 || top_k > CLLM_MAX_TOP_K || top_k > vocab)
         return host_fail(CLLM_ERR_INVALID_ARG, "token_scores: top_k %d (0 to %d, at most the vocabulary)", top_k,
                          CLLM_MAX_TOP_K);

@@ -25,7 +25,7 @@ class TokenScores(NamedTuple):
 
 
 def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, top_k: int = 0) -> TokenScores:
-    """Scores of fp32 CUDA logits [rows][vocab] (any row stride) and int32 tokens of one device, on torch's
+    """Scores of fp32 CUDA logits [rows][vocab] (rows apart or one expanded) and int32 tokens of one device, on torch's
     current stream of it."""
     device = logits.get_device()
     if device < 0 or logits.dtype != torch.float32 or logits.dim() != 2 or (

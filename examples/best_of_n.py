@@ -105,7 +105,7 @@ def best_of_n(model: Model, prompt, n: int = 8, steps: int = 32, keep: int = 2, 
 
     cache = cache.fork(torch.zeros(n, dtype=torch.int32, device="cuda"),
                        torch.full((n,), length, dtype=torch.int32, device="cuda"))
-    logits = logits.expand(n, -1).contiguous()
+    logits = logits.expand(n, -1)
     tokens, scores = [], []
     for step in range(steps):
         top = token_scores(logits, None, top_k)

@@ -460,7 +460,8 @@ int cllm_cuda_kv4_compact(void* pages, int n_layers, int n_pages, int64_t page_b
                           const int* page_table, const int* seq_len, int n_seqs, int max_pages, int* table_out,
                           int* n_live, void* stream);
 
-/* What a sampler reports of `rows` rows of logits (row stride ld): with p =
+/* What a sampler reports of `rows` rows of logits (row stride ld; 0: one row
+ * stands for all): with p =
  * softmax(row), logprob[r] = log p[tokens[r]]; rank[r] = how many entries come
  * before the token in the order of (logit descending, index ascending);
  * entropy[r] = -sum p log p; top_ids, top_logprobs [rows][top_k]: the first

@@ -17,3 +17,13 @@ def test_fork_refuses_lengths_written_over_its_request(lib, alias):
     rc = lib.cllm_cuda_kv4_fork(_at(1), 1, 4, 1280, 16, _at(2), _at(3), 1, request["source"], request["new_len"], 1, 1,
                                 _at(6), request[alias], None)
     assert rc == _lib.ERR_INVALID_ARG and "buffers of their own" in _lib.last_error()
+
+
+def test_scores_take_one_row_for_all(lib):
+    """A row stride of 0 (an expanded row) is an argument like any other: it gets past the sizes."""
+    def call(ld, logits=_at(1)):
+        return lib.cllm_cuda_token_scores(logits, ld, 2, 100, None, 0, None, _at(2), None, None, None, None)
+
+    assert call(0, None) == _lib.ERR_INVALID_ARG and "null argument" in _lib.last_error()
+    for ld in (-100, -1, 1, 99):
+        assert call(ld) == _lib.ERR_INVALID_ARG and "bad sizes" in _lib.last_error()

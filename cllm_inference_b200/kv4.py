@@ -86,7 +86,7 @@ class KV4Cache:
         _ready(table, _I32, "table", device)
         _ready(lens, _I32, "lens", device)
         shape, slots = pages.shape, table.shape
-        if len(shape) != 5 or len(slots) != 2 or lens.shape[0] != slots[0] or shape[4] not in (1280, 2560):
+        if len(shape) != 5 or len(slots) != 2 or lens.shape != slots[:1] or shape[4] not in (1280, 2560):
             _refuse("pages [layer][page][kv head][page_len/16][20 head_dim], table [sequence][slot], lens [sequence]")
         self.lib = _lib.load()
         self.pages, self.table, self.lens = pages, table, lens

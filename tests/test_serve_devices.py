@@ -129,3 +129,10 @@ def test_tensors_of_another_device_are_refused(calls):
             call()
         assert e.value.code == _lib.ERR_INVALID_ARG, n
     assert not calls
+
+
+@pytest.mark.parametrize("shape", [(), (2,), (3, 1), (3, 7)])
+def test_lengths_of_another_shape_are_refused(calls, shape):
+    with pytest.raises(_lib.CudaError) as e:
+        cache(lens=ints(*shape))
+    assert e.value.code == _lib.ERR_INVALID_ARG

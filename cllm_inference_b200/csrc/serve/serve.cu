@@ -164,7 +164,7 @@ int cllm_cuda_kv4_append(const float* q, int64_t ldq, float* q_out, const float*
                          const int* token_pos, void* pages, int n_pages, int page_len, int n_head_kv, int head_dim,
                          const int* page_table, int n_seqs, int max_pages, float* k_out, float* v_out, void* stream) {
     if (int rc = check_geometry("kv4_append", n_pages, page_len, n_head_kv, head_dim)) return rc;
-    if (n_tok < 0 || n_head < 0 || n_seqs <= 0 || max_pages <= 0 || (rope_table && n_pos <= 0))
+    if (n_tok < 0 || n_head < 0 || n_seqs < (n_tok > 0) || max_pages <= 0 || (rope_table && n_pos <= 0))
         return host_fail(CLLM_ERR_INVALID_ARG, "kv4_append: bad sizes");
     if (n_tok == 0) return CLLM_OK;
     if (!k || !v || !token_seq || !token_pos || !pages || !page_table || (n_head > 0 && (!q || !q_out)))
@@ -207,7 +207,7 @@ int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int
                             const int* seq_len, int n_seqs, int max_pages, float scale, float* out, float* lse,
                             void* stream) {
     if (int rc = check_geometry("kv4_attention", n_pages, page_len, n_head_kv, head_dim)) return rc;
-    if (n_tok < 0 || n_head <= 0 || n_head % n_head_kv || n_seqs <= 0 || max_pages <= 0 ||
+    if (n_tok < 0 || n_head <= 0 || n_head % n_head_kv || n_seqs < (n_tok > 0) || max_pages <= 0 ||
         (int64_t)max_pages * page_len > INT_MAX || !(std::fabs(scale) <= 3e38f))
         return host_fail(CLLM_ERR_INVALID_ARG, "kv4_attention: bad sizes (%d heads over %d KV heads)", n_head, n_head_kv);
     if (!q_begin && n_tok != n_seqs)
@@ -304,7 +304,7 @@ static int pages_call(const char* who, PagesArgs a, void* pages, int64_t page_by
 int cllm_cuda_kv4_fork(void* pages, int n_layers, int n_pages, int64_t page_bytes, int page_len,
                        const int* page_table, const int* seq_len, int n_old, const int* source, const int* new_len,
                        int n_new, int max_pages, int* table_out, int* len_out, void* stream) {
-    if (n_old <= 0 || n_new < 0) return host_fail(CLLM_ERR_INVALID_ARG, "kv4_fork: bad sizes");
+    if (n_old < (n_new > 0) || n_new < 0) return host_fail(CLLM_ERR_INVALID_ARG, "kv4_fork: bad sizes");
     if (n_new == 0) return CLLM_OK;
     if (!pages || !page_table || !seq_len || !source || !new_len || !table_out || !len_out)
         return host_fail(CLLM_ERR_INVALID_ARG, "kv4_fork: null argument");

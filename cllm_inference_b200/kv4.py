@@ -206,6 +206,9 @@ class KV4Cache:
         n = source.numel()
         if new_len.numel() != n:
             _refuse("source and new_len have one entry per new sequence")
+        if self.n_seqs == 0 and n > 0:  # the C call wants an old sequence: an empty one that no source names
+            one = self._with(self.table.new_zeros((1, self.max_pages)), self.lens.new_zeros(1), 1)
+            return one.fork(torch.where(source < 0, source, 1), new_len)
         table = torch.empty_like(self.table) if n == self.n_seqs else self.table.new_empty((n, self.max_pages))
         lens = torch.empty_like(new_len)
         rc = self.lib.cllm_cuda_kv4_fork(
@@ -222,6 +225,8 @@ class KV4Cache:
         if _current_device() != device:
             with torch.cuda.device(device):
                 return self.compact()
+        if self.n_seqs == 0:
+            return self, self.lens.new_zeros(1)
         table = torch.empty_like(self.table)
         live = self.lens.new_empty(1)
         rc = self.lib.cllm_cuda_kv4_compact(

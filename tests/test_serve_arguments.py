@@ -27,3 +27,20 @@ def test_scores_take_one_row_for_all(lib):
     assert call(0, None) == _lib.ERR_INVALID_ARG and "null argument" in _lib.last_error()
     for ld in (-100, -1, 1, 99):
         assert call(ld) == _lib.ERR_INVALID_ARG and "bad sizes" in _lib.last_error()
+
+
+def test_nothing_to_do_for_no_sequences(lib):
+    """A batch whose sequences have all left has no rows: no error, as for no rows of some sequences."""
+    P = _at(1)
+
+    def append(n, seqs):
+        return lib.cllm_cuda_kv4_append(P, 256, P, P, P, 256, n, 2, None, 0, P, P, P, 4, 16, 2, 128, P, seqs, 1, None,
+                                        None, None)
+
+    def attention(n, seqs):
+        return lib.cllm_cuda_kv4_attention(P, 512, P, n, 4, P, 4, 16, 2, 128, P, P, seqs, 2, 0.0, P, None, None)
+
+    for call in (append, attention):
+        assert call(0, 0) == 0 and call(0, 1) == 0
+        for n, seqs in ((1, 0), (0, -1), (-1, 0)):
+            assert call(n, seqs) == _lib.ERR_INVALID_ARG and "bad sizes" in _lib.last_error()

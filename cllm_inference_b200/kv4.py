@@ -54,10 +54,11 @@ def _ready(t: torch.Tensor, dtype, what: str, device: int) -> None:
 
 def _rows(t: torch.Tensor, what: str, device: int) -> tuple[int, int, int]:
     """(rows, values in a row, row stride) of a 2-D fp32 tensor whose rows are dense."""
-    if t.dtype is not _F32 or t.get_device() != device or t.dim() != 2:
+    steps = t.stride()
+    if len(steps) != 2 or t.dtype is not _F32 or t.get_device() != device:
         _refuse(f"{what} must be a 2-D fp32 tensor with dense rows on cuda:{device}")
     n, width = t.shape
-    ld, step = t.stride()
+    ld, step = steps
     if step != 1 and width > 1:
         _refuse(f"{what} must be a 2-D fp32 tensor with dense rows on cuda:{device}")
     return n, width, ld if n > 1 else width

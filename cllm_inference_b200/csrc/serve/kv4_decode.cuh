@@ -742,6 +742,9 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
             }
             // ---- p . (m / 2 + 4 d): column 2g of the product, lanes of an even r
             if (!edge) {
+                // twice of it where k > 0: small m may be subnormal, and half of one is not exact
+                const uint32_t twice = d_up > kOne ? 0x04000400u : 0u;
+                const __half2 by_d = bits_h2(0x44004400u + twice), by_m = bits_h2(0x38003800u + twice);  // 4 and 1/2
                 float chi[4], clo[4];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
@@ -750,8 +753,8 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                     for (int k = 0; k < 2; ++k) {  // (d, m) of group r / 2 at the positions of the lane's operand
                         const uint32_t row = pair + u * Tile<HD>::kBytes + kToV + k * kTwo + (r >> 1) * 4;
                         const uint32_t w0 = G == 4 || r < 4 ? lds32(row + at_d0) : 0u, w1 = G == 4 || r < 4 ? lds32(row + at_d1) : 0u;
-                        sum2(__hmul2(bits_h2(__byte_perm(w0, w1, 0x5410)), __float2half2_rn(4.f)),
-                             __hmul2(bits_h2(__byte_perm(w0, w1, 0x7632)), __float2half2_rn(0.5f)), &hi[k], &lo[k]);
+                        sum2(__hmul2(bits_h2(__byte_perm(w0, w1, 0x5410)), by_d),
+                             __hmul2(bits_h2(__byte_perm(w0, w1, 0x7632)), by_m), &hi[k], &lo[k]);
                     }
                     if (u == 0) {
                         mma16816_zero(chi, ph[u][0], pl[u][0], ph[u][1], pl[u][1], hi[0], hi[1]);
@@ -761,7 +764,7 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
                         mma16816(clo, ph[u][0], pl[u][0], ph[u][1], pl[u][1], lo[0], lo[1]);
                     }
                 }
-                om += (chi[0] + chi[2]) + (clo[0] + clo[2]);
+                om = fmaf(twice ? 0.5f : 1.f, (chi[0] + chi[2]) + (clo[0] + clo[2]), om);
             }
             // ---- (p d) . (n - 8)
             uint32_t v[2][2][G];

@@ -24,9 +24,10 @@ RAISED = 17.5  # nats by which the position stands out
 SINK = 3       # where it is
 
 
-def _cache(rng, hd, kv, n, size):
+def _cache(rng, hd, kv, n, size, digits=False):
     """One sequence of n positions, keys and values with numbers at random; the values (mean 0.1, deviation 0.1, times
-    `size`) of the position that dominates are small.  Returns the cache, its pages and table, and the direction of
+    `size`) of the position that dominates are small.  With `digits` the values' scales are whole numbers (the
+    minimum's odd) of fp16's last digit instead.  Returns the cache, its pages and table, and the direction of
     queries that the dominating key answers to."""
     from cllm_inference_b200.kv4 import KV4Cache
 
@@ -44,21 +45,25 @@ def _cache(rng, hd, kv, n, size):
     for at, up in zip(O.k_nibble(SINK, np.arange(hd), hd), side):
         b = first[:, at // 2]
         first[:, at // 2] = (b & 0x0F) | (0xF0 if up else 0) if at & 1 else (b & 0xF0) | (0x0F if up else 0)
+    if digits:
+        s[..., 1, :, :, 0] = rng.integers(1, 201, s.shape[:4] + s.shape[5:7]) * 2.0 ** -24
+        s[..., 1, :, :, 1] = (rng.integers(-1000, 1001, s.shape[:4] + s.shape[5:7]) * 2 + 1) * 2.0 ** -24
     p[..., 16 * hd:] = s.reshape(*p.shape[:4], -1).view(np.uint8)
     c = KV4Cache(torch.from_numpy(p).cuda(), torch.from_numpy(table).cuda(),
                  torch.tensor([n], dtype=torch.int32, device="cuda"))
     return c, p, table, 2.0 * side - 1.0
 
 
-def _check(hd, kv, rep, rows, n, size):
+def _check(hd, kv, rep, rows, n, size, digits=False):
     rng = np.random.default_rng(hd + rows + n)
-    cache, p, table, side = _cache(rng, hd, kv, n, size)
+    cache, p, table, side = _cache(rng, hd, kv, n, size, digits)
     heads = kv * rep
     q = (1.5 * rng.standard_normal((rows, heads, hd)) + 2 * side).astype(np.float32)
     begin = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
     o, lse = cache.attention(0, torch.from_numpy(q.reshape(rows, -1)).cuda(), begin=begin, lse=True)
     o, lse = o.cpu().numpy().astype(np.float64).reshape(rows, heads, hd), lse.cpu().numpy().astype(np.float64)
     k, v = O.sequence(p[0], table[0], n, hd)
+    largest = 200 * 2.0 ** -24 if digits else 0.0217 * size  # of the values' scales
     worst = 0.0
     for row in sorted({0, rows // 3, rows // 2, rows - 1}):
         sees = n - (rows - 1 - row)
@@ -73,7 +78,7 @@ def _check(hd, kv, rep, rows, n, size):
             want = w @ vv
             terms = np.abs(kk) @ np.abs(qq) / np.sqrt(hd)
             tol = (w * (2.0 ** -17 * terms + 2.0 ** -18)) @ np.abs(vv - want) + 2.0 ** -17 * (w @ np.abs(vv))
-            tol += 6 * np.sqrt(sees) * 2.0 ** -24 / np.sqrt(12) * 4.7 * 8 * 0.0217 * size / 1024
+            tol += 6 * np.sqrt(sees) * 2.0 ** -24 / np.sqrt(12) * 4.7 * 8 * largest / 1024
             worst = max(worst, float((np.abs(o[row, h] - want) / tol).max()))
             assert abs(lse[row, h] - (m + np.log(total))) <= 2.0 ** -17 * (1 + (w * terms).sum())
     assert worst <= 1, f"{worst:.3g} of the tolerance"
@@ -92,4 +97,11 @@ def test_small_weights_beside_a_dominating_position_prompts(cuda, lib, hd, kv, r
                                               (64, 1, 1, 1, 100000)])
 def test_small_weights_beside_a_dominating_position_one_row(cuda, lib, hd, kv, rep, rows, n, size):
     _check(hd, kv, rep, rows, n, size)
+    _lib.check(lib.cllm_cuda_check_device_status())
+
+
+@pytest.mark.parametrize("hd,kv,rep,rows,n", [(128, 1, 4, 1, 8000), (64, 2, 2, 1, 8000), (128, 2, 2, 160, 8000),
+                                              (64, 2, 2, 160, 8000)])
+def test_values_of_a_few_of_fp16s_last_digits(cuda, lib, hd, kv, rep, rows, n):
+    _check(hd, kv, rep, rows, n, 1.0, digits=True)
     _lib.check(lib.cllm_cuda_check_device_status())

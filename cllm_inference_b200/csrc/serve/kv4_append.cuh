@@ -14,8 +14,10 @@
 // page, position and rotation are looked up once for them, and four vectors'
 // loads are issued together; with few tokens span is 1.  2048 tokens of 32 query
 // and 8 + 8 key and value vectors of 128, all written out: 28.7 us, 3.6 TB/s (56 %
-// of a copy's rate); the warps wait for their first loads, which depend on the
-// token's page.  One token: 5 us on the GPU.
+// of a copy's rate).  The warps wait for loads: the vectors', whose addresses are
+// known from the start, are issued only once the token's sequence and position, and for
+// keys and values its page, are there to say whether they are wanted.  One token: 5 us
+// on the GPU.
 #pragma once
 #include <type_traits>
 

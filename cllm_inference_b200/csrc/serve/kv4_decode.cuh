@@ -5,11 +5,12 @@
 // with 4 * rep * head_dim operations a position: the HBM stream, were it not for
 // the instructions.  At 6.4 TB/s an SM gets a tile of 16 positions every 110
 // cycles (head_dim 128), in which its four schedulers issue 440 instructions: the
-// numbers must reach the tensor cores with very few of them.  This takes 500 a
-// tile (8 rows), and with the 12 warps that its registers allow the schedulers
-// issue in half of the cycles: 64 sequences of 150 to 8190 positions, 64 heads
-// over 8, 67.6 us, 2.5 TB/s; one of 131071, 32 over 8, 67 us, 2.5 TB/s (38 % of
-// a copy's rate).
+// numbers must reach the tensor cores with very few of them.  This takes 520 a
+// tile (8 rows), and the schedulers issue in half of the cycles: each warp is one
+// chain of loads, conversions, products and weights, and the registers that it
+// holds allow three warps a scheduler.  64 sequences of 150 to 8190 positions, 64
+// heads over 8, 67.8 us, 2.5 TB/s; one of 131071, 32 over 8, 67.7 us, 2.5 TB/s
+// (38 % of a copy's rate).
 //
 // * Numbers become fp16 two at a time: (w & 0x000F000F) | 0x64006400 is the pair
 //   (1024 + n, 1024 + n'), and one fused operation takes the 1024 off (and the 16
@@ -23,10 +24,11 @@
 //   is m_g, met by sum(q)_g).  sum p v = (p d) . (n - 8) + p . (m + 8 d): around the
 //   middle of the numbers, because p d n alone adds up to many times the result
 //   and every instruction cuts off towards zero; m + 8 d is an exact fp16 pair.
-// * fp32 accuracy.  The query rows (and p, p d) enter as fp16 hi + lo in the two
-//   halves of the instruction's 16 rows, 22 bits together: with at most 8 rows of
-//   one KV head the second half would be empty anyway.  hi and lo of p d come from
-//   three fp16 operations: hi = p_hi d, lo = fma(p_lo, d, fma(p_hi, d, -hi)).
+// * The bits of fp32.  The query rows (and p, p d) enter as fp16 hi + lo in the two
+//   halves of the instruction's 16 rows, 22 bits together, rounded to the nearest:
+//   with at most 8 rows of one KV head the second half would be empty anyway.  hi
+//   and lo of p d come from three fp16 operations: hi = p_hi d, lo = fma(p_lo, d,
+//   fma(p_hi, d, -hi)).  Of the last digits of small ones see below.
 // * The tensor cores add up the 32 positions of a step only; their sums are added
 //   to the result in fp32, rounded to nearest.
 // * No number changes lanes.  The tile's order gives each lane its operands of a
@@ -36,9 +38,12 @@
 //   score exceeds it by 2^14, so the accumulators are hardly ever rescaled.
 // * The values' scales get a power of two, which the accumulators carry, that brings
 //   the largest one so far below 2 and to 2^-3 or more: a p of at most 2^14 then keeps
-//   p d inside fp16, and p d is off by 2^-25 at most where p of the largest weight is 2^10
-//   or more, so small weights count beside a dominating one however small the values
-//   are.  Scales of 2^-3 to 2 need no power and take no time.
+//   p d inside fp16.  fp16's last digit is 2^-24, so beside a largest weight of 2^10 or
+//   more a p is off by 2^-35 of it at most, beyond its 22 bits, and a p d by that much of
+//   a scale of 1: small weights count beside a dominating one however small the values
+//   are.  Scales of 2^-3 to 2 need no power and take no time.  One position 17.5 nats
+//   above 8000 others, of small value: off by 9e-7 of the output's largest value (fp32
+//   arithmetic 6e-7), and by 3e-6 where the values are of 0.0004.
 // * Work: steps of 128 positions of (sequence, KV head, 8 rows), numbered through
 //   (and some for the item itself) and cut into equal runs, one per CTA,
 //   whatever the lengths are.  A CTA's four

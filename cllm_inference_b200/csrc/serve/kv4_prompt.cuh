@@ -2,9 +2,11 @@
 // (cllm_cuda_kv4_attention; prompts): a CTA takes 128 rows (tokens x heads of one
 // KV head) over all the positions they see, 64 at a time, on tcgen05 tensor cores.
 //
-// fp32 accuracy from fp16 operands: q, k, p and v enter as hi + lo (22 bits
+// The bits of fp32 from fp16 operands: q, k, p and v enter as hi + lo (22 bits
 // together), and a product is lo*hi + hi*lo + hi*hi, in that order, the small
-// terms first because the tensor cores cut off as they add.  For the same reason
+// terms first because the tensor cores cut off as they add.  lo*lo is left out:
+// up to 2^-21 of a product, with a sign of its own since q and p are split to the
+// nearest.  For the same reason
 // a tile's p v is not accumulated in TMEM over the whole sequence but added to
 // fp32 registers, rounded to nearest, tile by tile; that also does the rescaling.
 // k and v of a tile are scaled by a power of two that brings its largest value to
@@ -12,7 +14,9 @@
 // The values' stays in the fp32 sums, of weights as of weighted values, and a
 // tile's rescaling brings them to its power: p is not touched by it, and the largest
 // weight is 2^10 to 2^14 whatever the values are, so a weight keeps its 22 bits down to
-// 2^-12 of it and is no further off than 2^-35 below that.
+// 2^-12 of it and is no further off than 2^-35 of it below that.  One position 17.5
+// nats above 8000 others, of small value: off by 8e-7 of the output's largest value
+// (fp32 arithmetic 6e-7).
 //
 // What bounds it: three products a term, 6 * 128 * 64 * HD multiply-adds a tile
 // for 128 x 64 scores: 1536 cycles of the tensor cores (HD 128), beside which the
@@ -21,9 +25,11 @@
 // from the numbers: q and p come from TMEM, or the operands alone would take all
 // of its bandwidth.  A tile takes 3600 cycles, in which the schedulers issue 59 %
 // of what they could and the tensor cores work 44 %: 1024 tokens of 32 heads over
-// 8 on 8000 positions 425 to 429 us, 294 TFLOP/s counted once, three times that in
-// products (52 % of a plain bf16 GEMM's rate).  Each role is busy some 70 % of the
-// time and waits for the others in turn.
+// 8 on 8000 positions 417 to 428 us, 294 to 301 TFLOP/s counted once, three times
+// that in products (53 % of a plain bf16 GEMM's rate).  Each role is busy some 70 %
+// of the time and waits for the others in turn.  Most instructions turn keys and
+// values into operands, which every CTA does for its own 128 rows: here 32 CTAs do
+// the same ones.
 //
 // Work: tiles of (sequence, KV head, 128 rows), numbered through by
 // prompt_plan_kernel and cut into equal runs, one per SM; a run that ends inside an

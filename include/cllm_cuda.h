@@ -422,8 +422,9 @@ int cllm_cuda_kv4_append(const float* q, int64_t ldq, float* q_out, const float*
  * lse (NULL: none): [n_tok][n_head], log(sum(exp(scale * q.k))).  A row that
  * sees nothing, or belongs to no sequence, gets out = 0 and lse = -inf.
  * out is 16-byte aligned.  scale 0: 1 / sqrt(head_dim).  n_head: any multiple
- * of n_head_kv.  Products
- * are taken on tensor cores with fp32 accuracy. */
+ * of n_head_kv.  Sums are fp32; products are taken on tensor cores, of pairs of
+ * fp16 numbers (22 bits): about fp32 arithmetic's errors.  A weight is off by
+ * 2^-35 of its row's largest at most beyond those bits. */
 int cllm_cuda_kv4_attention(const float* q, int64_t ldq, const int* q_begin, int n_tok, int n_head, const void* pages,
                             int n_pages, int page_len, int n_head_kv, int head_dim, const int* page_table,
                             const int* seq_len, int n_seqs, int max_pages, float scale, float* out, float* lse,

@@ -747,8 +747,9 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) kv4_rows_kernel(co
             }
             // ---- p . (m / 2 + 4 d): column 2g of the product, lanes of an even r
             if (!edge) {
-                // twice of it where k > 0: small m may be subnormal, and half of one is not exact
-                const uint32_t twice = d_up > kOne ? 0x04000400u : 0u;
+                // twice of it where k >= 0 (d is below 2, so m + 8 d rounds to a finite number): m may be subnormal, and
+                // half of one is not exact
+                const uint32_t twice = d_up >= kOne ? 0x04000400u : 0u;
                 const __half2 by_d = bits_h2(0x44004400u + twice), by_m = bits_h2(0x38003800u + twice);  // 4 and 1/2
                 float chi[4], clo[4];
 #pragma unroll

@@ -24,10 +24,10 @@ RAISED = 17.5  # nats by which the position stands out
 SINK = 3       # where it is
 
 
-def _cache(rng, hd, kv, n, size, digits=False):
+def _cache(rng, hd, kv, n, size, digits="", raised=RAISED):
     """One sequence of n positions, keys and values with numbers at random; the values (mean 0.1, deviation 0.1, times
-    `size`) of the position that dominates are small.  With `digits` the values' scales are whole numbers (the
-    minimum's odd) of fp16's last digit instead.  Returns the cache, its pages and table, and the direction of
+    `size`) of the position that dominates are small.  digits "all": the values' scales are whole numbers (the minimum's
+    odd) of fp16's last digit instead; "one": those of the position that dominates.  Returns the cache, its pages and table, and the direction of
     queries that the dominating key answers to."""
     from cllm_inference_b200.kv4 import KV4Cache
 
@@ -39,31 +39,35 @@ def _cache(rng, hd, kv, n, size, digits=False):
     table = rng.permutation(slots).astype(np.int32)[None]
     first = p[0, table[0, 0], :, 0]
     side = rng.integers(0, 2, hd)
-    size_k = RAISED / 2 / np.sqrt(hd)
+    size_k = raised / 2 / np.sqrt(hd)
     s[0, table[0, 0], :, 0, 0, SINK] = 2 * size_k / 15, -size_k
     s[0, table[0, 0], :, 0, 1, SINK] = 0.0217 * size / 128, -0.0625 * size / 128
     for at, up in zip(O.k_nibble(SINK, np.arange(hd), hd), side):
         b = first[:, at // 2]
         first[:, at // 2] = (b & 0x0F) | (0xF0 if up else 0) if at & 1 else (b & 0xF0) | (0x0F if up else 0)
     if digits:
-        s[..., 1, :, :, 0] = rng.integers(1, 201, s.shape[:4] + s.shape[5:7]) * 2.0 ** -24
-        s[..., 1, :, :, 1] = (rng.integers(-1000, 1001, s.shape[:4] + s.shape[5:7]) * 2 + 1) * 2.0 ** -24
+        shape = s.shape[:4] + s.shape[5:7]
+        few = np.stack([rng.integers(1, 201, shape), rng.integers(-1000, 1001, shape) * 2 + 1], -1) * 2.0 ** -24
+        if digits == "all":
+            s[..., 1, :, :, :] = few
+        else:
+            s[0, table[0, 0], :, 0, 1, SINK] = few[0, table[0, 0], :, 0, SINK]
     p[..., 16 * hd:] = s.reshape(*p.shape[:4], -1).view(np.uint8)
     c = KV4Cache(torch.from_numpy(p).cuda(), torch.from_numpy(table).cuda(),
                  torch.tensor([n], dtype=torch.int32, device="cuda"))
     return c, p, table, 2.0 * side - 1.0
 
 
-def _check(hd, kv, rep, rows, n, size, digits=False):
+def _check(hd, kv, rep, rows, n, size, digits="", raised=RAISED):
     rng = np.random.default_rng(hd + rows + n)
-    cache, p, table, side = _cache(rng, hd, kv, n, size, digits)
+    cache, p, table, side = _cache(rng, hd, kv, n, size, digits, raised)
     heads = kv * rep
     q = (1.5 * rng.standard_normal((rows, heads, hd)) + 2 * side).astype(np.float32)
     begin = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
     o, lse = cache.attention(0, torch.from_numpy(q.reshape(rows, -1)).cuda(), begin=begin, lse=True)
     o, lse = o.cpu().numpy().astype(np.float64).reshape(rows, heads, hd), lse.cpu().numpy().astype(np.float64)
     k, v = O.sequence(p[0], table[0], n, hd)
-    largest = 200 * 2.0 ** -24 if digits else 0.0217 * size  # of the values' scales
+    largest = 200 * 2.0 ** -24 if digits == "all" else 0.0217 * size  # of the values' scales
     worst = 0.0
     for row in sorted({0, rows // 3, rows // 2, rows - 1}):
         sees = n - (rows - 1 - row)
@@ -103,5 +107,13 @@ def test_small_weights_beside_a_dominating_position_one_row(cuda, lib, hd, kv, r
 @pytest.mark.parametrize("hd,kv,rep,rows,n", [(128, 1, 4, 1, 8000), (64, 2, 2, 1, 8000), (128, 2, 2, 160, 8000),
                                               (64, 2, 2, 160, 8000)])
 def test_values_of_a_few_of_fp16s_last_digits(cuda, lib, hd, kv, rep, rows, n):
-    _check(hd, kv, rep, rows, n, 1.0, digits=True)
+    _check(hd, kv, rep, rows, n, 1.0, digits="all")
+    _lib.check(lib.cllm_cuda_check_device_status())
+
+
+@pytest.mark.parametrize("hd,kv,rep,rows,n", [(128, 2, 4, 1, 48), (64, 4, 4, 1, 48), (128, 40, 1, 160, 300),
+                                              (64, 40, 1, 160, 300)])
+def test_a_dominating_value_of_a_few_of_fp16s_last_digits(cuda, lib, hd, kv, rep, rows, n):
+    """Beside others with scales of 0.3, so that the cache as a whole needs no power of two."""
+    _check(hd, kv, rep, rows, n, 14.0, digits="one", raised=25.0)
     _lib.check(lib.cllm_cuda_check_device_status())
